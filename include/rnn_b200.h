@@ -12,7 +12,8 @@
  *     device-side error flags);
  *   - the plain-named entry points take HOST pointers, mirror the reference's
  *     Rust signatures, copy in, run, copy out and synchronise.
- * All tensors are f32, row-major / NCHW exactly as in the reference.
+ * All tensors are f32, row-major / NCHW exactly as in the reference; the
+ * entries that take a dtype also take bf16 tensors and explicit strides.
  * Gradients accumulate (+=) wherever the reference accumulates.
  *
  * A context owns one CUDA stream and a growable device workspace.  Calls on
@@ -35,6 +36,10 @@ extern "C" {
 #define RNN_ERR_DEVICE -4  /* a kernel raised its device error word (timeout) */
 #define RNN_ERR_UNSUPPORTED -5
 #define RNN_ERR_IO -6       /* a checkpoint file could not be read or written */
+
+/* element types of the entries that take a dtype */
+#define RNN_F32 0
+#define RNN_BF16 1
 
 typedef struct rnn_ctx rnn_ctx;
 typedef struct rnn_resnet rnn_resnet;
@@ -286,6 +291,75 @@ int rnn_kl_distill_dev(rnn_ctx *ctx, const float *student, const float *teacher,
 /* hint_mse (loss.rs:133-151): dz accumulates. */
 int rnn_hint_mse_dev(rnn_ctx *ctx, const float *pred, const float *target,
                      int n, int c, float scale, float *dz, float *loss_out);
+
+/* ---- rotary positions (no reference counterpart: its attention has a
+ * relative-position bias only) ---------------------------------------------- */
+/* y = R x for x [rows, heads, dh] (dtype), strides xrow / xhead in elements,
+ * columns contiguous.  pos [rows, axes] holds each token's integer coordinates
+ * (1 to 4 axes: time, height, width, ...); axis a owns the next pairs[a] (host
+ * array) pairs of every head's columns, and with total = sum of pairs,
+ * 2*total <= dh, pair p turns by the angle pos[row, axis(p)] * inv_freq[p]
+ * (inv_freq [total], f32):
+ *   y_i = x_i cos - x_j sin,  y_j = x_i sin + x_j cos,
+ * (i, j) = (p, p + total), or (2p, 2p + 1) when interleaved.  Columns from
+ * 2*total on are copied.  backward != 0 turns by the negative angle: the
+ * gradient of x from that of y.  Angles are exact to f32 at any position;
+ * the rotation is f32, rounded once to dtype.  y may be x with the same
+ * strides; otherwise they must not share elements. */
+int rnn_rope_dev(rnn_ctx *ctx, int dtype, const void *x, long long xrow,
+                 long long xhead, int rows, int heads, int dh,
+                 const int32_t *pos, int axes, const int *pairs,
+                 const float *inv_freq, int interleaved, int backward, void *y,
+                 long long yrow, long long yhead);
+
+/* ---- differential attention (no reference counterpart) ------------------- */
+/* Shape, strides (in elements; columns contiguous) and masks of one call.
+ * A head's queries and keys are two halves of dh columns, q = [q1 | q2],
+ * k = [k1 | k2]; its values and outputs are 2*dh wide.  Query head e reads
+ * key head e / (h / hkv).  q [n, tq, h, 2*dh], k and v [n, tk, hkv, 2*dh],
+ * o [n, tq, h, 2*dh].
+ * Key j of sequence b is visible to query i when j < klen[b] (klen NULL: tk;
+ * values are clamped to [0, tk]), kmask[b * kmask_batch + j] != 0 (kmask
+ * NULL: all), and
+ *   causal RNN_CAUSAL_START: j <= i          (query i sits at key i),
+ *   causal RNN_CAUSAL_END:   j <= i + klen[b] - tq  (the last query sits at
+ *                            the last key: new tokens against a cache).
+ * Keys and values that klen or kmask hides may hold anything. */
+#define RNN_CAUSAL_NONE 0
+#define RNN_CAUSAL_START 1
+#define RNN_CAUSAL_END 2
+typedef struct rnn_diffattn {
+  int dtype, causal;
+  int n, h, hkv, dh, tq, tk;
+  float scale; /* of the scores, e.g. 1/sqrt(dh) */
+  int reserved; /* 0 */
+  long long q_batch, q_row, q_head;
+  long long k_batch, k_row, k_head;
+  long long v_batch, v_row, v_head;
+  long long o_batch, o_row, o_head;
+  const int32_t *klen;  /* [n] device, or NULL */
+  const uint8_t *kmask; /* [n, tk] device, or NULL */
+  long long kmask_batch;
+} rnn_diffattn;
+/* s_m = scale q_m k_m^T and P_m = softmax(s_m) over the visible keys, m = 1, 2;
+ * o = (P_1 - lambda[head] P_2) v.  lambda [h] f32.  A query that sees no key
+ * gets 0.  For the backward pass, o2 (dtype, contiguous [n, tq, h, 2*dh]; P_2 v)
+ * and lse (f32, [n, h, 2, tq]: log2 of each map's sum of exponentials, +inf
+ * for a query that sees no key) are written when non-NULL, both or neither.
+ * No score matrix is stored.  dh in 1 .. 64. */
+int rnn_diffattn_fwd_dev(rnn_ctx *ctx, const rnn_diffattn *d, const void *q,
+                         const void *k, const void *v, const float *lambda,
+                         void *o, void *o2, float *lse);
+/* Gradients from dout and the forward's o, o2 and lse: dq, dk, dv are written,
+ * dlambda [h] (f32) accumulates.  The q, k, v and o strides of g are those of
+ * dq, dk, dv and dout (nothing else of g is read); g NULL: those of d.
+ * Deterministic. */
+int rnn_diffattn_bwd_dev(rnn_ctx *ctx, const rnn_diffattn *d,
+                         const rnn_diffattn *g, const void *q, const void *k,
+                         const void *v, const float *lambda,
+                         const void *o, const void *o2, const float *lse,
+                         const void *dout, void *dq, void *dk, void *dv,
+                         float *dlambda);
 
 /* ---- host-pointer tier of the attention / norm / optimiser entries -------
  * Same arguments as the _dev entries above, on host memory: the call stages

@@ -25,6 +25,11 @@ pub const RNN_ERR_DEVICE: c_int = -4;
 pub const RNN_ERR_UNSUPPORTED: c_int = -5;
 pub const RNN_ERR_IO: c_int = -6;
 pub const RNN_UID_BYTES: usize = 128;
+pub const RNN_F32: c_int = 0;
+pub const RNN_BF16: c_int = 1;
+pub const RNN_CAUSAL_NONE: c_int = 0;
+pub const RNN_CAUSAL_START: c_int = 1;
+pub const RNN_CAUSAL_END: c_int = 2;
 
 #[repr(C)]
 pub struct RnnCtx {
@@ -41,6 +46,36 @@ pub struct RnnRustvit {
 #[repr(C)]
 pub struct RnnComm {
     _p: [u8; 0],
+}
+
+/// Shape, strides (elements) and masks of a differential attention call.
+#[repr(C)]
+pub struct RnnDiffAttn {
+    pub dtype: c_int,
+    pub causal: c_int,
+    pub n: c_int,
+    pub h: c_int,
+    pub hkv: c_int,
+    pub dh: c_int,
+    pub tq: c_int,
+    pub tk: c_int,
+    pub scale: f32,
+    pub reserved: c_int,
+    pub q_batch: i64,
+    pub q_row: i64,
+    pub q_head: i64,
+    pub k_batch: i64,
+    pub k_row: i64,
+    pub k_head: i64,
+    pub v_batch: i64,
+    pub v_row: i64,
+    pub v_head: i64,
+    pub o_batch: i64,
+    pub o_row: i64,
+    pub o_head: i64,
+    pub klen: *const i32,
+    pub kmask: *const u8,
+    pub kmask_batch: i64,
 }
 
 extern "C" {
@@ -106,6 +141,9 @@ extern "C" {
     pub fn rnn_ce_soft_dev(ctx: *mut RnnCtx, logits: *const f32, target: *const f32, hard: *const u32, n: c_int, nclass: c_int, scale: f32, dz: *mut f32, loss_out: *mut f32, correct_out: *mut c_int) -> c_int;
     pub fn rnn_kl_distill_dev(ctx: *mut RnnCtx, student: *const f32, teacher: *const f32, n: c_int, nclass: c_int, temp: f32, scale: f32, dz: *mut f32, loss_out: *mut f32) -> c_int;
     pub fn rnn_hint_mse_dev(ctx: *mut RnnCtx, pred: *const f32, target: *const f32, n: c_int, c: c_int, scale: f32, dz: *mut f32, loss_out: *mut f32) -> c_int;
+    pub fn rnn_rope_dev(ctx: *mut RnnCtx, dtype: c_int, x: *const c_void, xrow: i64, xhead: i64, rows: c_int, heads: c_int, dh: c_int, pos: *const i32, axes: c_int, pairs: *const c_int, inv_freq: *const f32, interleaved: c_int, backward: c_int, y: *mut c_void, yrow: i64, yhead: i64) -> c_int;
+    pub fn rnn_diffattn_fwd_dev(ctx: *mut RnnCtx, d: *const RnnDiffAttn, q: *const c_void, k: *const c_void, v: *const c_void, lambda: *const f32, o: *mut c_void, o2: *mut c_void, lse: *mut f32) -> c_int;
+    pub fn rnn_diffattn_bwd_dev(ctx: *mut RnnCtx, d: *const RnnDiffAttn, g: *const RnnDiffAttn, q: *const c_void, k: *const c_void, v: *const c_void, lambda: *const f32, o: *const c_void, o2: *const c_void, lse: *const f32, dout: *const c_void, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, dlambda: *mut f32) -> c_int;
     pub fn rnn_attn_fwd(ctx: *mut RnnCtx, n: c_int, h: c_int, dh: c_int, th: c_int, tw: c_int, mh: c_int, mw: c_int, mask_diag: c_int, q: *const f32, qstride: c_int, qoff: c_int, kv: *const f32, kvstride: c_int, koff: c_int, voff: c_int, tau: *const f32, rel: *const f32, p: *mut f32, o: *mut f32) -> c_int;
     pub fn rnn_attn_bwd(ctx: *mut RnnCtx, n: c_int, h: c_int, dh: c_int, th: c_int, tw: c_int, mh: c_int, mw: c_int, q: *const f32, qstride: c_int, qoff: c_int, kv: *const f32, kvstride: c_int, koff: c_int, voff: c_int, tau: *const f32, p: *const f32, dout: *const f32, dq: *mut f32, dkv: *mut f32, dtau: *mut f32, drel: *mut f32) -> c_int;
     pub fn rnn_layernorm_fwd(ctx: *mut RnnCtx, x: *const f32, rows: c_int, c: c_int, gamma: *const f32, beta: *const f32, eps: f32, y: *mut f32, xhat: *mut f32, invstd: *mut f32) -> c_int;

@@ -40,6 +40,20 @@ CTX = C.POINTER(_CtxS)
 NET = C.POINTER(_NetS)
 VIT = C.POINTER(_VitS)
 
+RNN_F32, RNN_BF16 = 0, 1
+
+
+class DiffAttn(C.Structure):
+    """rnn_diffattn: shape, strides and masks of a differential attention call."""
+
+    _fields_ = ([(f, C.c_int) for f in ("dtype", "causal", "n", "h", "hkv", "dh", "tq", "tk")]
+                + [("scale", C.c_float), ("reserved", C.c_int)]
+                + [(f"{t}_{f}", C.c_longlong) for t in "qkvo" for f in ("batch", "row", "head")]
+                + [("klen", C.c_void_p), ("kmask", C.c_void_p), ("kmask_batch", C.c_longlong)])
+
+
+LL = C.c_longlong
+
 # name -> argtypes; every function returns int unless listed in _RESTYPE
 SIGS = {
     "rnn_device_ok": [I],
@@ -117,6 +131,9 @@ SIGS = {
     "rnn_ce_soft_dev": [CTX, FP, FP, FP, I, I, F, FP, FP, FP],
     "rnn_kl_distill_dev": [CTX, FP, FP, I, I, F, F, FP, FP],
     "rnn_hint_mse_dev": [CTX, FP, FP, I, I, F, FP, FP],
+    "rnn_rope_dev": [CTX, I, FP, LL, LL, I, I, I, P, I, P, FP, I, I, FP, LL, LL],
+    "rnn_diffattn_fwd_dev": [CTX, C.POINTER(DiffAttn), FP, FP, FP, FP, FP, FP, FP],
+    "rnn_diffattn_bwd_dev": [CTX, C.POINTER(DiffAttn), C.POINTER(DiffAttn), FP, FP, FP, FP, FP, FP, FP, FP, FP, FP, FP, FP],
     "rnn_attn_fwd": [CTX, I, I, I, I, I, I, I, I, FP, I, I, FP, I, I, I, FP, FP, FP, FP],
     "rnn_attn_bwd": [CTX, I, I, I, I, I, I, I, FP, I, I, FP, I, I, I, FP, FP, FP, FP, FP, FP, FP],
     "rnn_layernorm_fwd": [CTX, FP, I, I, FP, FP, F, FP, FP, FP],

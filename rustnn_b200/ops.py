@@ -1,7 +1,7 @@
 """Operator-level API over the C ABI, mirroring the reference's Rust calls.
 
 Tensors are torch CUDA float32 tensors (torch is used only for device memory
-and streams).  Every op runs on the current torch stream, through a context
+and streams); rope and diffattn also take bfloat16 and strided views.  Every op runs on the current torch stream, through a context
 bound to it, and raises ``RnnError`` on any failure; there is no CPU path.
 
 Reference interfaces mirrored here:
@@ -18,7 +18,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import CTX, RnnError, call, check, lib
+from ._lib import CTX, RNN_BF16, RNN_F32, DiffAttn, RnnError, call, check, lib
 
 __all__ = [
     "Context", "default_context", "matmul", "gemm_small", "matmul_dw", "conv2d_forward", "conv2d_dgrad",
@@ -28,6 +28,7 @@ __all__ = [
     "linear_backward", "layernorm_res_forward", "linear_forward_packed", "swiglu_fused_forward", "newton_schulz_", "muon_step_", "adamw_step_", "clip_", "ema_update_",
     "layerscale_forward", "layerscale_backward", "swiglu_forward", "swiglu_backward", "dwconv3_forward",
     "dwconv3_backward", "seqpool_forward", "seqpool_backward", "droppath_forward_", "droppath_backward_",
+    "rope", "rope_backward", "diffattn_forward", "diffattn_backward",
     "token_merge", "tok_layout", "taxo_forward_", "taxo_backward", "ce_soft", "kl_distill", "hint_mse",
 ]
 
@@ -259,6 +260,140 @@ def attn_backward(n, h, dh, th, tw, mh, mw, q, qstride, qoff, kv, kvstride, koff
     call("rnn_attn_bwd_dev", _ctx_of(q, ctx), n, h, dh, th, tw, mh, mw, _ptr(q, "q"), qstride, qoff, _ptr(kv, "kv"),
          kvstride, koff, voff, _ptr(tau, "tau"), _ptr(p, "p"), _ptr(dout, "dout"), _ptr(dq, "dq"), _ptr(dkv, "dkv"),
          _ptr(dtau, "dtau"), _ptr(drel, "drel"))
+
+
+# ---------------------------------------------------------------- rotary positions, differential attention
+
+
+_DTYPES = {torch.float32: RNN_F32, torch.bfloat16: RNN_BF16}
+
+
+def _view(t, name, shape, like=None):
+    """Checks a float32 or bfloat16 CUDA tensor of the given shape (None: any
+    extent) with contiguous columns; of the type and device of `like`."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DTYPES:
+        raise RnnError(f"{name}: expected a CUDA float32 or bfloat16 tensor")
+    if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+        raise RnnError(f"{name}: shape {tuple(t.shape)}, expected {tuple('*' if w is None else w for w in shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise RnnError(f"{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise RnnError(f"{name}: columns must be contiguous")
+    return C.c_void_p(t.data_ptr())
+
+
+def _plain(t, name, dtypes, shape, device):
+    """Checks a contiguous tensor of one of the types and the given shape."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != device:
+        raise RnnError(f"{name}: expected a {' or '.join(str(d) for d in dtypes)} tensor on {device}")
+    if tuple(t.shape) != tuple(shape):
+        raise RnnError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise RnnError(f"{name}: tensor must be contiguous")
+    return C.c_void_p(t.data_ptr())
+
+
+def _rope(x, pos, inv_freq, pairs, interleaved, backward, out, ctx):
+    xp = _view(x, "x", (None, None, None))
+    rows, heads, dh = x.shape
+    pairs = tuple(int(p) for p in pairs)
+    pp = _plain(pos, "pos", (torch.int32,), (rows, len(pairs)), x.device)
+    fp = _plain(inv_freq, "inv_freq", (torch.float32,), (sum(pairs),), x.device)
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    yp = _view(out, "out", x.shape, x)
+    call("rnn_rope_dev", _ctx_of(x, ctx), _DTYPES[x.dtype], xp, x.stride(0), x.stride(1), rows, heads, dh, pp,
+         len(pairs), (C.c_int * len(pairs))(*pairs), fp, int(bool(interleaved)), int(backward), yp, out.stride(0),
+         out.stride(1))
+    return out
+
+
+def rope(x, pos, inv_freq, pairs, interleaved=False, out=None, ctx=None):
+    """Rotary positions over 1 to 4 axes.
+
+    x [rows, heads, dh] (float32 or bfloat16, any row and head strides); pos
+    [rows, axes] int32, the tokens' coordinates (time, height, width, ...);
+    axis a owns pairs[a] pairs of every head's columns, and pair p turns by
+    pos[:, axis(p)] * inv_freq[p] (inv_freq [sum(pairs)] float32).  Pair p is
+    the columns (p, p + sum(pairs)), or (2p, 2p + 1) when interleaved; columns
+    from 2 * sum(pairs) on stay.  out=x rotates in place."""
+    return _rope(x, pos, inv_freq, pairs, interleaved, 0, out, ctx)
+
+
+def rope_backward(dy, pos, inv_freq, pairs, interleaved=False, out=None, ctx=None):
+    """Gradient of rope's x from that of its output (the inverse rotation)."""
+    return _rope(dy, pos, inv_freq, pairs, interleaved, 1, out, ctx)
+
+
+_CAUSAL = {None: 0, "start": 1, "end": 2}
+
+
+def _diffattn(q, k, v, lam, o, scale, causal, klen, kmask):
+    """Checks a differential attention call; (description, pointers of q, k, v, lam, o)."""
+    qp = _view(q, "q", (None, None, None, None))
+    n, tq, h, w = q.shape
+    kp = _view(k, "k", (n, None, None, w), q)
+    tk, hkv = k.shape[1:3]
+    vp = _view(v, "v", (n, tk, hkv, w), q)
+    op = _view(o, "out", q.shape, q)
+    lp = _plain(lam, "lam", (torch.float32,), (h,), q.device)
+    if w % 2 or w == 0:
+        raise RnnError(f"q: {w} columns, expected two halves")
+    if causal not in _CAUSAL:
+        raise RnnError(f"causal: {causal!r}, expected None, 'start' or 'end'")
+    d = DiffAttn(_DTYPES[q.dtype], _CAUSAL[causal], n, h, hkv, w // 2, tq, tk,
+                 (w // 2) ** -0.5 if scale is None else scale, 0,
+                 *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
+    if klen is not None:
+        d.klen = _plain(klen, "klen", (torch.int32,), (n,), q.device)
+    if kmask is not None:
+        d.kmask = _plain(kmask, "kmask", (torch.bool, torch.uint8), (n, tk), q.device)
+        d.kmask_batch = tk
+    return d, (qp, kp, vp, lp), op
+
+
+def diffattn_forward(q, k, v, lam, scale=None, causal=None, klen=None, kmask=None, save=False, out=None, ctx=None):
+    """Differential attention: (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v.
+
+    q [n, tq, h, 2*dh], k and v [n, tk, hkv, 2*dh] (float32 or bfloat16, any
+    strides, columns contiguous), q and k as two halves of dh <= 64 columns;
+    query head e reads key head e // (h // hkv).  lam [h] float32.  scale
+    defaults to 1/sqrt(dh).  Key j is visible to query i when j < klen[b]
+    (int32 [n]), kmask[b, j] (bool [n, tk]) and, for causal "start", j <= i, or
+    for "end", j <= i + klen[b] - tq (new tokens against a cache).  A query that
+    sees no key gets 0; hidden keys and values may hold anything.
+
+    Returns o [n, tq, h, 2*dh], or with save (o, o2, lse) for the backward."""
+    if out is None:
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if isinstance(q, torch.Tensor) else None
+    d, ptrs, op = _diffattn(q, k, v, lam, out, scale, causal, klen, kmask)
+    o2 = lse = None
+    if save:
+        o2 = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty((d.n, d.h, 2, d.tq), device=q.device, dtype=torch.float32)
+    call("rnn_diffattn_fwd_dev", _ctx_of(q, ctx), C.byref(d), *ptrs, op, None if o2 is None else o2.data_ptr(),
+         None if lse is None else lse.data_ptr())
+    return (out, o2, lse) if save else out
+
+
+def diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam, scale=None, causal=None, klen=None, kmask=None, dq=None,
+                      dk=None, dv=None, ctx=None):
+    """Gradients of diffattn_forward from its o, o2 and lse: returns (dq, dk,
+    dv), written; dlam [h] accumulates.  dout, dq, dk and dv may have strides of
+    their own (the parts of a fused projection's gradient, say); those of dq,
+    dk, dv that are not given are allocated."""
+    d, ptrs, op = _diffattn(q, k, v, lam, o, scale, causal, klen, kmask)
+    gp = _view(dout, "dout", o.shape, q)
+    o2p = _plain(o2, "o2", (q.dtype,), q.shape, q.device)
+    lsep = _plain(lse, "lse", (torch.float32,), (d.n, d.h, 2, d.tq), q.device)
+    dlp = _plain(dlam, "dlam", (torch.float32,), (d.h,), q.device)
+    grads = [torch.empty(t.shape, device=q.device, dtype=q.dtype) if g is None else g
+             for g, t in ((dq, q), (dk, k), (dv, v))]
+    gptrs = [_view(g, name, t.shape, q) for g, t, name in zip(grads, (q, k, v), ("dq", "dk", "dv"))]
+    gd = DiffAttn(d.dtype, d.causal, d.n, d.h, d.hkv, d.dh, d.tq, d.tk, d.scale, 0,
+                  *(x for t in (*grads, dout) for x in t.stride()[:3]))
+    call("rnn_diffattn_bwd_dev", _ctx_of(q, ctx), C.byref(d), C.byref(gd), *ptrs, op, o2p, lsep, gp, *gptrs, dlp)
+    return tuple(grads)
 
 
 # ---------------------------------------------------------------- norm.rs / linear.rs

@@ -1,0 +1,354 @@
+"""GPU parity of differential attention, forward and backward, against the
+definition in 64 bits (autograd of the plain formula), on the inputs as the
+kernels get them.
+
+Bounds (relative Frobenius per output).  f32: scores come from split-TF32
+products (2^-22) of magnitude up to about 8 in base 2, so a map entry is off by
+at most about 2^-20; subtracting the maps at most triples that: 1e-5.  bf16:
+rounding to 8 bits leaves a relative error of at most 2^-8, 2^-8 / sqrt(3) =
+2.3e-3 in the mean square; the combined map and the output are each rounded
+once, 3.2e-3 together; the gradients read D from saved outputs that were
+rounded once more: 5e-3.  dlam is summed in
+f32 either way: 4e-6 of the sum of the magnitudes of its terms."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+TOL = {torch.float32: 1e-5, torch.bfloat16: 5e-3}
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from rustnn_b200 import ops as _ops
+
+    return _ops
+
+
+def visible(n, tq, tk, causal, klen, kmask):
+    i, j = torch.arange(tq, device="cuda")[:, None], torch.arange(tk, device="cuda")[None]
+    length = (klen.long().clamp(0, tk) if klen is not None else torch.full((n,), tk, device="cuda"))[:, None, None]
+    see = (j < length).expand(n, tq, tk)
+    if causal == "start":
+        see = see & (j <= i)
+    elif causal == "end":
+        see = see & (j <= i + length - tq)
+    if kmask is not None:
+        see = see & kmask.bool()[:, None]
+    return see
+
+
+def reference(q, k, v, lam, dout, scale, causal=None, klen=None, kmask=None):
+    """o, P_2 v, dq, dk, dv, dlam and the magnitude of dlam's terms, in 64 bits."""
+    n, tq, h, w = q.shape
+    tk, hkv, dh = k.shape[1], k.shape[2], q.shape[3] // 2
+    see = visible(n, tq, tk, causal, klen, kmask)[:, None]
+    hidden = torch.zeros(n, tk, dtype=torch.bool, device="cuda") if tk == 0 else ~see.any(2)[:, 0]
+    # what no query sees may hold anything
+    k = k.double().masked_fill(hidden[:, :, None, None], 0.0)
+    v = v.double().masked_fill(hidden[:, :, None, None], 0.0)
+    q, lam = q.double().requires_grad_(), lam.double().requires_grad_()
+    k, v = k.requires_grad_(), v.requires_grad_()
+    rep = h // hkv
+    kk, vv = k.repeat_interleave(rep, 2).transpose(1, 2), v.repeat_interleave(rep, 2).transpose(1, 2)
+    qq = q.transpose(1, 2)
+    some = see.any(-1, keepdim=True) if tk else torch.zeros(n, 1, tq, 1, dtype=torch.bool, device="cuda")
+    bias = torch.zeros(see.shape, dtype=torch.float64, device="cuda").masked_fill(~see & some, -math.inf)
+    maps = [torch.softmax(qq[..., c] @ kk[..., c].transpose(-1, -2) * scale + bias, -1) * some
+            for c in (slice(0, dh), slice(dh, w))]
+    o2 = maps[1] @ vv
+    o = maps[0] @ vv - lam.view(1, h, 1, 1) * o2
+    grads = torch.autograd.grad(o, (q, k, v, lam), dout.double().transpose(1, 2), allow_unused=True)
+    grads = [torch.zeros_like(t) if g is None else g for g, t in zip(grads, (q, k, v, lam))]
+    dp = dout.double().transpose(1, 2) @ vv.transpose(-1, -2)
+    size = (maps[1] * dp.abs()).sum((0, 2, 3)).detach()
+    return [x.detach() for x in (o.transpose(1, 2), o2.transpose(1, 2), *grads, size)]
+
+
+def make(n, tq, tk, h, hkv, dh, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def r(*s):
+        return torch.randn(*s, device="cuda", generator=g).to(dtype)
+
+    lam = 0.2 + 0.6 * torch.rand(h, device="cuda", generator=g)
+    return r(n, tq, h, 2 * dh), r(n, tk, hkv, 2 * dh), r(n, tk, hkv, 2 * dh), lam, r(n, tq, h, 2 * dh)
+
+
+def rel(got, want):
+    d, s = float((got.double() - want).norm()), float(want.norm())
+    return d / s if s > 0 else d
+
+
+def run_all(ops, q, k, v, lam, dout, **how):
+    o, o2, lse = ops.diffattn_forward(q, k, v, lam, save=True, **how)
+    dlam = torch.zeros_like(lam)
+    dq, dk, dv = ops.diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam, **how)
+    return o, o2, lse, dq, dk, dv, dlam
+
+
+def check_all(ops, q, k, v, lam, dout, **how):
+    scale = how.get("scale") or (q.shape[-1] // 2) ** -0.5
+    want = reference(q, k, v, lam, dout, scale, how.get("causal"), how.get("klen"), how.get("kmask"))
+    o, o2, lse, dq, dk, dv, dlam = run_all(ops, q, k, v, lam, dout, **how)
+    # without the saved tensors the result is the same
+    assert torch.equal(ops.diffattn_forward(q, k, v, lam, **how), o)
+    tol = TOL[q.dtype]
+    for name, got, ref in zip(("o", "o2", "dq", "dk", "dv"), (o, o2, dq, dk, dv), want):
+        assert got.dtype == q.dtype
+        assert rel(got, ref) < tol, (name, rel(got, ref))
+    assert bool(((dlam.double() - want[5]).abs() <= 4e-6 * want[6] + 1e-30).all())
+    return o, lse
+
+
+SHAPES = [
+    # n, tq, tk, h, hkv, dh: one token up to several tiles, around the tile sizes, odd widths, shared key heads
+    (1, 1, 1, 1, 1, 8),
+    (2, 1, 5, 2, 1, 16),
+    (3, 7, 3, 2, 2, 4),
+    (2, 16, 16, 4, 2, 8),
+    (1, 31, 33, 1, 1, 32),
+    (2, 64, 64, 4, 4, 32),
+    (2, 65, 63, 3, 1, 24),
+    (1, 128, 129, 2, 2, 64),
+    (2, 100, 257, 6, 2, 40),
+    (1, 300, 300, 2, 1, 64),
+    (2, 50, 70, 2, 2, 1),
+    (2, 50, 70, 2, 2, 5),
+    (1, 77, 90, 3, 3, 33),
+    (1, 33, 1000, 8, 2, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [None, "start", "end"])
+@pytest.mark.parametrize("n,tq,tk,h,hkv,dh", SHAPES)
+def test_parity(ops, n, tq, tk, h, hkv, dh, causal, dtype):
+    check_all(ops, *make(n, tq, tk, h, hkv, dh, dtype, tq + tk + dh), causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [None, "start", "end"])
+@pytest.mark.parametrize("tq,tk", [(80, 200), (129, 129), (300, 90), (3, 500)])
+def test_lengths_and_masks_with_anything_hidden(ops, tq, tk, causal, dtype):
+    """Lengths from 0 to beyond tk, key masks that hide a whole sequence, and
+    NaN, infinities and the type's lowest value in every hidden key and value:
+    rows that see nothing are 0 with no gradient."""
+    n, h, hkv, dh = 6, 4, 2, 32
+    q, k, v, lam, dout = make(n, tq, tk, h, hkv, dh, dtype, 11)
+    klen = torch.tensor([0, 1, tk // 2, tk, tk - 1, tk + 7], dtype=torch.int32, device="cuda")
+    kmask = torch.rand(n, tk, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) < 0.7
+    kmask[3] = False
+    kmask[1, 0] = True
+    see = visible(n, tq, tk, causal, klen, kmask)
+    hidden = ~((torch.arange(tk, device="cuda")[None] < klen[:, None]) & kmask)
+    for i, bad in enumerate((math.nan, math.inf, -math.inf, torch.finfo(dtype).min)):
+        at = hidden & (torch.arange(tk, device="cuda")[None] % 4 == i)
+        k.masked_fill_(at[:, :, None, None], bad)
+        v.masked_fill_(at[:, :, None, None], bad)
+    how = dict(causal=causal, klen=klen, kmask=kmask)
+    o, lse = check_all(ops, q, k, v, lam, dout, **how)
+    none = ~see.any(-1)
+    assert bool((o[none] == 0).all())
+    assert bool(torch.isposinf(lse.permute(0, 3, 1, 2)[none]).all())
+    assert bool(torch.isfinite(lse.permute(0, 3, 1, 2)[~none]).all())
+    _, _, _, dq, dk, dv, _ = run_all(ops, q, k, v, lam, dout, **how)
+    assert bool((dq[none] == 0).all())
+    assert bool((dk[hidden] == 0).all()) and bool((dv[hidden] == 0).all())
+    # the same by a byte mask with the length written into it
+    both = ((torch.arange(tk, device="cuda")[None] < klen[:, None]) & kmask).to(torch.uint8) * 3
+    if causal != "end":
+        assert torch.equal(ops.diffattn_forward(q, k, v, lam, causal=causal, kmask=both), o)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_single_key_has_no_score_gradient(ops, dtype):
+    """One visible key: the maps are 1, o = (1 - lam) v, dq and dk are exactly 0."""
+    q, k, v, lam, dout = make(3, 5, 9, 2, 2, 16, dtype, 4)
+    klen = torch.ones(3, dtype=torch.int32, device="cuda")
+    _, _, _, dq, dk, _, _ = run_all(ops, q, k, v, lam, dout, klen=klen)
+    assert bool((dq == 0).all()) and bool((dk == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,tq,tk,h,hkv,dh", [(2, 1, 4097, 4, 1, 64), (1, 1, 20000, 2, 2, 32), (3, 2, 3001, 8, 1, 64),
+                                              (1, 5, 9000, 3, 1, 16), (2, 16, 2500, 1, 1, 40), (1, 40, 7000, 2, 2, 64)])
+def test_few_rows_over_a_long_cache(ops, n, tq, tk, h, hkv, dh, dtype):
+    """New tokens against a cache: the keys are split over blocks and joined."""
+    q, k, v, lam, dout = make(n, tq, tk, h, hkv, dh, dtype, tk)
+    check_all(ops, q, k, v, lam, dout, causal="end")
+    klen = torch.randint(1, tk, (n,), dtype=torch.int32, device="cuda",
+                         generator=torch.Generator(device="cuda").manual_seed(2))
+    klen[0] = 3
+    check_all(ops, q, k, v, lam, dout, causal="end", klen=klen)
+
+
+def test_large_scores(ops):
+    """Scores far apart, and maps whose sums differ by many orders: no overflow, no loss to the running ratio."""
+    q, k, v, lam, dout = make(2, 70, 300, 2, 2, 32, F32, 8)
+    check_all(ops, q, k, v, lam, dout, scale=2.0)
+    up = torch.linspace(-1, 1, 300, device="cuda")[None, :, None, None]
+    k2 = k.clone()
+    k2[..., 32:] = q[:, :1, :, 32:] * up * 3  # the second map moves to the late keys
+    check_all(ops, q, k2, v, lam, dout)
+    check_all(ops, q, k, v, lam, dout, scale=-0.2)
+    for value in (0.0, -0.5, 1.5):
+        check_all(ops, q, k, v, torch.full_like(lam, value), dout)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_maps_in_common_are_rounded_together(ops, dtype):
+    """Nearly equal maps: what is left of the difference keeps the type's precision."""
+    q, k, v, _, dout = make(2, 130, 200, 2, 2, 32, dtype, 9)
+    q[..., 32:], k[..., 32:] = q[..., :32], k[..., :32]
+    lam = torch.full((2,), 0.75, device="cuda")
+    want = reference(q, k, v, lam, dout, 32 ** -0.5)[0]
+    # o = P v / 4: off by the map's and the output's rounding alone in bf16; f32 subtracts terms 4 times o
+    assert rel(ops.diffattn_forward(q, k, v, lam), want) < (2.0 ** -8 if dtype == BF16 else 1e-5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_fused_projection_views(ops, dtype, shift):
+    """q, k, v and their gradients as parts of one buffer, at any alignment, and heads outermost."""
+    n, t, h, dh = 2, 90, 3, 32
+    g = torch.Generator(device="cuda").manual_seed(0)
+    base = torch.randn(n * t * 3 * h * 2 * dh + shift, device="cuda", generator=g).to(dtype)
+    qkv = base[shift:].view(n, t, 3, h, 2 * dh)
+    q, k, v = qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]
+    lam = torch.rand(h, device="cuda", generator=g)
+    dout = torch.randn(n, h, t, 2 * dh, device="cuda", generator=g).to(dtype).transpose(1, 2)
+    want = reference(q, k, v, lam, dout, dh ** -0.5, "start")
+    out = torch.empty(n, h, t, 2 * dh, device="cuda", dtype=dtype).transpose(1, 2)
+    o, o2, lse = ops.diffattn_forward(q, k, v, lam, causal="start", save=True, out=out)
+    assert o is out and rel(o, want[0]) < TOL[dtype]
+    dbase = torch.full_like(base, 7.0)
+    dqkv = dbase[shift:].view(n, t, 3, h, 2 * dh)
+    dlam = torch.ones(h, device="cuda")
+    got = ops.diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam, causal="start", dq=dqkv[:, :, 0],
+                                dk=dqkv[:, :, 1], dv=dqkv[:, :, 2])
+    for x, y in zip(got, want[2:5]):
+        assert rel(x, y) < TOL[dtype]
+    assert bool((dbase[:shift] == 7).all())
+    # dlam accumulates: 1 was there
+    assert bool(((dlam.double() - 1 - want[5]).abs() <= 4e-6 * want[6] + 1e-6).all())
+
+
+def test_broadcast_keys(ops):
+    """One memory for all sequences: k and v expanded (stride 0); the gradient comes per sequence."""
+    q, k, v, lam, dout = make(3, 40, 50, 2, 2, 16, F32, 2)
+    k, v = k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)
+    check_all(ops, q, k, v, lam, dout)
+
+
+def test_offsets_past_32_bits(ops):
+    """A cache whose rows lie more than 2^31 elements from its first."""
+    n, tq, tk, h, dh = 1, 1, 70, 1, 32
+    stride = 1 << 26
+    kb = torch.empty(tk * stride, device="cuda", dtype=BF16)
+    q, k, v, lam, dout = make(n, tq, tk, h, h, dh, BF16, 3)
+    kv = kb.as_strided((n, tk, h, 2 * dh), (0, stride, 0, 1))
+    vv = kb[64:].as_strided((n, tk, h, 2 * dh), (0, stride, 0, 1))
+    kv.copy_(k)
+    vv.copy_(v)
+    want = reference(q, k, v, lam, dout, dh ** -0.5)
+    assert rel(ops.diffattn_forward(q, kv, vv, lam), want[0]) < TOL[BF16]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_deterministic(ops, dtype):
+    args = make(2, 200, 333, 4, 2, 64, dtype, 6)
+    first = run_all(ops, *args, causal="end")
+    for _ in range(3):
+        for a, b in zip(first, run_all(ops, *args, causal="end")):
+            assert torch.equal(a, b)
+    q, k, v, lam, _ = make(1, 1, 9000, 4, 1, 64, dtype, 6)
+    assert torch.equal(ops.diffattn_forward(q, k, v, lam), ops.diffattn_forward(q, k, v, lam))
+
+
+def test_side_stream(ops):
+    args = make(2, 100, 100, 2, 2, 32, F32, 1)
+    want = run_all(ops, *args)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = run_all(ops, *args)
+    s.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_nothing_to_do(ops):
+    """No sequence, no query, no key."""
+    for n, tq, tk in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
+        q, k, v, lam, dout = make(n, tq, tk, 2, 1, 8, F32)
+        o, o2, lse, dq, dk, dv, dlam = run_all(ops, q, k, v, lam, dout)
+        assert o.shape == q.shape and not bool(o.any()) and not bool(dq.any())
+        assert not bool(dk.any()) and not bool(dv.any()) and not bool(dlam.any())
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "lam"])
+def test_gradient_against_differences(ops, which):
+    """Directional derivative of sum(o * dout): central differences of the f32
+    forward pass with step 1e-2 have a truncation error near 1e-4 and a rounding
+    error near 1e-5 of the terms summed; 5e-3 as the framework's other checks."""
+    q, k, v, lam, dout = make(2, 20, 45, 2, 1, 16, F32, 21)
+    how = dict(causal="end", klen=torch.tensor([45, 30], dtype=torch.int32, device="cuda"))
+    _, _, _, dq, dk, dv, dlam = run_all(ops, q, k, v, lam, dout, **how)
+    grad = {"q": dq, "k": dk, "v": dv, "lam": dlam}[which].double()
+    args = {"q": q, "k": k, "v": v, "lam": lam}
+    # along the gradient itself the derivative is its norm
+    step = grad / grad.norm()
+
+    def loss(e):
+        moved = dict(args)
+        moved[which] = (args[which].double() + e * step).float()
+        return float((ops.diffattn_forward(**moved, **how).double() * dout.double()).sum())
+
+    num = (loss(1e-2) - loss(-1e-2)) / 2e-2
+    assert abs(num - float(grad.norm())) / float(grad.norm()) < 5e-3
+
+
+def test_refusals(ops):
+    q, k, v, lam, dout = make(2, 8, 9, 4, 2, 16, F32)
+    f = ops.diffattn_forward
+    o, o2, lse = f(q, k, v, lam, save=True)
+    dlam = torch.zeros_like(lam)
+    wide = make(1, 2, 2, 1, 1, 65, F32)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    bad = [
+        lambda: f(q.half(), k.half(), v.half(), lam),
+        lambda: f(q, k.bfloat16(), v, lam),
+        lambda: f(q[0], k[0], v[0], lam),
+        lambda: f(q, k[:1], v[:1], lam),
+        lambda: f(q, k, v[:, :8], lam),
+        lambda: f(q[:, :, :3], k, v, lam[:3]),  # 3 heads over 2
+        lambda: f(q[..., :31], k[..., :31], v[..., :31], lam),
+        lambda: f(q.transpose(2, 3), k, v, lam),
+        lambda: f(q, k, v, lam[:2]),
+        lambda: f(q, k, v, lam.bfloat16()),
+        lambda: f(q, k, v, lam.cpu()),
+        lambda: f(q, k, v, lam, causal="both"),
+        lambda: f(q, k, v, lam, klen=torch.zeros(3, **i32)),
+        lambda: f(q, k, v, lam, klen=torch.zeros(2, device="cuda")),
+        lambda: f(q, k, v, lam, kmask=torch.ones(2, 8, dtype=torch.bool, device="cuda")),
+        lambda: f(q, k, v, lam, kmask=torch.ones(2, 9, device="cuda")),
+        lambda: f(q, k, v, lam, out=torch.empty_like(q)[:1].expand(2, -1, -1, -1)),
+        lambda: f(*wide[:4]),  # more than 64 columns a half
+        lambda: ops.diffattn_backward(dout[:1], q, k, v, lam, o, o2, lse, dlam),
+        lambda: ops.diffattn_backward(dout, q, k, v, lam, o, o2[:, :4], lse, dlam),
+        lambda: ops.diffattn_backward(dout, q, k, v, lam, o, o2, lse[:1], dlam),
+        lambda: ops.diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam[:1]),
+        lambda: ops.diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam, dk=torch.empty_like(q)),
+        lambda: ops.diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam,
+                                      dk=torch.empty_like(k)[:1].expand(2, -1, -1, -1)),
+    ]
+    for i, g in enumerate(bad):
+        with pytest.raises(ops.RnnError):
+            g()
+            pytest.fail(f"call {i} was not refused")
+    with pytest.raises(ops.RnnError, match="UNSUPPORTED"):
+        f(*wide[:4])
