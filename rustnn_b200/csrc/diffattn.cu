@@ -19,7 +19,7 @@
 // atomics: results do not depend on scheduling.
 #include <algorithm>
 
-#include "diffattn.cuh"
+#include "diffattn_tc.cuh"
 
 namespace rnn {
 namespace diff {
@@ -1143,7 +1143,8 @@ extern "C" int rnn_diffattn_fwd_dev(rnn_ctx* ctx, const rnn_diffattn* d, const v
   a.vec = a.dh % (16 / esz) == 0 && diff::aligned({q, k, v}, 16) &&
           diff::multiples({a.qb, a.qr, a.qh, a.kb, a.kr, a.kh, a.vb, a.vr, a.vh}, 16 / esz);
   a.pair = diff::multiples({a.ob, a.orow, a.oh}, 2) && diff::aligned({o}, 2 * esz);
-  return d->dtype == RNN_F32 ? diff::fwd_type<float>(ctx, a) : diff::fwd_type<__nv_bfloat16>(ctx, a);
+  if (d->dtype == RNN_F32) return diff::fwd_type<float>(ctx, a);
+  return diff::tc_fwd_ok(a) ? diff::tc_fwd(ctx, a) : diff::fwd_type<__nv_bfloat16>(ctx, a);
 }
 
 extern "C" int rnn_diffattn_bwd_dev(rnn_ctx* ctx, const rnn_diffattn* d, const rnn_diffattn* g, const void* q,

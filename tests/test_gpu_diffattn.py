@@ -352,3 +352,38 @@ def test_refusals(ops):
             pytest.fail(f"call {i} was not refused")
     with pytest.raises(ops.RnnError, match="UNSUPPORTED"):
         f(*wide[:4])
+
+
+@pytest.mark.parametrize("causal", [None, "start"])
+@pytest.mark.parametrize("second", [False, True])
+def test_scores_that_keep_rising(ops, second, causal):
+    """bf16 over several key tiles, each tile's scores far above those before
+    it (up to 2^400 in all), in one map or in both: the running references move
+    at every tile.  The scores themselves are exact to 2^-15 in f32, so the
+    bounds of the type hold for the outputs.  (Not for dq: its sum of dS k cancels
+    against the large column of k that all keys of a step have in common.)"""
+    n, t, h, dh = 1, 700, 2, 32
+    q, k, v, lam, dout = make(n, t, t, h, h, dh, BF16, 31)
+    step = (torch.arange(t, device="cuda") // 50).float()[None, :, None]
+    for half in ((0, 32) if second else (0,)):
+        q[..., half] = 8.0
+        k[..., half] = (step * 14).to(BF16)  # 8 * 14 / sqrt(32) = 20 more each 50 keys, 28 in base 2
+    want = reference(q, k, v, lam, dout, dh ** -0.5, causal)
+    o, o2, lse = ops.diffattn_forward(q, k, v, lam, causal=causal, save=True)
+    assert rel(o, want[0]) < TOL[BF16] and rel(o2, want[1]) < TOL[BF16]
+    assert bool(torch.isfinite(lse).all())
+
+
+def test_many_blocks_same_result(ops):
+    """More blocks than SMs, long rows, run after run the same bits, and the same as without the fast path's
+    conditions (a key mask that hides nothing) up to rounding."""
+    q, k, v, lam, _ = make(2, 2500, 2500, 16, 8, 64, BF16, 12)
+    first = ops.diffattn_forward(q, k, v, lam, causal="start", save=True)
+    for _ in range(8):
+        for a, b in zip(first, ops.diffattn_forward(q, k, v, lam, causal="start", save=True)):
+            assert torch.equal(a, b)
+    mask = torch.ones(2, 2500, dtype=torch.bool, device="cuda")
+    other = ops.diffattn_forward(q, k, v, lam, causal="start", kmask=mask, save=True)
+    row = (first[0].double() - other[0].double()).norm(dim=-1) / other[0].double().norm(dim=-1)
+    assert float(row.max()) < 2.0 ** -6  # two results, each within 2^-7 of every row
+    assert rel(first[2], other[2].double()) < 1e-6
