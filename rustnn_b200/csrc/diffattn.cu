@@ -1010,10 +1010,6 @@ int bwd_launch(rnn_ctx* ctx, Args a) {
   const long long qblocks = (rows + FQ::ROWS - 1) / FQ::ROWS * nbh;
   const long long kblocks = std::max<long long>((a.tk + FK::KEYS - 1ll) / FK::KEYS * nbh, a.h);
   RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
-  const size_t nrow = static_cast<size_t>(a.n) * a.h * a.tq;
-  RNN_TRY(ensure_ws(ctx, nrow * 3 * sizeof(float)));
-  a.dsum = static_cast<float*>(ctx->ws);
-  a.dlrow = a.dsum + 2 * nrow;
   RNN_TRY(allow_smem(bwd_q_kernel<T, DH>, FQ::SMEM));
   RNN_TRY(allow_smem(bwd_kv_kernel<T, DH>, FK::SMEM));
   if (qblocks > 0) {
@@ -1188,5 +1184,9 @@ extern "C" int rnn_diffattn_bwd_dev(rnn_ctx* ctx, const rnn_diffattn* d, const r
           diff::multiples({a.qb, a.qr, a.qh, a.kb, a.kr, a.kh, a.vb, a.vr, a.vh, a.gb, a.gr, a.gh}, 16 / esz);
   a.pair = a.dh % 2 == 0 && diff::aligned({dq, dk, dv}, 2 * esz) &&
            diff::multiples({a.dqb, a.dqr, a.dqh, a.dkb, a.dkr, a.dkh, a.dvb, a.dvr, a.dvh}, 2);
-  return d->dtype == RNN_F32 ? diff::bwd_type<float>(ctx, a) : diff::bwd_type<__nv_bfloat16>(ctx, a);
+  RNN_TRY(ensure_ws(ctx, nrow * 3 * sizeof(float)));
+  a.dsum = static_cast<float*>(ctx->ws);
+  a.dlrow = a.dsum + 2 * nrow;
+  if (d->dtype == RNN_F32) return diff::bwd_type<float>(ctx, a);
+  return diff::tc_bwd_ok(a) ? diff::tc_bwd(ctx, a) : diff::bwd_type<__nv_bfloat16>(ctx, a);
 }

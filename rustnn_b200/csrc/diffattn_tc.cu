@@ -86,7 +86,7 @@ struct alignas(64) FwdParams {
 };
 
 struct FwdShared {
-  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], clean, s1_full[2], s2_full[2], s1_free[2], p_full[2];
+  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], last_full, s1_full[2], s2_full[2], s1_free[2], p_full[2];
   uint64_t pv_last, o_full, tok[4], drain;
   uint32_t tmem;
   int abort_flag;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
       mbar_init(&sh.kv_full[i], 1);
       mbar_init(&sh.kv_empty[i], 1);
     }
-    mbar_init(&sh.clean, 1);
+    mbar_init(&sh.last_full, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh.s1_full[i], 1);
       mbar_init(&sh.s2_full[i], 1);
@@ -427,22 +427,25 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
           const int st = j % STAGES;
           if (j >= STAGES && !wait(&sh.kv_empty[st], (j / STAGES - 1) & 1, abort_flag, dev_error)) break;
           const uint32_t dst = skv + st * STAGE_BYTES;
-          mbar_arrive_expect_tx(&sh.kv_full[st], (2 + wide) * HALF_BYTES);
+          // a tile to be cleared lands for the clearing warp, which passes it on
+          uint64_t* bar = dirty && j == nt - 1 ? &sh.last_full : &sh.kv_full[st];
+          mbar_arrive_expect_tx(bar, (2 + wide) * HALF_BYTES);
           for (int half = 0; half < 2; half++)
-            tma_5d(dst + half * HALF_BYTES, &p.k, 0, half, kvh, j * KEYS, b, &sh.kv_full[st]);
+            tma_5d(dst + half * HALF_BYTES, &p.k, 0, half, kvh, j * KEYS, b, bar);
           for (int c = 0; c < wide; c++)
-            tma_5d(dst + (2 + c) * HALF_BYTES, &p.v, c * 64, 0, kvh, j * KEYS, b, &sh.kv_full[st]);
+            tma_5d(dst + (2 + c) * HALF_BYTES, &p.v, c * 64, 0, kvh, j * KEYS, b, bar);
         }
-        if (j < nt) {  // aborting: let the copies in flight land
-          settle(&sh.q_full, 0);
-          for (int i = max(0, j - STAGES); i < j; i++) settle(&sh.kv_full[i % STAGES], (i / STAGES) & 1);
-        }
+        // what was asked for lands before the block may end, aborting or not
+        settle(&sh.q_full, 0);
+        for (int t = max(0, j - STAGES); t < j; t++)
+          settle(dirty && t == nt - 1 ? &sh.last_full : &sh.kv_full[t % STAGES],
+                 dirty && t == nt - 1 ? 0 : (t / STAGES) & 1);
       }
       __syncwarp();
     } else if (warp == WARP_CLEAR) {
       if (dirty) {
         const int j = nt - 1, st = j % STAGES;
-        if (warp_wait(&sh.kv_full[st], (j / STAGES) & 1, abort_flag, dev_error)) {
+        if (warp_wait(&sh.last_full, 0, abort_flag, dev_error)) {
           // hidden values may be NaN: P = 0 there, so v has to be finite
           uint8_t* v = base + Q_BYTES + st * STAGE_BYTES + 2 * HALF_BYTES;
           for (int r = len - j * KEYS; r < KEYS; r++)
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
               *reinterpret_cast<uint4*>(v + (c >> 3) * HALF_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           fence_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.clean);
+          if (lane == 0) mbar_arrive(&sh.kv_full[st]);
         }
       }
     } else if (warp == WARP_MMA) {
@@ -469,9 +472,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
             if (ks < ksteps) mma_ss(d, q + ks * 2, k + ks * 2, id_s, ks > 0, lead);
           commit(half ? &sh.s2_full[j & 1] : &sh.s1_full[j & 1], lead);
         };
-        auto landed = [&](int j, int st) {
-          return done(&sh.kv_full[st], (j / STAGES) & 1) && (!(dirty && j == nt - 1) || done(&sh.clean, 0));
-        };
+        auto landed = [&](int j, int st) { return done(&sh.kv_full[st], (j / STAGES) & 1); };
         // products of tile j with v
         auto products = [&](int j, int st) {
           tc_fence_after();

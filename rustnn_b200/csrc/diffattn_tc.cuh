@@ -146,6 +146,12 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[16]) 
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // Two f32 operations in one instruction, on register pairs.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float x, float y) {
@@ -164,6 +170,12 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   f32x2 d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 
@@ -208,8 +220,12 @@ int encode_map(CUtensorMap* m, const void* base, int n, int t, int heads, int ha
 // Whether a view can be read so: 16-byte aligned, strides that a map can hold.
 bool map_ok(const void* base, int n, int t, int heads, int cols, long long sb, long long sr, long long sh);
 
+// Whether the tensor-core kernels take a call, and the calls themselves (the
+// backward's workspace pointers are set).
 bool tc_fwd_ok(const Args& a);
 int tc_fwd(rnn_ctx* ctx, const Args& a);
+bool tc_bwd_ok(const Args& a);
+int tc_bwd(rnn_ctx* ctx, const Args& a);
 
 }  // namespace diff
 }  // namespace rnn

@@ -1,0 +1,705 @@
+// Differential attention backward on tcgen05: bf16, halves of 16 .. 64 columns
+// (multiples of 8).  Two kernels, as in diffattn.cu: one owns 128 queries of a
+// head (dq, D_1, D_2, the row sums of P_2 dP), one owns 128 keys of a key head
+// (dk, dv).  Both form scores and dP = do v^T anew, 64 columns at a time, and
+// both are bound by the exponentials and the tensor cores about alike.
+//
+// 16 warps turn scores into dS, 16 columns of a row at a time: with the saved
+// log-sums no thread needs another's values, so a row is shared by four of
+// them.  Warp 16 copies tiles, warp 17 issues MMAs, warp 18 clears what lies
+// beyond a sequence's length (queries' kernel) or brings the queries' log-sums
+// and D (keys' kernel), warp 19 sums dlam.
+#include <algorithm>
+
+#include "diffattn_tc.cuh"
+
+namespace rnn {
+namespace diff {
+namespace {
+
+constexpr int THREADS = 640, SOFT = 16, WARP_COPY = 16, WARP_MMA = 17, WARP_AUX = 18, WARP_SUM = 19;
+constexpr int ROWS = 128, COLS = 64;               // a block's rows, a tile's columns
+constexpr uint32_t BIG = ROWS * 128, SMALL = COLS * 128;  // 64-column parts of a 128- and a 64-row tile, bytes
+
+struct alignas(64) Params {
+  CUtensorMap q, k, v, g;  // g: dout
+  Args a;
+  int* dev_error;
+  int st16;  // 16-byte stores of the gradients are aligned
+};
+
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+
+// 16 values times f to bf16 at p, the first n of them (a multiple of 8).
+__device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&v)[16], float f, bool on, int n, bool st16) {
+  uint32_t w[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) w[k] = on ? pack2(v[2 * k] * f, v[2 * k + 1] * f) : 0u;
+  if (st16) {
+    if (n > 0) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (n > 8) *reinterpret_cast<uint4*>(p + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; k++)
+      if (k < n) p[k] = __ushort_as_bfloat16(static_cast<unsigned short>(w[k >> 1] >> (16 * (k & 1))));
+  }
+}
+
+// ------------------------------------------------------------------ queries
+//
+// Tensor memory: dq_1 | dq_2 at [0, 128); S_1 | S_2 | dP of even tiles at
+// [128, 320), of odd ones at [320, 512).  dS overwrites the scores in place:
+// the 32 keys of one half of a tile become 16 words at the head of their own
+// columns.
+
+constexpr int Q_STAGES = 4;
+constexpr uint32_t Q_STAGE = 4 * SMALL;  // k halves, v parts
+struct QShared {
+  uint64_t q_full, kv_full[Q_STAGES], kv_empty[Q_STAGES], last_full, s_full[2], p_full[2], o_full, drain;
+  uint32_t tmem;
+  int abort_flag;
+  float2 part[4][ROWS];
+};
+constexpr size_t Q_SMEM = 1024 + 4 * BIG + Q_STAGES * Q_STAGE + sizeof(QShared);
+
+__global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  const Args& a = p.a;
+  uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  const uint32_t sq = smem_u32(base), sg = sq + 2 * BIG, skv = sg + 2 * BIG;
+  QShared& sh = *reinterpret_cast<QShared*>(base + 4 * BIG + Q_STAGES * Q_STAGE);
+  volatile int* abort_flag = &sh.abort_flag;
+  int* dev_error = p.dev_error;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ntile = (a.tq + ROWS - 1) / ROWS, nbh = a.n * a.h;
+  const int tile = ntile - 1 - static_cast<int>(blockIdx.x) / nbh;  // longest causal rows first
+  const int bh = static_cast<int>(blockIdx.x) % nbh;
+  const int b = bh / a.h, head = bh - b * a.h, kvh = head / a.grp;
+  const int i0 = tile * ROWS;
+  const int len = key_len(a, b);
+  const int kend = row_limit(a, min(i0 + ROWS, a.tq) - 1, len);
+  const int nt = (kend + COLS - 1) / COLS;
+  const bool dirty = nt > 0 && nt * COLS > len && len < a.tk;
+  const int wide = 2 * a.dh > 64 ? 2 : 1, ksteps = (a.dh + 15) / 16, dsteps = a.dh / 8;
+
+  if (tid == 0) {
+    mbar_init(&sh.q_full, 1);
+    for (int i = 0; i < Q_STAGES; i++) {
+      mbar_init(&sh.kv_full[i], 1);
+      mbar_init(&sh.kv_empty[i], 1);
+    }
+    mbar_init(&sh.last_full, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 8);
+    }
+    mbar_init(&sh.o_full, 1);
+    mbar_init(&sh.drain, 1);
+    sh.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == WARP_MMA) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  // registers: 640 threads x 96 at launch = 512 x 104 + 128 x 64
+  if (warp < SOFT) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int team = warp >> 3, half = (warp >> 2) & 1, w = warp & 3, row = w * 32 + lane, i = i0 + row;
+    const int k4 = team * 2 + half;  // which of the row's four threads
+    const uint32_t lanes = static_cast<uint32_t>(w * 32) << 16;
+    const uint32_t ts = tmem + lanes + 128 + team * 192 + half * 32;
+    const bool in = i < a.tq;
+    const int lim = (in ? row_limit(a, i, len) : 0) - half * 32;
+    const int full = __reduce_min_sync(0xffffffffu, lim);
+    const float lam = __ldg(a.lam + head), c2 = a.slog2;
+    const long long stat = (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
+    const float ls1 = in ? a.flse[stat] : CUDART_INF_F, ls2 = in ? a.flse[stat + a.tq] : CUDART_INF_F;
+    const f32x2 cc = pair(c2, c2), n1 = pair(-ls1, -ls1), n2 = pair(-ls2, -ls2);
+
+    // both maps' entries of 16 columns from the scores
+    auto maps = [&](uint32_t t, float (&x)[16], float (&y)[16], float (&dp)[16], int visible, bool edge) {
+      tmem_ld(t, x);
+      tmem_ld(t + 64, y);
+      tmem_ld(t + 128, dp);
+      tmem_landed(x);
+      tmem_landed(y);
+      tmem_landed(dp);
+#pragma unroll
+      for (int c = 0; c < 16; c += 2) {
+        unpair(fma2(pair(x[c], x[c + 1]), cc, n1), x[c], x[c + 1]);
+        unpair(fma2(pair(y[c], y[c + 1]), cc, n2), y[c], y[c + 1]);
+        x[c] = ex2(x[c]);
+        x[c + 1] = ex2(x[c + 1]);
+        y[c] = ex2(y[c]);
+        y[c + 1] = ex2(y[c + 1]);
+      }
+      if (__builtin_expect(edge, 0)) {
+#pragma unroll
+        for (int c = 0; c < 16; c++)
+          if (c >= visible) x[c] = y[c] = 0.0f;
+      }
+    };
+
+    // D_1 and D_2: from o and o2, or, where a row sees at most two tiles, from
+    // P dP itself (see diffattn.cu on what their rounding does to short rows).
+    float d1 = 0.0f, d2 = 0.0f;
+    if (nt > 2) {
+      if (in) {
+        const int c0 = k4 * (a.dh / 2);
+        const __nv_bfloat16* po = static_cast<const __nv_bfloat16*>(a.fo) + b * a.ob + head * a.oh + i * a.orow + c0;
+        const __nv_bfloat16* py = static_cast<const __nv_bfloat16*>(a.fo2) +
+                                  ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + c0;
+        const __nv_bfloat16* pg = static_cast<const __nv_bfloat16*>(a.dout) + b * a.gb + head * a.gh + i * a.gr + c0;
+#pragma unroll 2
+        for (int c = 0; c < a.dh / 2; c += 4) {
+          const uint2 uo = *reinterpret_cast<const uint2*>(po + c), uy = *reinterpret_cast<const uint2*>(py + c),
+                      ug = *reinterpret_cast<const uint2*>(pg + c);
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const uint32_t wo = e ? uo.y : uo.x, wy = e ? uy.y : uy.x, wg = e ? ug.y : ug.x;
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+              // a bf16 is the high half of the f32 it stands for
+              const float o = __uint_as_float(f ? wo & 0xffff0000u : wo << 16);
+              const float y = __uint_as_float(f ? wy & 0xffff0000u : wy << 16);
+              const float g = __uint_as_float(f ? wg & 0xffff0000u : wg << 16);
+              d2 += g * y;
+              d1 += g * (o + lam * y);
+            }
+          }
+        }
+      }
+    } else if (team < nt) {
+      warp_wait(&sh.s_full[team], 0, abort_flag, dev_error);
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < 32; c += 16) {
+        float x[16], y[16], dp[16];
+        maps(ts + c, x, y, dp, lim - team * COLS - c, true);
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          d1 += x[e] * dp[e];
+          d2 += y[e] * dp[e];
+        }
+      }
+    }
+    sh.part[k4][row] = make_float2(d1, d2);
+    soft_sync();
+    d1 = d2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      d1 += sh.part[k][row].x;
+      d2 += sh.part[k][row].y;
+    }
+    if (in && k4 == 0) {
+      a.dsum[stat] = d1;
+      a.dsum[stat + a.tq] = d2;
+    }
+    soft_sync();
+
+    const f32x2 e1 = pair(-d1, -d1), e2 = pair(-d2, -d2);
+    f32x2 dl = 0ull;
+    for (int j = team; j < nt; j += 2) {
+      if (!warp_wait(&sh.s_full[team], (j >> 1) & 1, abort_flag, dev_error)) break;
+      tc_fence_after();
+      const bool edge = j * COLS + 32 > full;
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        float x[16], y[16], dp[16];
+        maps(ts + c * 16, x, y, dp, lim - j * COLS - c * 16, edge);
+        uint32_t u[8], v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const f32x2 g = pair(dp[2 * e], dp[2 * e + 1]), y2 = pair(y[2 * e], y[2 * e + 1]);
+          dl = fma2(y2, g, dl);
+          float r0, r1;
+          unpair(mul2(pair(x[2 * e], x[2 * e + 1]), add2(g, e1)), r0, r1);
+          u[e] = pack2(r0, r1);
+          unpair(mul2(y2, add2(g, e2)), r0, r1);
+          v[e] = pack2(r0, r1);
+        }
+        tmem_st(ts + c * 8, u);
+        tmem_st(ts + 64 + c * 8, v);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[team]);
+    }
+    float l0, l1;
+    unpair(dl, l0, l1);
+    sh.part[k4][row].x = l0 + l1;
+    soft_sync();
+    if (in && k4 == 0)
+      a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
+          (sh.part[0][row].x + sh.part[1][row].x) + (sh.part[2][row].x + sh.part[3][row].x);
+
+    bool ok = true;
+    if (nt > 0) {
+      ok = warp_wait(&sh.o_full, 0, abort_flag, dev_error);
+      tc_fence_after();
+    }
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.dq) + b * a.dqb + head * a.dqh + i * a.dqr;
+    if (ok) {
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        float x[16] = {};
+        if (nt > 0) {
+          tmem_ld(tmem + lanes + m * 64 + k4 * 16, x);
+          tmem_landed(x);
+        }
+        if (in) store16(o + m * a.dh + k4 * 16, x, m ? -a.scale * lam : a.scale, nt > 0, a.dh - k4 * 16, p.st16);
+        __syncwarp();
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == WARP_COPY) {
+      if (elect_one() && nt > 0) {
+        mbar_arrive_expect_tx(&sh.q_full, (2 + wide) * BIG);
+        for (int h = 0; h < 2; h++) tma_5d(sq + h * BIG, &p.q, 0, h, head, i0, b, &sh.q_full);
+        for (int c = 0; c < wide; c++) tma_5d(sg + c * BIG, &p.g, c * 64, 0, head, i0, b, &sh.q_full);
+        int j = 0;
+        for (; j < nt; j++) {
+          const int st = j % Q_STAGES;
+          if (j >= Q_STAGES && !wait(&sh.kv_empty[st], (j / Q_STAGES - 1) & 1, abort_flag, dev_error)) break;
+          const uint32_t dst = skv + st * Q_STAGE;
+          // a tile to be cleared lands for the clearing warp, which passes it on
+          uint64_t* bar = dirty && j == nt - 1 ? &sh.last_full : &sh.kv_full[st];
+          mbar_arrive_expect_tx(bar, (2 + wide) * SMALL);
+          for (int h = 0; h < 2; h++) tma_5d(dst + h * SMALL, &p.k, 0, h, kvh, j * COLS, b, bar);
+          for (int c = 0; c < wide; c++) tma_5d(dst + (2 + c) * SMALL, &p.v, c * 64, 0, kvh, j * COLS, b, bar);
+        }
+        // what was asked for lands before the block may end, aborting or not
+        settle(&sh.q_full, 0);
+        for (int t = max(0, j - Q_STAGES); t < j; t++)
+          settle(dirty && t == nt - 1 ? &sh.last_full : &sh.kv_full[t % Q_STAGES],
+                 dirty && t == nt - 1 ? 0 : (t / Q_STAGES) & 1);
+      }
+      __syncwarp();
+    } else if (warp == WARP_AUX) {
+      if (dirty) {
+        const int j = nt - 1, st = j % Q_STAGES;
+        if (warp_wait(&sh.last_full, 0, abort_flag, dev_error)) {
+          // hidden keys and values may be NaN: both meet P = 0 in a product
+          uint8_t* kv = base + 4 * BIG + st * Q_STAGE;
+          for (int r = len - j * COLS; r < COLS; r++)
+            for (int c = lane; c < (2 + wide) * 8; c += 32)
+              *reinterpret_cast<uint4*>(kv + (c >> 3) * SMALL + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.kv_full[st]);
+        }
+      }
+    } else if (warp == WARP_MMA && nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      // one accumulator shape for all: MMAs then execute in the order of issue,
+      // and the next scores may overwrite dS right after the products with it
+      const uint32_t id_s = idesc_bf16(ROWS, 64, false), id_o = idesc_bf16(ROWS, 64, true);
+      const uint64_t dq = desc_k(sq), dg = desc_k(sg), dkv = desc_k(skv), dmn = desc_mn(skv, 0);
+      auto done = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, dev_error); };
+      auto landed = [&](int j, int st) { return done(&sh.kv_full[st], (j / Q_STAGES) & 1); };
+      auto scores = [&](int j, int st) {
+        tc_fence_after();
+        const uint64_t kv = dkv + st * (Q_STAGE / 16);
+        const uint32_t d = tmem + 128 + (j & 1) * 192;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++)
+            if (ks < ksteps)
+              mma_ss(d + h * 64, dq + (h * BIG + ks * 32) / 16, kv + (h * SMALL + ks * 32) / 16, id_s, ks > 0, lead);
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++)
+          if (ks < dsteps)
+            mma_ss(d + 128, dg + ((ks >> 2) * BIG + (ks & 3) * 32) / 16,
+                   kv + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
+        commit(&sh.s_full[j & 1], lead);
+      };
+      bool ok = done(&sh.q_full, 0);
+      for (int j = 0; ok && j < min(nt, 2); j++)
+        if ((ok = landed(j, j))) scores(j, j);
+      int st = 0, st2 = 2;
+      for (int j = 0; ok && j < nt; j++) {
+        if (!(ok = done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
+        tc_fence_after();
+        const uint64_t k = dmn + st * (Q_STAGE / 16);
+        const uint32_t s = tmem + 128 + (j & 1) * 192;
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++)
+            mma_ts(tmem + m * 64, s + m * 64 + (ks >> 1) * 32 + (ks & 1) * 8, k + (m * SMALL + ks * 2048) / 16, id_o,
+                   j > 0 || ks > 0, lead);
+        commit(&sh.kv_empty[st], lead);
+        if (j + 1 == nt) commit(&sh.o_full, lead);
+        if (j + 2 < nt) {
+          if (!(ok = landed(j + 2, st2))) break;
+          scores(j + 2, st2);
+        }
+        if (++st == Q_STAGES) st = 0;
+        if (++st2 == Q_STAGES) st2 = 0;
+      }
+      if (!ok) {  // no MMA may write tensor memory after it is released
+        commit(&sh.drain, lead);
+        settle(&sh.drain, 0);
+      }
+      __syncwarp();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+}
+
+// --------------------------------------------------------------------- keys
+//
+// Rows are keys, columns the queries of a tile.  Tensor memory: dv at [0, 128),
+// dk_1 | dk_2 at [128, 256), S_1 | S_2 | dP at [256, 448), dS_1 | dS_2 (bf16) at
+// [448, 512).  The combined map, operand of dv, goes through shared memory.
+// The scores are read into registers at once, so that the next tile's are
+// formed while this one's exponentials are taken.
+
+constexpr int K_STAGES = 4;
+constexpr uint32_t K_STAGE = 4 * SMALL;  // q halves, dout parts
+struct KShared {
+  uint64_t kv_full, q_full[K_STAGES], q_empty[K_STAGES], s_full, s_free, p_full, pv, o_full, drain;
+  uint32_t tmem;
+  int abort_flag;
+  float st[K_STAGES][4][COLS];  // -lse_1, -lse_2, -D_1, -D_2 of a tile's queries
+};
+constexpr size_t K_SMEM = 1024 + 4 * BIG + K_STAGES * K_STAGE + BIG + sizeof(KShared);
+
+__global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  const Args& a = p.a;
+  uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  const uint32_t sk = smem_u32(base), sv = sk + 2 * BIG, sqg = sv + 2 * BIG, sp = sqg + K_STAGES * K_STAGE;
+  KShared& sh = *reinterpret_cast<KShared*>(base + 4 * BIG + K_STAGES * K_STAGE + BIG);
+  volatile int* abort_flag = &sh.abort_flag;
+  int* dev_error = p.dev_error;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nbh = a.n * a.hkv, nkt = (a.tk + ROWS - 1) / ROWS;
+  const bool work = static_cast<int>(blockIdx.x) < nkt * nbh;  // else a block for dlam only
+  const int kt = static_cast<int>(blockIdx.x) / nbh;           // the earliest keys, which most queries see, first
+  const int bh = static_cast<int>(blockIdx.x) % nbh;
+  const int b = bh / a.hkv, kvh = bh - b * a.hkv;
+  const int key0 = kt * ROWS;
+  const int len = key_len(a, b);
+  // queries before `qbeg` see none of these keys
+  int qbeg = 0;
+  if (!work || key0 >= len) {
+    qbeg = a.tq;
+  } else if (a.causal == RNN_CAUSAL_START) {
+    qbeg = min(a.tq, key0);
+  } else if (a.causal == RNN_CAUSAL_END) {
+    qbeg = min(a.tq, max(0, key0 - (len - a.tq)));
+  }
+  const int per = (a.tq - qbeg + COLS - 1) / COLS, nt = per * a.grp;
+  const int wide = 2 * a.dh > 64 ? 2 : 1, ksteps = (a.dh + 15) / 16, dsteps = a.dh / 8;
+
+  if (tid == 0) {
+    mbar_init(&sh.kv_full, 1);
+    for (int i = 0; i < K_STAGES; i++) {
+      mbar_init(&sh.q_full[i], 2);
+      mbar_init(&sh.q_empty[i], 1);
+    }
+    mbar_init(&sh.s_full, 1);
+    mbar_init(&sh.s_free, SOFT);
+    mbar_init(&sh.p_full, SOFT);
+    mbar_init(&sh.pv, 1);
+    mbar_init(&sh.o_full, 1);
+    mbar_init(&sh.drain, 1);
+    sh.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == WARP_MMA) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < SOFT) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int k4 = warp >> 2, w = warp & 3, row = w * 32 + lane, key = key0 + row;
+    const uint32_t lanes = static_cast<uint32_t>(w * 32) << 16;
+    const uint32_t ts = tmem + lanes + 256 + k4 * 16;
+    const f32x2 cc = pair(a.slog2, a.slog2);
+    uint8_t* pc = base + 4 * BIG + K_STAGES * K_STAGE + row * 128;
+    const int ch0 = ((2 * k4) ^ (row & 7)) << 4, ch1 = ((2 * k4 + 1) ^ (row & 7)) << 4;
+
+    int st = 0, e = 0, q0 = qbeg;
+    for (int t = 0; t < nt; t++) {
+      const float lam = __ldg(a.lam + kvh * a.grp + e);
+      float x[16], y[16], dp[16];
+      if (!warp_wait(&sh.q_full[st], (t / K_STAGES) & 1, abort_flag, dev_error)) break;
+      if (!warp_wait(&sh.s_full, t & 1, abort_flag, dev_error)) break;
+      tc_fence_after();
+      tmem_ld(ts, x);
+      tmem_ld(ts + 64, y);
+      tmem_ld(ts + 128, dp);
+      tmem_landed(x);
+      tmem_landed(y);
+      tmem_landed(dp);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.s_free);
+      const float* s = &sh.st[st][0][k4 * 16];
+      const f32x2 ll = pair(-lam, -lam);
+#pragma unroll
+      for (int c = 0; c < 16; c += 2) {
+        unpair(fma2(pair(x[c], x[c + 1]), cc, *reinterpret_cast<const f32x2*>(s + c)), x[c], x[c + 1]);
+        unpair(fma2(pair(y[c], y[c + 1]), cc, *reinterpret_cast<const f32x2*>(s + COLS + c)), y[c], y[c + 1]);
+        x[c] = ex2(x[c]);
+        x[c + 1] = ex2(x[c + 1]);
+        y[c] = ex2(y[c]);
+        y[c + 1] = ex2(y[c + 1]);
+      }
+      if (a.causal) {
+        // the first query that sees this key
+        const int first = (a.causal == RNN_CAUSAL_START ? key : key - (len - a.tq)) - (q0 + k4 * 16);
+        if (__any_sync(0xffffffffu, first > 0)) {
+#pragma unroll
+          for (int c = 0; c < 16; c++)
+            if (c < first) x[c] = y[c] = 0.0f;
+        }
+      }
+      uint32_t u[8], v[8], z[8];
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        const f32x2 g = pair(dp[2 * c], dp[2 * c + 1]), x2 = pair(x[2 * c], x[2 * c + 1]);
+        const f32x2 y2 = mul2(pair(y[2 * c], y[2 * c + 1]), ll);  // -lam P_2
+        float r0, r1;
+        unpair(mul2(x2, add2(g, *reinterpret_cast<const f32x2*>(s + 2 * COLS + 2 * c))), r0, r1);
+        u[c] = pack2(r0, r1);
+        unpair(mul2(y2, add2(g, *reinterpret_cast<const f32x2*>(s + 3 * COLS + 2 * c))), r0, r1);
+        v[c] = pack2(r0, r1);
+        unpair(add2(x2, y2), r0, r1);
+        z[c] = pack2(r0, r1);
+      }
+      // the products of the tile before have read the operands
+      if (t > 0 && !warp_wait(&sh.pv, (t - 1) & 1, abort_flag, dev_error)) break;
+      tc_fence_after();
+      *reinterpret_cast<uint4*>(pc + ch0) = make_uint4(z[0], z[1], z[2], z[3]);
+      *reinterpret_cast<uint4*>(pc + ch1) = make_uint4(z[4], z[5], z[6], z[7]);
+      fence_async_smem();
+      tmem_st(tmem + lanes + 448 + k4 * 8, u);
+      tmem_st(tmem + lanes + 480 + k4 * 8, v);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full);
+      if (++st == K_STAGES) st = 0;
+      q0 += COLS;
+      if (q0 >= qbeg + per * COLS) {
+        q0 = qbeg;
+        e++;
+      }
+    }
+    bool ok = true;
+    if (nt > 0) {
+      ok = warp_wait(&sh.o_full, 0, abort_flag, dev_error);
+      tc_fence_after();
+    }
+    if (ok && work) {
+      const bool some = nt > 0 && key < len;
+      __nv_bfloat16* odk = static_cast<__nv_bfloat16*>(a.dk) + b * a.dkb + kvh * a.dkh + key * a.dkr;
+      __nv_bfloat16* odv = static_cast<__nv_bfloat16*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr;
+#pragma unroll
+      for (int m = 0; m < 4; m++) {
+        float x[16] = {};
+        if (nt > 0) {
+          tmem_ld(tmem + lanes + m * 64 + k4 * 16, x);
+          tmem_landed(x);
+        }
+        if (key < a.tk) {
+          if (m < 2) {
+            store16(odv + m * 64 + k4 * 16, x, 1.0f, some, 2 * a.dh - m * 64 - k4 * 16, p.st16);
+          } else {
+            store16(odk + (m - 2) * a.dh + k4 * 16, x, a.scale, some, a.dh - k4 * 16, p.st16);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == WARP_COPY) {
+      if (elect_one() && nt > 0) {
+        mbar_arrive_expect_tx(&sh.kv_full, (2 + wide) * BIG);
+        for (int h = 0; h < 2; h++) tma_5d(sk + h * BIG, &p.k, 0, h, kvh, key0, b, &sh.kv_full);
+        for (int c = 0; c < wide; c++) tma_5d(sv + c * BIG, &p.v, c * 64, 0, kvh, key0, b, &sh.kv_full);
+        int t = 0;
+        for (; t < nt; t++) {
+          const int st = t % K_STAGES;
+          if (t >= K_STAGES && !wait(&sh.q_empty[st], (t / K_STAGES - 1) & 1, abort_flag, dev_error)) break;
+          const uint32_t dst = sqg + st * K_STAGE;
+          const int head = kvh * a.grp + t / per, i0 = qbeg + (t % per) * COLS;
+          mbar_arrive_expect_tx(&sh.q_full[st], (2 + wide) * SMALL);
+          for (int h = 0; h < 2; h++) tma_5d(dst + h * SMALL, &p.q, 0, h, head, i0, b, &sh.q_full[st]);
+          for (int c = 0; c < wide; c++) tma_5d(dst + (2 + c) * SMALL, &p.g, c * 64, 0, head, i0, b, &sh.q_full[st]);
+        }
+        // what was asked for lands before the block may end, aborting or not
+        settle(&sh.kv_full, 0);
+        for (int i = max(0, t - K_STAGES); i < t; i++) settle(&sh.q_full[i % K_STAGES], (i / K_STAGES) & 1);
+      }
+      __syncwarp();
+    } else if (warp == WARP_AUX) {
+      for (int t = 0; t < nt; t++) {
+        const int st = t % K_STAGES;
+        if (t >= K_STAGES && !warp_wait(&sh.q_empty[st], (t / K_STAGES - 1) & 1, abort_flag, dev_error)) break;
+        const int head = kvh * a.grp + t / per, i0 = qbeg + (t % per) * COLS;
+        const long long at = (static_cast<long long>(b) * a.h + head) * 2 * a.tq;
+#pragma unroll
+        for (int c = lane; c < COLS; c += 32) {
+          const int i = i0 + c;
+          const bool in = i < a.tq;
+          sh.st[st][0][c] = in ? -a.flse[at + i] : -CUDART_INF_F;
+          sh.st[st][1][c] = in ? -a.flse[at + a.tq + i] : -CUDART_INF_F;
+          sh.st[st][2][c] = in ? -a.dsum[at + i] : 0.0f;
+          sh.st[st][3][c] = in ? -a.dsum[at + a.tq + i] : 0.0f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_full[st]);
+      }
+    } else if (warp == WARP_SUM) {
+      // dlam: block `head` sums that head's rows in a fixed order
+      if (static_cast<int>(blockIdx.x) < a.h && a.tq > 0) {
+        const long long cnt = static_cast<long long>(a.n) * a.tq;
+        const float* x = a.dlrow + blockIdx.x * cnt;
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+        long long i = lane;
+        for (; i + 96 < cnt; i += 128)
+#pragma unroll
+          for (int k = 0; k < 4; k++) s[k] += x[i + 32 * k];
+        for (; i < cnt; i += 32) s[0] += x[i];
+        double sum = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) a.dlam[blockIdx.x] -= static_cast<float>(sum);
+      }
+    } else if (warp == WARP_MMA && nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      const uint32_t id_s = idesc_bf16(ROWS, 64, false), id_k = idesc_bf16(ROWS, 64, true),
+                     id_v = idesc_bf16(ROWS, 2 * a.dh, true);
+      const uint64_t dk = desc_k(sk), dv = desc_k(sv), dqg = desc_k(sqg), dp = desc_k(sp);
+      const uint64_t mq = desc_mn(sqg, 0), mg = desc_mn(sqg + 2 * SMALL, SMALL);
+      auto done = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, dev_error); };
+      auto scores = [&](int st) {
+        tc_fence_after();
+        const uint64_t q = dqg + st * (K_STAGE / 16);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++)
+            if (ks < ksteps)
+              mma_ss(tmem + 256 + h * 64, dk + (h * BIG + ks * 32) / 16, q + (h * SMALL + ks * 32) / 16, id_s, ks > 0,
+                     lead);
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++)
+          if (ks < dsteps)
+            mma_ss(tmem + 384, dv + ((ks >> 2) * BIG + (ks & 3) * 32) / 16,
+                   q + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
+        commit(&sh.s_full, lead);
+      };
+      bool ok = done(&sh.kv_full, 0) && done(&sh.q_full[0], 0);
+      if (ok) scores(0);
+      int st = 0, st1 = 1;  // stages of tiles t and t + 1
+      for (int t = 0; ok && t < nt; t++) {
+        if (t + 1 < nt) {
+          if (!(ok = done(&sh.q_full[st1], ((t + 1) / K_STAGES) & 1) && done(&sh.s_free, t & 1))) break;
+          scores(st1);
+        }
+        if (!(ok = done(&sh.p_full, t & 1))) break;
+        tc_fence_after();
+        const uint64_t q = mq + st * (K_STAGE / 16), g = mg + st * (K_STAGE / 16);
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++)
+            mma_ts(tmem + 128 + m * 64, tmem + 448 + m * 32 + ks * 8, q + (m * SMALL + ks * 2048) / 16, id_k,
+                   t > 0 || ks > 0, lead);
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) mma_ss(tmem, dp + ks * 2, g + ks * (2048 / 16), id_v, t > 0 || ks > 0, lead);
+        commit(&sh.pv, lead);
+        commit(&sh.q_empty[st], lead);
+        if (t + 1 == nt) commit(&sh.o_full, lead);
+        if (++st == K_STAGES) st = 0;
+        if (++st1 == K_STAGES) st1 = 0;
+      }
+      if (!ok) {  // no MMA may write tensor memory after it is released
+        commit(&sh.drain, lead);
+        settle(&sh.drain, 0);
+      }
+      __syncwarp();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+}
+
+bool mult8(std::initializer_list<long long> s) {
+  for (long long x : s)
+    if (x % 8) return false;
+  return true;
+}
+
+}  // namespace
+
+bool tc_bwd_ok(const Args& a) {
+  if (a.dh % 8 || a.dh < 16 || a.dh > 64 || a.kmask || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
+  if (a.tq < 64 || a.tk < 64) return false;
+  if (reinterpret_cast<uintptr_t>(a.fo) % 16 || reinterpret_cast<uintptr_t>(a.fo2) % 16) return false;
+  if (!mult8({a.ob, a.orow, a.oh})) return false;
+  return map_ok(a.q, a.n, a.tq, a.h, a.dh, a.qb, a.qr, a.qh) && map_ok(a.k, a.n, a.tk, a.hkv, a.dh, a.kb, a.kr, a.kh) &&
+         map_ok(a.v, a.n, a.tk, a.hkv, 2 * a.dh, a.vb, a.vr, a.vh) &&
+         map_ok(a.dout, a.n, a.tq, a.h, 2 * a.dh, a.gb, a.gr, a.gh);
+}
+
+int tc_bwd(rnn_ctx* ctx, const Args& a) {
+  Params p;
+  p.a = a;
+  p.dev_error = ctx->dev_error;
+  p.st16 = mult8({a.dqb, a.dqr, a.dqh, a.dkb, a.dkr, a.dkh, a.dvb, a.dvr, a.dvh}) &&
+           (reinterpret_cast<uintptr_t>(a.dq) | reinterpret_cast<uintptr_t>(a.dk) | reinterpret_cast<uintptr_t>(a.dv)) %
+                   16 == 0;
+  const long long qblocks = (a.tq + ROWS - 1ll) / ROWS * a.n * a.h;
+  const long long kblocks = std::max<long long>((a.tk + ROWS - 1ll) / ROWS * a.n * a.hkv, a.h);
+  RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31), "diffattn: too many rows");
+  static std::atomic<unsigned long long> optin_q{0}, optin_k{0};
+  RNN_TRY(tc::ensure_smem_optin(tc_bwd_q_kernel, optin_q, ctx->device, static_cast<int>(Q_SMEM)));
+  RNN_TRY(tc::ensure_smem_optin(tc_bwd_kv_kernel, optin_k, ctx->device, static_cast<int>(K_SMEM)));
+  RNN_TRY(encode_map(&p.q, a.q, a.n, a.tq, a.h, 2, a.dh, a.qb, a.qr, a.qh, ROWS));
+  RNN_TRY(encode_map(&p.g, a.dout, a.n, a.tq, a.h, 1, 2 * a.dh, a.gb, a.gr, a.gh, ROWS));
+  RNN_TRY(encode_map(&p.k, a.k, a.n, a.tk, a.hkv, 2, a.dh, a.kb, a.kr, a.kh, COLS));
+  RNN_TRY(encode_map(&p.v, a.v, a.n, a.tk, a.hkv, 1, 2 * a.dh, a.vb, a.vr, a.vh, COLS));
+  tc_bwd_q_kernel<<<static_cast<unsigned>(qblocks), THREADS, Q_SMEM, ctx->stream>>>(p);
+  RNN_CHECK_LAUNCH();
+  // the keys' kernel owns 128 keys and reads the queries 64 at a time
+  RNN_TRY(encode_map(&p.q, a.q, a.n, a.tq, a.h, 2, a.dh, a.qb, a.qr, a.qh, COLS));
+  RNN_TRY(encode_map(&p.g, a.dout, a.n, a.tq, a.h, 1, 2 * a.dh, a.gb, a.gr, a.gh, COLS));
+  RNN_TRY(encode_map(&p.k, a.k, a.n, a.tk, a.hkv, 2, a.dh, a.kb, a.kr, a.kh, ROWS));
+  RNN_TRY(encode_map(&p.v, a.v, a.n, a.tk, a.hkv, 1, 2 * a.dh, a.vb, a.vr, a.vh, ROWS));
+  tc_bwd_kv_kernel<<<static_cast<unsigned>(kblocks), THREADS, K_SMEM, ctx->stream>>>(p);
+  RNN_CHECK_LAUNCH();
+  return RNN_OK;
+}
+
+}  // namespace diff
+}  // namespace rnn

@@ -165,6 +165,26 @@ def test_lengths_and_masks_with_anything_hidden(ops, tq, tk, causal, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [None, "start", "end"])
+@pytest.mark.parametrize("tq,tk,h,hkv,dh", [(700, 700, 2, 1, 40), (130, 1000, 2, 2, 64), (300, 700, 1, 1, 16)])
+def test_ragged_lengths_over_many_tiles(ops, tq, tk, h, hkv, dh, causal, dtype):
+    """Lengths that end anywhere in any of many key tiles; what lies beyond them is NaN or infinite."""
+    lens = [0, 1, 63, 64, 65, 127, 130, 300, 449, 511, 577, 640, 699, tk]
+    q, k, v, lam, dout = make(len(lens), tq, tk, h, hkv, dh, dtype, 17)
+    klen = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    hidden = torch.arange(tk, device="cuda")[None] >= klen[:, None]
+    k.masked_fill_(hidden[:, :, None, None], math.nan)
+    v.masked_fill_(hidden[:, :, None, None], math.inf)
+    check_all(ops, q, k, v, lam, dout, causal=causal, klen=klen)
+    # and each sequence by itself, whose rows outweigh none
+    want = reference(q, k, v, lam, dout, dh ** -0.5, causal, klen)
+    got = run_all(ops, q, k, v, lam, dout, causal=causal, klen=klen)
+    for b in range(len(lens)):
+        for x, y in zip((got[0], got[3], got[4], got[5]), (want[0], want[2], want[3], want[4])):
+            assert rel(x[b], y[b]) < 2 * TOL[dtype] or lens[b] <= 1, (lens[b], rel(x[b], y[b]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_single_key_has_no_score_gradient(ops, dtype):
     """One visible key: the maps are 1, o = (1 - lam) v, dq and dk are exactly 0."""
     q, k, v, lam, dout = make(3, 5, 9, 2, 2, 16, dtype, 4)
