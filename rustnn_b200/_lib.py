@@ -242,4 +242,6 @@ def check(code: int, what: str = "") -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    code = getattr(_lib or lib(), name)(*args)
+    if code != RNN_OK:
+        check(code, name)

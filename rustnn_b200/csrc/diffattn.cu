@@ -950,12 +950,6 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
 
 // --------------------------------------------------------------------- host
 
-template <class K>
-int allow_smem(K kernel, size_t bytes) {
-  RNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-  return RNN_OK;
-}
-
 template <class T, int DH, int RW>
 int fwd_launch(rnn_ctx* ctx, Args a) {
   using F = Fwd<T, DH, RW>;
@@ -963,11 +957,16 @@ int fwd_launch(rnn_ctx* ctx, Args a) {
   const long long nbh = static_cast<long long>(a.n) * a.hkv;
   const long long blocks = (rows + F::ROWS - 1) / F::ROWS * nbh;
   RNN_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
-  RNN_TRY(allow_smem(fwd_kernel<T, DH, RW>, F::SMEM));
+  static std::atomic<unsigned long long> optin{0};
+  RNN_TRY(tc::ensure_smem_optin(fwd_kernel<T, DH, RW>, optin, ctx->device, static_cast<int>(F::SMEM)));
   // Split the keys when the rows alone do not give every SM a block, in parts
   // of at least four tiles.
-  int per_sm = 1;
-  RNN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fwd_kernel<T, DH, RW>, THREADS, F::SMEM));
+  static std::atomic<int> resident{0};  // blocks of this kernel an SM holds (every device here is the same part)
+  int per_sm = resident.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    RNN_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fwd_kernel<T, DH, RW>, THREADS, F::SMEM));
+    resident.store(per_sm, std::memory_order_relaxed);
+  }
   const long long slots = static_cast<long long>(ctx->num_sms) * std::max(1, per_sm);
   const int tiles = (a.tk + F::BN - 1) / F::BN;
   long long ns = std::min<long long>(slots / std::max(1ll, blocks), tiles / 4);
@@ -1010,8 +1009,9 @@ int bwd_launch(rnn_ctx* ctx, Args a) {
   const long long qblocks = (rows + FQ::ROWS - 1) / FQ::ROWS * nbh;
   const long long kblocks = std::max<long long>((a.tk + FK::KEYS - 1ll) / FK::KEYS * nbh, a.h);
   RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
-  RNN_TRY(allow_smem(bwd_q_kernel<T, DH>, FQ::SMEM));
-  RNN_TRY(allow_smem(bwd_kv_kernel<T, DH>, FK::SMEM));
+  static std::atomic<unsigned long long> optin_q{0}, optin_kv{0};
+  RNN_TRY(tc::ensure_smem_optin(bwd_q_kernel<T, DH>, optin_q, ctx->device, static_cast<int>(FQ::SMEM)));
+  RNN_TRY(tc::ensure_smem_optin(bwd_kv_kernel<T, DH>, optin_kv, ctx->device, static_cast<int>(FK::SMEM)));
   if (qblocks > 0) {
     bwd_q_kernel<T, DH><<<static_cast<unsigned>(qblocks), THREADS, FQ::SMEM, ctx->stream>>>(a);
     RNN_CHECK_LAUNCH();
@@ -1037,6 +1037,7 @@ size_t extent(int n, int t, int heads, long long sb, long long sr, long long sh,
 // Whether no two (sequence, row, head) of a written view share an element:
 // sorted by stride, each step has to clear what the smaller ones span.
 bool disjoint(int n, int t, int heads, long long sb, long long sr, long long sh, int cols) {
+  if (n == 0 || t == 0 || heads == 0) return true;
   std::pair<long long, int> d[3] = {{sb, n}, {sr, t}, {sh, heads}};
   std::sort(d, d + 3);
   long long span = cols;
@@ -1116,6 +1117,14 @@ bool aligned(std::initializer_list<const void*> ps, size_t bytes) {
 }
 
 }  // namespace
+
+int join_parts(rnn_ctx* ctx, const Args& a) {
+  const long long rows = static_cast<long long>(a.n) * a.h * a.tq;
+  join_kernel<__nv_bfloat16, 128><<<static_cast<unsigned>((rows + 3) / 4), THREADS, 0, ctx->stream>>>(a);
+  RNN_CHECK_LAUNCH();
+  return RNN_OK;
+}
+
 }  // namespace diff
 }  // namespace rnn
 
@@ -1140,6 +1149,7 @@ extern "C" int rnn_diffattn_fwd_dev(rnn_ctx* ctx, const rnn_diffattn* d, const v
           diff::multiples({a.qb, a.qr, a.qh, a.kb, a.kr, a.kh, a.vb, a.vr, a.vh}, 16 / esz);
   a.pair = diff::multiples({a.ob, a.orow, a.oh}, 2) && diff::aligned({o}, 2 * esz);
   if (d->dtype == RNN_F32) return diff::fwd_type<float>(ctx, a);
+  if (diff::dec_ok(a)) return diff::dec_fwd(ctx, a);
   return diff::tc_fwd_ok(a) ? diff::tc_fwd(ctx, a) : diff::fwd_type<__nv_bfloat16>(ctx, a);
 }
 

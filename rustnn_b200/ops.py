@@ -15,6 +15,7 @@ Reference interfaces mirrored here:
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -33,6 +34,11 @@ __all__ = [
 ]
 
 
+# the current stream's handle without building a Stream object, which costs more than a small launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 class Context:
     """An rnn_ctx on one device (its stream follows torch's current stream)."""
 
@@ -47,7 +53,7 @@ class Context:
         self._stream = None
 
     def bind(self):
-        s = torch.cuda.current_stream(self.device).cuda_stream
+        s = _raw_stream(self.device)
         if s != self._stream:
             call("rnn_ctx_set_stream", self.h, C.c_void_p(s))
             self._stream = s
@@ -268,43 +274,57 @@ def attn_backward(n, h, dh, th, tw, mh, mw, q, qstride, qoff, kv, kvstride, koff
 _DTYPES = {torch.float32: RNN_F32, torch.bfloat16: RNN_BF16}
 
 
-def _view(t, name, shape, like=None):
-    """Checks a float32 or bfloat16 CUDA tensor of the given shape (None: any
-    extent) with contiguous columns; of the type and device of `like`."""
+def _view(t, name, dim, dtype=None, shape=None, device=None):
+    """(shape, strides, address) of a float32 or bfloat16 CUDA tensor with `dim`
+    axes and contiguous columns, of the given type, shape and device if any."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DTYPES:
         raise RnnError(f"{name}: expected a CUDA float32 or bfloat16 tensor")
-    if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-        raise RnnError(f"{name}: shape {tuple(t.shape)}, expected {tuple('*' if w is None else w for w in shape)}")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise RnnError(f"{name}: {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.dim() != dim:
+        raise RnnError(f"{name}: {t.dim()} axes, expected {dim}")
+    got, strides = t.shape, t.stride()
+    if shape is not None and got != shape:
+        raise RnnError(f"{name}: shape {tuple(got)}, expected {tuple(shape)}")
+    if dtype is not None and (t.dtype != dtype or t.device != device):
+        raise RnnError(f"{name}: {t.dtype} on {t.device}, expected {dtype} on {device}")
+    if strides[-1] != 1 and got[-1] > 1:
         raise RnnError(f"{name}: columns must be contiguous")
-    return C.c_void_p(t.data_ptr())
+    return got, strides, t.data_ptr()
 
 
 def _plain(t, name, dtypes, shape, device):
-    """Checks a contiguous tensor of one of the types and the given shape."""
+    """The address of a contiguous tensor of one of the types, of the given shape."""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != device:
         raise RnnError(f"{name}: expected a {' or '.join(str(d) for d in dtypes)} tensor on {device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise RnnError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     if not t.is_contiguous():
         raise RnnError(f"{name}: tensor must be contiguous")
-    return C.c_void_p(t.data_ptr())
+    return t.data_ptr()
+
+
+_F32, _I32, _BYTES = (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
+
+
+@functools.lru_cache(maxsize=None)
+def _pairs(pairs):
+    """(ctypes array, sum) of a tuple of pair counts."""
+    return (C.c_int * len(pairs))(*pairs), sum(pairs)
 
 
 def _rope(x, pos, inv_freq, pairs, interleaved, backward, out, ctx):
-    xp = _view(x, "x", (None, None, None))
-    rows, heads, dh = x.shape
-    pairs = tuple(int(p) for p in pairs)
-    pp = _plain(pos, "pos", (torch.int32,), (rows, len(pairs)), x.device)
-    fp = _plain(inv_freq, "inv_freq", (torch.float32,), (sum(pairs),), x.device)
+    shape, xs, xp = _view(x, "x", 3)
+    rows, heads, dh = shape
+    dtype, device = x.dtype, x.device
+    counts, total = _pairs(pairs if type(pairs) is tuple else tuple(int(p) for p in pairs))
+    pp = _plain(pos, "pos", _I32, (rows, len(counts)), device)
+    fp = _plain(inv_freq, "inv_freq", _F32, (total,), device)
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    yp = _view(out, "out", x.shape, x)
-    call("rnn_rope_dev", _ctx_of(x, ctx), _DTYPES[x.dtype], xp, x.stride(0), x.stride(1), rows, heads, dh, pp,
-         len(pairs), (C.c_int * len(pairs))(*pairs), fp, int(bool(interleaved)), int(backward), yp, out.stride(0),
-         out.stride(1))
+        out = torch.empty(shape, dtype=dtype, device=device)
+        ys, yp = (heads * dh, dh), out.data_ptr()
+    else:
+        _, ys, yp = _view(out, "out", 3, dtype, shape, device)
+    call("rnn_rope_dev", _ctx_of(x, ctx), _DTYPES[dtype], xp, xs[0], xs[1], rows, heads, dh, pp, len(counts), counts, fp,
+         1 if interleaved else 0, backward, yp, ys[0], ys[1])
     return out
 
 
@@ -329,27 +349,34 @@ _CAUSAL = {None: 0, "start": 1, "end": 2}
 
 
 def _diffattn(q, k, v, lam, o, scale, causal, klen, kmask):
-    """Checks a differential attention call; (description, pointers of q, k, v, lam, o)."""
-    qp = _view(q, "q", (None, None, None, None))
-    n, tq, h, w = q.shape
-    kp = _view(k, "k", (n, None, None, w), q)
-    tk, hkv = k.shape[1:3]
-    vp = _view(v, "v", (n, tk, hkv, w), q)
-    op = _view(o, "out", q.shape, q)
-    lp = _plain(lam, "lam", (torch.float32,), (h,), q.device)
+    """Checks a differential attention call, allocating o if it is None;
+    (description, o, addresses of q, k, v, lam, o)."""
+    shape, qs, qp = _view(q, "q", 4)
+    n, tq, h, w = shape
+    dtype, device = q.dtype, q.device
+    kshape, ks, kp = _view(k, "k", 4, dtype, None, device)
+    tk, hkv = kshape[1], kshape[2]
+    if kshape[0] != n or kshape[3] != w:
+        raise RnnError(f"k: shape {tuple(kshape)}, expected ({n}, *, *, {w})")
+    _, vs, vp = _view(v, "v", 4, dtype, kshape, device)
+    if o is None:
+        o = torch.empty(shape, device=device, dtype=dtype)
+        os, op = (tq * h * w, h * w, w), o.data_ptr()
+    else:
+        _, os, op = _view(o, "out", 4, dtype, shape, device)
+    lp = _plain(lam, "lam", _F32, (h,), device)
     if w % 2 or w == 0:
         raise RnnError(f"q: {w} columns, expected two halves")
     if causal not in _CAUSAL:
         raise RnnError(f"causal: {causal!r}, expected None, 'start' or 'end'")
-    d = DiffAttn(_DTYPES[q.dtype], _CAUSAL[causal], n, h, hkv, w // 2, tq, tk,
-                 (w // 2) ** -0.5 if scale is None else scale, 0,
-                 *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
+    d = DiffAttn(_DTYPES[dtype], _CAUSAL[causal], n, h, hkv, w // 2, tq, tk, (w // 2) ** -0.5 if scale is None else scale,
+                 0, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os[0], os[1], os[2])
     if klen is not None:
-        d.klen = _plain(klen, "klen", (torch.int32,), (n,), q.device)
+        d.klen = _plain(klen, "klen", _I32, (n,), device)
     if kmask is not None:
-        d.kmask = _plain(kmask, "kmask", (torch.bool, torch.uint8), (n, tk), q.device)
+        d.kmask = _plain(kmask, "kmask", _BYTES, (n, tk), device)
         d.kmask_batch = tk
-    return d, (qp, kp, vp, lp), op
+    return d, o, (qp, kp, vp, lp, op)
 
 
 def diffattn_forward(q, k, v, lam, scale=None, causal=None, klen=None, kmask=None, save=False, out=None, ctx=None):
@@ -364,14 +391,12 @@ def diffattn_forward(q, k, v, lam, scale=None, causal=None, klen=None, kmask=Non
     sees no key gets 0; hidden keys and values may hold anything.
 
     Returns o [n, tq, h, 2*dh], or with save (o, o2, lse) for the backward."""
-    if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype) if isinstance(q, torch.Tensor) else None
-    d, ptrs, op = _diffattn(q, k, v, lam, out, scale, causal, klen, kmask)
+    d, out, ptrs = _diffattn(q, k, v, lam, out, scale, causal, klen, kmask)
     o2 = lse = None
     if save:
         o2 = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         lse = torch.empty((d.n, d.h, 2, d.tq), device=q.device, dtype=torch.float32)
-    call("rnn_diffattn_fwd_dev", _ctx_of(q, ctx), C.byref(d), *ptrs, op, None if o2 is None else o2.data_ptr(),
+    call("rnn_diffattn_fwd_dev", _ctx_of(q, ctx), d, *ptrs, None if o2 is None else o2.data_ptr(),
          None if lse is None else lse.data_ptr())
     return (out, o2, lse) if save else out
 
@@ -382,17 +407,21 @@ def diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam, scale=None, causal=N
     dv), written; dlam [h] accumulates.  dout, dq, dk and dv may have strides of
     their own (the parts of a fused projection's gradient, say); those of dq,
     dk, dv that are not given are allocated."""
-    d, ptrs, op = _diffattn(q, k, v, lam, o, scale, causal, klen, kmask)
-    gp = _view(dout, "dout", o.shape, q)
-    o2p = _plain(o2, "o2", (q.dtype,), q.shape, q.device)
-    lsep = _plain(lse, "lse", (torch.float32,), (d.n, d.h, 2, d.tq), q.device)
-    dlp = _plain(dlam, "dlam", (torch.float32,), (d.h,), q.device)
-    grads = [torch.empty(t.shape, device=q.device, dtype=q.dtype) if g is None else g
+    if o is None:
+        raise RnnError("o: the forward's output is needed")
+    d, o, ptrs = _diffattn(q, k, v, lam, o, scale, causal, klen, kmask)
+    dtype, device = q.dtype, q.device
+    _, gs, gp = _view(dout, "dout", 4, dtype, o.shape, device)
+    o2p = _plain(o2, "o2", (dtype,), q.shape, device)
+    lsep = _plain(lse, "lse", _F32, (d.n, d.h, 2, d.tq), device)
+    dlp = _plain(dlam, "dlam", _F32, (d.h,), device)
+    grads = [torch.empty(t.shape, device=device, dtype=dtype) if g is None else g
              for g, t in ((dq, q), (dk, k), (dv, v))]
-    gptrs = [_view(g, name, t.shape, q) for g, t, name in zip(grads, (q, k, v), ("dq", "dk", "dv"))]
-    gd = DiffAttn(d.dtype, d.causal, d.n, d.h, d.hkv, d.dh, d.tq, d.tk, d.scale, 0,
-                  *(x for t in (*grads, dout) for x in t.stride()[:3]))
-    call("rnn_diffattn_bwd_dev", _ctx_of(q, ctx), C.byref(d), C.byref(gd), *ptrs, op, o2p, lsep, gp, *gptrs, dlp)
+    (_, qs, qp), (_, ks, kp), (_, vs, vp) = (_view(g, name, 4, dtype, t.shape, device)
+                                             for g, t, name in zip(grads, (q, k, v), ("dq", "dk", "dv")))
+    gd = DiffAttn(d.dtype, d.causal, d.n, d.h, d.hkv, d.dh, d.tq, d.tk, d.scale, 0, qs[0], qs[1], qs[2], ks[0], ks[1],
+                  ks[2], vs[0], vs[1], vs[2], gs[0], gs[1], gs[2])
+    call("rnn_diffattn_bwd_dev", _ctx_of(q, ctx), d, gd, *ptrs, o2p, lsep, gp, qp, kp, vp, dlp)
     return tuple(grads)
 
 
