@@ -166,11 +166,9 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
         for (int nb = 0; nb < NS; nb += 2) {
           typename FR::B f[2];
           FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma(s1[nb], q1, f[0]);
-          FR::mma(s1[nb + 1], q1, f[1]);
+          FR::mma2(s1[nb], s1[nb + 1], q1, f);
           FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma(s2[nb], q2, f[0]);
-          FR::mma(s2[nb + 1], q2, f[1]);
+          FR::mma2(s2[nb], s2[nb + 1], q2, f);
         }
       }
       const bool edge = mask != nullptr || j0 + SUB > full;
@@ -238,10 +236,7 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
         for (int ks = 0; ks < SUB / KS; ks++) {
           typename FR::B f[2];
           FR::ldB2_kn(f, v, PITCH, s0 + ks * KS, nb * 8, lane);
-          FR::mma(x[0], pa[ks], f[0]);
-          FR::mma(x[1], pa[ks], f[1]);
-          FR::mma(y[0], pb[ks], f[0]);
-          FR::mma(y[1], pb[ks], f[1]);
+          FR::mma4(x, y, pa[ks], pb[ks], f);
         }
 #pragma unroll
         for (int i = 0; i < 2; i++)
@@ -378,60 +373,91 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
   }
 }
 
-// Joins the key parts of a row: one warp per packed row.
+// Joins the key parts of a row: one block per packed row.  Its threads weigh the
+// parts first; then 2 * W threads take a column each and groups of them a share
+// of the parts each, so that the loads of all parts are in flight at once.
+constexpr int JOIN_THREADS = 256, JOIN_PARTS = 1184;  // parts at most: eight for each SM
+
 template <class T, int W>
-__global__ void __launch_bounds__(THREADS) join_kernel(Args a) {
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(Args a) {
+  constexpr int GROUPS = JOIN_THREADS / W > 0 ? JOIN_THREADS / W : 1;
+  __shared__ float4 w[JOIN_PARTS];  // w_1, w_2 and what the sums get of each
+  __shared__ float2 red[JOIN_THREADS / 32], acc[GROUPS][W];
   const int rows = a.grp * a.tq;
-  const long long total = static_cast<long long>(a.n) * a.hkv * rows;
-  const long long idx = static_cast<long long>(blockIdx.x) * (THREADS / 32) + (threadIdx.x >> 5);
-  if (idx >= total) return;
-  const int lane = threadIdx.x & 31;
+  const long long total = static_cast<long long>(a.n) * a.hkv * rows, idx = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int p = static_cast<int>(idx % rows), bh = static_cast<int>(idx / rows);
   const int b = bh / a.hkv, kvh = bh - b * a.hkv;
   float M1 = -CUDART_INF_F, M2 = -CUDART_INF_F;
-  for (int s = lane; s < a.nsplit; s += 32) {
-    const float4 v = *reinterpret_cast<const float4*>(a.stat + (s * total + idx) * 4);
-    M1 = fmaxf(M1, v.x);
-    M2 = fmaxf(M2, v.z);
+  for (int s = tid; s < a.nsplit; s += JOIN_THREADS) {
+    w[s] = *reinterpret_cast<const float4*>(a.stat + (s * total + idx) * 4);
+    M1 = fmaxf(M1, w[s].x);
+    M2 = fmaxf(M2, w[s].z);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     M1 = fmaxf(M1, __shfl_xor_sync(0xffffffffu, M1, o));
     M2 = fmaxf(M2, __shfl_xor_sync(0xffffffffu, M2, o));
   }
-  const float U1 = M1 == -CUDART_INF_F ? 0.0f : M1, U2 = M2 == -CUDART_INF_F ? 0.0f : M2;
-  constexpr int C = W / 32;
-  float x[C] = {}, y[C] = {}, L1 = 0.0f, L2 = 0.0f;
-  for (int s = 0; s < a.nsplit; s++) {
-    const float4 v = *reinterpret_cast<const float4*>(a.stat + (s * total + idx) * 4);
-    const float w1 = ex2(v.x - U1), w2 = ex2(v.z - U2);
-    L1 += w1 * v.y;
-    L2 += w2 * v.w;
-    const float* q = a.part + (s * total + idx) * (2 * W) + lane;
+  if (lane == 0) red[tid >> 5] = make_float2(M1, M2);
+  __syncthreads();
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-      x[c] += w1 * q[32 * c];
-      y[c] += w2 * q[W + 32 * c];
-    }
+  for (int i = 0; i < JOIN_THREADS / 32; i++) {
+    M1 = fmaxf(M1, red[i].x);
+    M2 = fmaxf(M2, red[i].y);
+  }
+  const float U1 = M1 == -CUDART_INF_F ? 0.0f : M1, U2 = M2 == -CUDART_INF_F ? 0.0f : M2;
+  for (int s = tid; s < a.nsplit; s += JOIN_THREADS) {
+    const float4 v = w[s];
+    const float w1 = ex2(v.x - U1), w2 = ex2(v.z - U2);
+    w[s] = make_float4(w1, w2, w1 * v.y, w2 * v.w);
+  }
+  __syncthreads();
+  const int col = tid % W, grp = tid / W;
+  float x = 0.0f, y = 0.0f;
+#pragma unroll 8
+  for (int s = grp; s < a.nsplit; s += GROUPS) {
+    const float* q = a.part + (s * total + idx) * (2 * W) + col;
+    x += w[s].x * q[0];
+    y += w[s].y * q[W];
+  }
+  acc[grp][col] = make_float2(x, y);
+  __syncthreads();
+  if (tid >= W) return;
+  float L1 = 0.0f, L2 = 0.0f;
+  for (int s = 0; s < a.nsplit; s++) {
+    L1 += w[s].z;
+    L2 += w[s].w;
+  }
+  x = y = 0.0f;
+#pragma unroll
+  for (int k = 0; k < GROUPS; k++) {
+    x += acc[k][col].x;
+    y += acc[k][col].y;
   }
   const int e = p / a.tq, i = p - e * a.tq;
   const int head = kvh * a.grp + e;
   const float i1 = L1 > 0.0f ? 1.0f / L1 : 0.0f, i2 = L2 > 0.0f ? 1.0f / L2 : 0.0f;
-  const float lm = __ldg(a.lam + head);
-  T* o = static_cast<T*>(a.o) + b * a.ob + head * a.oh + i * a.orow;
-  T* o2 = a.o2 ? static_cast<T*>(a.o2) + ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) : nullptr;
-#pragma unroll
-  for (int c = 0; c < C; c++) {
-    const int col = lane + 32 * c;
-    if (col >= 2 * a.dh) continue;
-    o[col] = from_f<T>(x[c] * i1 - lm * (y[c] * i2));
-    if (o2) o2[col] = from_f<T>(y[c] * i2);
+  if (col < 2 * a.dh) {
+    static_cast<T*>(a.o)[b * a.ob + head * a.oh + i * a.orow + col] = from_f<T>(x * i1 - __ldg(a.lam + head) * (y * i2));
+    if (a.o2)
+      static_cast<T*>(a.o2)[((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + col] =
+          from_f<T>(y * i2);
   }
-  if (a.lse && lane == 0) {
+  if (a.lse && tid == 0) {
     float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
     s[0] = L1 > 0.0f ? M1 + log2f(L1) : CUDART_INF_F;
     s[a.tq] = L2 > 0.0f ? M2 + log2f(L2) : CUDART_INF_F;
   }
+}
+
+template <class T, int W>
+int join_launch(rnn_ctx* ctx, const Args& a) {
+  const long long rows = static_cast<long long>(a.n) * a.h * a.tq;
+  RNN_REQUIRE(rows < (1ll << 31) && a.nsplit <= JOIN_PARTS, "diffattn: too many rows or parts to join");
+  join_kernel<T, W><<<static_cast<unsigned>(rows), JOIN_THREADS, 0, ctx->stream>>>(a);
+  RNN_CHECK_LAUNCH();
+  return RNN_OK;
 }
 
 // ----------------------------------------------------------------- backward
@@ -621,11 +647,9 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
         for (int nb = 0; nb < NS; nb += 2) {
           typename FR::B f[2];
           FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma(s1[nb], q1, f[0]);
-          FR::mma(s1[nb + 1], q1, f[1]);
+          FR::mma2(s1[nb], s1[nb + 1], q1, f);
           FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma(s2[nb], q2, f[0]);
-          FR::mma(s2[nb + 1], q2, f[1]);
+          FR::mma2(s2[nb], s2[nb + 1], q2, f);
         }
       }
 #pragma unroll
@@ -635,8 +659,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
         for (int nb = 0; nb < NS; nb += 2) {
           typename FR::B f[2];
           FR::ldB2_nk(f, v, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma(dp[nb], g, f[0]);
-          FR::mma(dp[nb + 1], g, f[1]);
+          FR::mma2(dp[nb], dp[nb + 1], g, f);
         }
       }
       const bool edge = mask != nullptr || j0 + SUB > full;
@@ -688,8 +711,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
           for (int ks = 0; ks < SUB / KS; ks++) {
             typename FR::B f[2];
             FR::ldB2_kn(f, k, PITCH, s0 + ks * KS, nb * 8, lane);
-            FR::mma(x[0], ds[ks], f[0]);
-            FR::mma(x[1], ds[ks], f[1]);
+            FR::mma2(x[0], x[1], ds[ks], f);
           }
 #pragma unroll
           for (int i = 0; i < 2; i++)
@@ -869,11 +891,9 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
         for (int nb = 0; nb < NS; nb += 2) {
           typename FR::B f[2];
           FR::ldB2_nk(f, q, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma(s1[nb], k1, f[0]);
-          FR::mma(s1[nb + 1], k1, f[1]);
+          FR::mma2(s1[nb], s1[nb + 1], k1, f);
           FR::ldB2_nk(f, q, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma(s2[nb], k2, f[0]);
-          FR::mma(s2[nb + 1], k2, f[1]);
+          FR::mma2(s2[nb], s2[nb + 1], k2, f);
         }
       }
 #pragma unroll
@@ -883,8 +903,7 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
         for (int nb = 0; nb < NS; nb += 2) {
           typename FR::B f[2];
           FR::ldB2_nk(f, g, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma(dp[nb], x, f[0]);
-          FR::mma(dp[nb + 1], x, f[1]);
+          FR::mma2(dp[nb], dp[nb + 1], x, f);
         }
       }
       // after this: s1 = dS_1, s2 = dS_2, dp = P_1 - lam P_2 (transposed)
@@ -914,8 +933,7 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
           for (int ks = 0; ks < SUB / KS; ks++) {
             typename FR::B w[2];
             FR::ldB2_kn(w, src, PITCH, s0 + ks * KS, nb * 8, lane);
-            FR::mma(x[0], f[ks], w[0]);
-            FR::mma(x[1], f[ks], w[1]);
+            FR::mma2(x[0], x[1], f[ks], w);
           }
 #pragma unroll
           for (int i = 0; i < 2; i++)
@@ -982,11 +1000,7 @@ int fwd_launch(rnn_ctx* ctx, Args a) {
   }
   fwd_kernel<T, DH, RW><<<dim3(static_cast<unsigned>(blocks), a.nsplit), THREADS, F::SMEM, ctx->stream>>>(a);
   RNN_CHECK_LAUNCH();
-  if (a.nsplit > 1) {
-    join_kernel<T, F::G::W><<<static_cast<unsigned>((nbh * rows + 3) / 4), THREADS, 0, ctx->stream>>>(a);
-    RNN_CHECK_LAUNCH();
-  }
-  return RNN_OK;
+  return a.nsplit > 1 ? join_launch<T, F::G::W>(ctx, a) : RNN_OK;
 }
 
 template <class T, int DH>
@@ -1118,12 +1132,7 @@ bool aligned(std::initializer_list<const void*> ps, size_t bytes) {
 
 }  // namespace
 
-int join_parts(rnn_ctx* ctx, const Args& a) {
-  const long long rows = static_cast<long long>(a.n) * a.h * a.tq;
-  join_kernel<__nv_bfloat16, 128><<<static_cast<unsigned>((rows + 3) / 4), THREADS, 0, ctx->stream>>>(a);
-  RNN_CHECK_LAUNCH();
-  return RNN_OK;
-}
+int join_parts(rnn_ctx* ctx, const Args& a) { return join_launch<__nv_bfloat16, 128>(ctx, a); }
 
 }  // namespace diff
 }  // namespace rnn

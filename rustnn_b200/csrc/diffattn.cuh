@@ -166,10 +166,19 @@ struct Frag<__nv_bfloat16> {
               pack(c[2 * ks + 1][0], c[2 * ks + 1][1]), pack(c[2 * ks + 1][2], c[2 * ks + 1][3])}};
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const A& a, const B& b) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x[0]), "r"(a.x[1]), "r"(a.x[2]), "r"(a.x[3]), "r"(b.x[0]), "r"(b.x[1]));
+  }
+  // two products with one A operand; four with two
+  static __device__ __forceinline__ void mma2(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
+    mma(d0, a, b[0]);
+    mma(d1, a, b[1]);
+  }
+  static __device__ __forceinline__ void mma4(float (&d)[2][4], float (&e)[2][4], const A& a, const A& c,
+                                              const B (&b)[2]) {
+    mma2(d[0], d[1], a, b);
+    mma2(e[0], e[1], c, b);
   }
 };
 
@@ -222,15 +231,34 @@ struct Frag<float> {
     return a;
   }
   static __device__ __forceinline__ void mma1(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
   }
-  static __device__ __forceinline__ void mma(float (&d)[4], const A& a, const B& b) {
-    mma1(d, a.lo, b.hi);
-    mma1(d, a.hi, b.lo);
-    mma1(d, a.hi, b.hi);
+  // The three parts of a product depend on one another; several products take
+  // turns so that none waits for its own last part.
+  static __device__ __forceinline__ void mma2(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
+    mma1(d0, a.lo, b[0].hi);
+    mma1(d1, a.lo, b[1].hi);
+    mma1(d0, a.hi, b[0].lo);
+    mma1(d1, a.hi, b[1].lo);
+    mma1(d0, a.hi, b[0].hi);
+    mma1(d1, a.hi, b[1].hi);
+  }
+  static __device__ __forceinline__ void mma4(float (&d)[2][4], float (&e)[2][4], const A& a, const A& c,
+                                              const B (&b)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) mma1(d[i], a.lo, b[i].hi);
+#pragma unroll
+    for (int i = 0; i < 2; i++) mma1(e[i], c.lo, b[i].hi);
+#pragma unroll
+    for (int i = 0; i < 2; i++) mma1(d[i], a.hi, b[i].lo);
+#pragma unroll
+    for (int i = 0; i < 2; i++) mma1(e[i], c.hi, b[i].lo);
+#pragma unroll
+    for (int i = 0; i < 2; i++) mma1(d[i], a.hi, b[i].hi);
+#pragma unroll
+    for (int i = 0; i < 2; i++) mma1(e[i], c.hi, b[i].hi);
   }
 };
 
