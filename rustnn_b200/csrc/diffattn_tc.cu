@@ -5,8 +5,10 @@
 // thread per query, that take the 64-key tiles alternately, so that the
 // exponentials of one team (the bound: two per query and key, 16 a clock and SM)
 // run while the tensor cores form scores and the products with v for the other.
-// Warp 8 copies tiles, warp 9 issues MMAs, warp 10 clears what lies beyond a
-// sequence's length.  Tensor memory (512 columns):
+// Warp 8 copies tiles; warps 9 and 10 issue MMAs, 10 the scores of the first map,
+// 9 the others (an issuing warp stalls while the tensor cores are busy, and one
+// warp alone left them idle at each of its waits); warp 11 clears what lies
+// beyond a sequence's length.  Tensor memory (512 columns):
 //   [0, 128)    A = sum (P_1 - r P_2) v        [128, 256)  B = sum P_2 v
 //   [256, 384)  S_1 | S_2 of even tiles        [384, 512)  the same of odd tiles
 // The bf16 maps overwrite S_2 alone: S_1 of a team's next tile is formed as soon
@@ -71,7 +73,7 @@ namespace {
 
 constexpr int QROWS = 128, KEYS = 64, STAGES = 5;
 constexpr int FWD_THREADS = 384;
-constexpr int SOFT_WARPS = 8, WARP_COPY = 8, WARP_MMA = 9, WARP_CLEAR = 10;
+constexpr int SOFT_WARPS = 8, WARP_COPY = 8, WARP_MMA = 9, WARP_SCORE = 10, WARP_CLEAR = 11;
 constexpr uint32_t Q_BYTES = 2 * QROWS * 128;      // two halves, rows of 128 bytes
 constexpr uint32_t HALF_BYTES = KEYS * 128;        // one half of k, or 64 columns of v
 constexpr uint32_t STAGE_BYTES = 4 * HALF_BYTES;   // k halves, then v columns
@@ -87,7 +89,7 @@ struct alignas(64) FwdParams {
 
 struct FwdShared {
   uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], last_full, s1_full[2], s2_full[2], s1_free[2], p_full[2];
-  uint64_t pv_last, o_full, tok[4], drain;
+  uint64_t pv_last, o_full, tok[4], drain[2];
   uint32_t tmem;
   int abort_flag;
   float4 ref[QROWS];     // a row's m_1, m_2, r
@@ -227,7 +229,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
     for (int i = 0; i < 4; i++) {
       mbar_init(&sh.tok[i], 1);
     }
-    mbar_init(&sh.drain, 1);
+    mbar_init(&sh.drain[0], 1);
+    mbar_init(&sh.drain[1], 1);
     sh.abort_flag = 0;
     fence_barrier_init();
   }
@@ -456,25 +459,42 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
           if (lane == 0) mbar_arrive(&sh.kv_full[st]);
         }
       }
-    } else if (warp == WARP_MMA) {
-      if (nt > 0) {
-        const uint32_t lead = elect_one() ? 1u : 0u;
-        const uint32_t id_s = idesc_bf16(QROWS, KEYS, false), id_o = idesc_bf16(QROWS, 64, true);
-        const uint64_t dq = desc_k(sq), dkv = desc_k(skv), dv = desc_mn(skv + 2 * HALF_BYTES, 0);
-        auto done = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, dev_error); };
-        // scores of one map of tile j (stage st); descriptors count 16 bytes
-        auto scores = [&](int j, int st, int half) {
-          tc_fence_after();
-          const uint64_t q = dq + half * (QROWS * 128 / 16), k = dkv + (st * STAGE_BYTES + half * HALF_BYTES) / 16;
-          const uint32_t d = tmem + COL_S + (j & 1) * 128 + half * KEYS;
+    } else if (nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      const uint32_t id_s = idesc_bf16(QROWS, KEYS, false);
+      const uint64_t dq = desc_k(sq), dkv = desc_k(skv);
+      auto done = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, dev_error); };
+      auto landed = [&](int j, int st) { return done(&sh.kv_full[st], (j / STAGES) & 1); };
+      // scores of one map of tile j (stage st); descriptors count 16 bytes
+      auto scores = [&](int j, int st, int half) {
+        const uint64_t q = dq + half * (QROWS * 128 / 16), k = dkv + (st * STAGE_BYTES + half * HALF_BYTES) / 16;
+        const uint32_t d = tmem + COL_S + (j & 1) * 128 + half * KEYS;
 #pragma unroll
-          for (int ks = 0; ks < 4; ks++)
-            if (ks < ksteps) mma_ss(d, q + ks * 2, k + ks * 2, id_s, ks > 0, lead);
-          commit(half ? &sh.s2_full[j & 1] : &sh.s1_full[j & 1], lead);
-        };
-        auto landed = [&](int j, int st) { return done(&sh.kv_full[st], (j / STAGES) & 1); };
-        // products of tile j with v
-        auto products = [&](int j, int st) {
+        for (int ks = 0; ks < 4; ks++)
+          if (ks < ksteps) mma_ss(d, q + ks * 2, k + ks * 2, id_s, ks > 0, lead);
+        commit(half ? &sh.s2_full[j & 1] : &sh.s1_full[j & 1], lead);
+      };
+      bool ok = done(&sh.q_full, 0);
+      int st = 0;
+      if (warp == WARP_SCORE) {
+        for (int j = 0; ok && j < nt; j++) {
+          // the team has the scores of tile j - 2 in registers
+          if (!(ok = landed(j, st) && (j < 2 || done(&sh.s1_free[j & 1], ((j >> 1) - 1) & 1)))) break;
+          tc_fence_after();
+          scores(j, st, 0);
+          if (++st == STAGES) st = 0;
+        }
+      } else {
+        const uint32_t id_o = idesc_bf16(QROWS, 64, true);
+        const uint64_t dv = desc_mn(skv + 2 * HALF_BYTES, 0);
+        for (int j = 0; ok && j < min(nt, 2); j++)
+          if ((ok = landed(j, j))) {
+            tc_fence_after();
+            scores(j, j, 1);
+          }
+        int st2 = 2;
+        for (int j = 0; ok && j < nt; j++) {
+          if (!(ok = (j + 2 >= nt || landed(j + 2, st2)) && done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
           tc_fence_after();
           const uint64_t v = dv + st * (STAGE_BYTES / 16);
           const uint32_t s = tmem + COL_S + (j & 1) * 128 + KEYS;
@@ -486,38 +506,22 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
               mma_ts(tmem + COL_B + c * 64, s + 32 + ks * 8, d, id_o, j > 0 || ks > 0, lead);
             }
           }
+          // the scores of tile j are long done: its maps came of them
           commit(&sh.kv_empty[st], lead);
-        };
-        bool ok = done(&sh.q_full, 0);
-        for (int j = 0; ok && j < min(nt, 2); j++)
-          if ((ok = landed(j, j))) {
-            scores(j, j, 0);
-            scores(j, j, 1);
-          }
-        int j = 0, st = 0, st2 = 2;  // stages of tiles j and j + 2
-        for (; ok && j + 2 < nt; j++) {
-          const uint32_t par = (j >> 1) & 1;
-          if (!(ok = landed(j + 2, st2) && done(&sh.s1_free[j & 1], par))) break;
-          scores(j + 2, st2, 0);
-          if (!(ok = done(&sh.p_full[j & 1], par))) break;
-          products(j, st);
+          if (j + 2 == nt) commit(&sh.pv_last, lead);
+          if (j + 1 == nt) commit(&sh.o_full, lead);
           // The next scores of the second map overwrite the maps that these
-          // products read.  All MMAs here have one accumulator shape (128 x 64),
-          // which makes them execute in the order they are issued in.
-          scores(j + 2, st2, 1);
+          // products read.  This warp's MMAs have one accumulator shape
+          // (128 x 64), which makes them execute in the order of issue.
+          if (j + 2 < nt) scores(j + 2, st2, 1);
           if (++st == STAGES) st = 0;
           if (++st2 == STAGES) st2 = 0;
         }
-        for (; ok && j < nt; j++) {
-          if (!(ok = done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
-          products(j, st);
-          commit(j + 1 == nt ? &sh.o_full : &sh.pv_last, lead);
-          if (++st == STAGES) st = 0;
-        }
-        if (!ok) {  // no MMA may write tensor memory after it is released
-          commit(&sh.drain, lead);
-          settle(&sh.drain, 0);
-        }
+      }
+      if (!ok) {  // no MMA may write tensor memory after it is released
+        uint64_t* drain = &sh.drain[warp == WARP_SCORE];
+        commit(drain, lead);
+        settle(drain, 0);
       }
       __syncwarp();
     }

@@ -6,9 +6,11 @@
 //
 // 16 warps turn scores into dS, 16 columns of a row at a time: with the saved
 // log-sums no thread needs another's values, so a row is shared by four of
-// them.  Warp 16 copies tiles, warp 17 issues MMAs, warp 18 clears what lies
-// beyond a sequence's length (queries' kernel) or brings the queries' log-sums
-// and D (keys' kernel), warp 19 sums dlam.
+// them.  Warp 16 copies tiles (and in the keys' kernel brings the queries'
+// log-sums and D).  Two warps issue MMAs, 17 the products with dS and dP, 18 the
+// scores: an issuing warp stalls while the tensor cores are busy, and one warp
+// alone left them idle at each of its waits.  Warp 19 clears what lies beyond a
+// sequence's length (queries' kernel) or sums dlam (keys' kernel).
 #include <algorithm>
 
 #include "diffattn_tc.cuh"
@@ -17,7 +19,7 @@ namespace rnn {
 namespace diff {
 namespace {
 
-constexpr int THREADS = 640, SOFT = 16, WARP_COPY = 16, WARP_MMA = 17, WARP_AUX = 18, WARP_SUM = 19;
+constexpr int THREADS = 640, SOFT = 16, WARP_COPY = 16, WARP_MMA = 17, WARP_SCORE = 18, WARP_AUX = 19;
 constexpr int ROWS = 128, COLS = 64;               // a block's rows, a tile's columns
 constexpr uint32_t BIG = ROWS * 128, SMALL = COLS * 128;  // 64-column parts of a 128- and a 64-row tile, bytes
 
@@ -47,15 +49,18 @@ __device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&v)[16], 
 
 // ------------------------------------------------------------------ queries
 //
-// Tensor memory: dq_1 | dq_2 at [0, 128); S_1 | S_2 | dP of even tiles at
-// [128, 320), of odd ones at [320, 512).  dS overwrites the scores in place:
-// the 32 keys of one half of a tile become 16 words at the head of their own
-// columns.
+// Two teams of 8 warps take the tiles alternately.  Tensor memory: dq_1 | dq_2
+// at [0, 128); S_1 | S_2 | dP of even tiles at [128, 320), of odd ones at
+// [320, 512).  dS takes the place of dP (16 keys of both maps: the 16 columns
+// that their dP had), so that the scores of a team's next tile are formed as
+// soon as this one's are in registers; only its dP waits for the products with
+// dS, behind the exponentials.
 
 constexpr int Q_STAGES = 4;
 constexpr uint32_t Q_STAGE = 4 * SMALL;  // k halves, v parts
 struct QShared {
-  uint64_t q_full, kv_full[Q_STAGES], kv_empty[Q_STAGES], last_full, s_full[2], p_full[2], o_full, drain;
+  uint64_t q_full, kv_full[Q_STAGES], kv_empty[Q_STAGES], last_full, s_full[2], s_free[2], d_full[2], p_full[2];
+  uint64_t o_full, drain[2];
   uint32_t tmem;
   int abort_flag;
   float2 part[4][ROWS];
@@ -92,10 +97,13 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     mbar_init(&sh.last_full, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.s_free[i], 8);
+      mbar_init(&sh.d_full[i], 1);
       mbar_init(&sh.p_full[i], 8);
     }
     mbar_init(&sh.o_full, 1);
-    mbar_init(&sh.drain, 1);
+    mbar_init(&sh.drain[0], 1);
+    mbar_init(&sh.drain[1], 1);
     sh.abort_flag = 0;
     fence_barrier_init();
   }
@@ -124,13 +132,11 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     const f32x2 cc = pair(c2, c2), n1 = pair(-ls1, -ls1), n2 = pair(-ls2, -ls2);
 
     // both maps' entries of 16 columns from the scores
-    auto maps = [&](uint32_t t, float (&x)[16], float (&y)[16], float (&dp)[16], int visible, bool edge) {
+    auto maps = [&](uint32_t t, float (&x)[16], float (&y)[16], int visible, bool edge) {
       tmem_ld(t, x);
       tmem_ld(t + 64, y);
-      tmem_ld(t + 128, dp);
       tmem_landed(x);
       tmem_landed(y);
-      tmem_landed(dp);
 #pragma unroll
       for (int c = 0; c < 16; c += 2) {
         unpair(fma2(pair(x[c], x[c + 1]), cc, n1), x[c], x[c + 1]);
@@ -178,11 +184,14 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       }
     } else if (team < nt) {
       warp_wait(&sh.s_full[team], 0, abort_flag, dev_error);
+      warp_wait(&sh.d_full[team], 0, abort_flag, dev_error);
       tc_fence_after();
 #pragma unroll 1
       for (int c = 0; c < 32; c += 16) {
         float x[16], y[16], dp[16];
-        maps(ts + c, x, y, dp, lim - team * COLS - c, true);
+        maps(ts + c, x, y, lim - team * COLS - c, true);
+        tmem_ld(ts + 128 + c, dp);
+        tmem_landed(dp);
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           d1 += x[e] * dp[e];
@@ -207,26 +216,40 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     const f32x2 e1 = pair(-d1, -d1), e2 = pair(-d2, -d2);
     f32x2 dl = 0ull;
     for (int j = team; j < nt; j += 2) {
-      if (!warp_wait(&sh.s_full[team], (j >> 1) & 1, abort_flag, dev_error)) break;
-      tc_fence_after();
+      const uint32_t par = (j >> 1) & 1;
       const bool edge = j * COLS + 32 > full;
+      float x[2][16], y[2][16];
+      if (!warp_wait(&sh.s_full[team], par, abort_flag, dev_error)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; c++) maps(ts + c * 16, x[c], y[c], lim - j * COLS - c * 16, edge);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.s_free[team]);
+      if (!warp_wait(&sh.d_full[team], par, abort_flag, dev_error)) break;
+      tc_fence_after();
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        float x[16], y[16], dp[16];
-        maps(ts + c * 16, x, y, dp, lim - j * COLS - c * 16, edge);
         uint32_t u[8], v[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const f32x2 g = pair(dp[2 * e], dp[2 * e + 1]), y2 = pair(y[2 * e], y[2 * e + 1]);
-          dl = fma2(y2, g, dl);
-          float r0, r1;
-          unpair(mul2(pair(x[2 * e], x[2 * e + 1]), add2(g, e1)), r0, r1);
-          u[e] = pack2(r0, r1);
-          unpair(mul2(y2, add2(g, e2)), r0, r1);
-          v[e] = pack2(r0, r1);
+        for (int h = 0; h < 2; h++) {
+          float dp[8];
+          tmem_ld(ts + 128 + c * 16 + h * 8, dp);
+          tmem_landed(dp);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int k = h * 4 + e;
+            const f32x2 g = pair(dp[2 * e], dp[2 * e + 1]), y2 = pair(y[c][2 * k], y[c][2 * k + 1]);
+            dl = fma2(y2, g, dl);
+            float r0, r1;
+            unpair(mul2(pair(x[c][2 * k], x[c][2 * k + 1]), add2(g, e1)), r0, r1);
+            u[k] = pack2(r0, r1);
+            unpair(mul2(y2, add2(g, e2)), r0, r1);
+            v[k] = pack2(r0, r1);
+          }
         }
-        tmem_st(ts + c * 8, u);
-        tmem_st(ts + 64 + c * 8, v);
+        tmem_st(ts + 128 + c * 16, u);
+        tmem_st(ts + 128 + c * 16 + 8, v);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -298,58 +321,73 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
           if (lane == 0) mbar_arrive(&sh.kv_full[st]);
         }
       }
-    } else if (warp == WARP_MMA && nt > 0) {
+    } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
-      // one accumulator shape for all: MMAs then execute in the order of issue,
-      // and the next scores may overwrite dS right after the products with it
-      const uint32_t id_s = idesc_bf16(ROWS, 64, false), id_o = idesc_bf16(ROWS, 64, true);
-      const uint64_t dq = desc_k(sq), dg = desc_k(sg), dkv = desc_k(skv), dmn = desc_mn(skv, 0);
+      const uint32_t id_s = idesc_bf16(ROWS, 64, false);
       auto done = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, dev_error); };
       auto landed = [&](int j, int st) { return done(&sh.kv_full[st], (j / Q_STAGES) & 1); };
-      auto scores = [&](int j, int st) {
-        tc_fence_after();
-        const uint64_t kv = dkv + st * (Q_STAGE / 16);
-        const uint32_t d = tmem + 128 + (j & 1) * 192;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int ks = 0; ks < 4; ks++)
-            if (ks < ksteps)
-              mma_ss(d + h * 64, dq + (h * BIG + ks * 32) / 16, kv + (h * SMALL + ks * 32) / 16, id_s, ks > 0, lead);
-#pragma unroll
-        for (int ks = 0; ks < 8; ks++)
-          if (ks < dsteps)
-            mma_ss(d + 128, dg + ((ks >> 2) * BIG + (ks & 3) * 32) / 16,
-                   kv + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
-        commit(&sh.s_full[j & 1], lead);
-      };
       bool ok = done(&sh.q_full, 0);
-      for (int j = 0; ok && j < min(nt, 2); j++)
-        if ((ok = landed(j, j))) scores(j, j);
-      int st = 0, st2 = 2;
-      for (int j = 0; ok && j < nt; j++) {
-        if (!(ok = done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
-        tc_fence_after();
-        const uint64_t k = dmn + st * (Q_STAGE / 16);
-        const uint32_t s = tmem + 128 + (j & 1) * 192;
+      int st = 0;
+      if (warp == WARP_SCORE) {
+        const uint64_t dq = desc_k(sq), dkv = desc_k(skv);
+        for (int j = 0; ok && j < nt; j++) {
+          // the team has the scores of tile j - 2 in registers
+          if (!(ok = landed(j, st) && (j < 2 || done(&sh.s_free[j & 1], ((j >> 1) - 1) & 1)))) break;
+          tc_fence_after();
+          const uint64_t kv = dkv + st * (Q_STAGE / 16);
+          const uint32_t d = tmem + 128 + (j & 1) * 192;
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+          for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int ks = 0; ks < 4; ks++)
-            mma_ts(tmem + m * 64, s + m * 64 + (ks >> 1) * 32 + (ks & 1) * 8, k + (m * SMALL + ks * 2048) / 16, id_o,
-                   j > 0 || ks > 0, lead);
-        commit(&sh.kv_empty[st], lead);
-        if (j + 1 == nt) commit(&sh.o_full, lead);
-        if (j + 2 < nt) {
-          if (!(ok = landed(j + 2, st2))) break;
-          scores(j + 2, st2);
+            for (int ks = 0; ks < 4; ks++)
+              if (ks < ksteps)
+                mma_ss(d + h * 64, dq + (h * BIG + ks * 32) / 16, kv + (h * SMALL + ks * 32) / 16, id_s, ks > 0, lead);
+          commit(&sh.s_full[j & 1], lead);
+          if (++st == Q_STAGES) st = 0;
         }
-        if (++st == Q_STAGES) st = 0;
-        if (++st2 == Q_STAGES) st2 = 0;
+      } else {
+        // One accumulator shape: MMAs of a thread then execute in the order of
+        // issue, and the next dP may take the place of dS right after the
+        // products with it.
+        const uint32_t id_o = idesc_bf16(ROWS, 64, true);
+        const uint64_t dg = desc_k(sg), dkv = desc_k(skv), dmn = desc_mn(skv, 0);
+        auto slopes = [&](int j, int s1) {
+          const uint64_t kv = dkv + s1 * (Q_STAGE / 16);
+#pragma unroll
+          for (int ks = 0; ks < 8; ks++)
+            if (ks < dsteps)
+              mma_ss(tmem + 256 + (j & 1) * 192, dg + ((ks >> 2) * BIG + (ks & 3) * 32) / 16,
+                     kv + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
+          commit(&sh.d_full[j & 1], lead);
+        };
+        for (int j = 0; ok && j < min(nt, 2); j++)
+          if ((ok = landed(j, j))) {
+            tc_fence_after();
+            slopes(j, j);
+          }
+        int st2 = 2;
+        for (int j = 0; ok && j < nt; j++) {
+          if (!(ok = (j + 2 >= nt || landed(j + 2, st2)) && done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
+          tc_fence_after();
+          const uint64_t k = dmn + st * (Q_STAGE / 16);
+          const uint32_t s = tmem + 256 + (j & 1) * 192;
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++)
+              mma_ts(tmem + m * 64, s + ks * 16 + m * 8, k + (m * SMALL + ks * 2048) / 16, id_o, j > 0 || ks > 0, lead);
+          // the scores of tile j are long done: dS came of them
+          commit(&sh.kv_empty[st], lead);
+          if (j + 1 == nt) commit(&sh.o_full, lead);
+          if (j + 2 < nt) slopes(j + 2, st2);
+          if (++st == Q_STAGES) st = 0;
+          if (++st2 == Q_STAGES) st2 = 0;
+        }
       }
       if (!ok) {  // no MMA may write tensor memory after it is released
-        commit(&sh.drain, lead);
-        settle(&sh.drain, 0);
+        uint64_t* drain = &sh.drain[warp == WARP_SCORE];
+        commit(drain, lead);
+        settle(drain, 0);
       }
       __syncwarp();
     }
@@ -363,28 +401,32 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
 
 // --------------------------------------------------------------------- keys
 //
-// Rows are keys, columns the queries of a tile.  Tensor memory: dv at [0, 128),
-// dk_1 | dk_2 at [128, 256), S_1 | S_2 | dP at [256, 448), dS_1 | dS_2 (bf16) at
-// [448, 512).  The combined map, operand of dv, goes through shared memory.
+// Rows are keys, columns the queries of a tile; all 16 warps share a tile.
+// Tensor memory: dv at [0, 128), dk_1 | dk_2 at [128, 256), S_1 | S_2 at
+// [256, 384), dP of even tiles at [384, 448), of odd ones at [448, 512), with dS
+// in its place (16 queries of both maps: the 16 columns that their dP had).  The
+// combined map, operand of dv, goes through shared memory, two tiles' worth.
 // The scores are read into registers at once, so that the next tile's are
-// formed while this one's exponentials are taken.
+// formed while this one's exponentials are taken, and no warp waits for the
+// products of the tile before.
 
-constexpr int K_STAGES = 4;
+constexpr int K_STAGES = 3;
 constexpr uint32_t K_STAGE = 4 * SMALL;  // q halves, dout parts
 struct KShared {
-  uint64_t kv_full, q_full[K_STAGES], q_empty[K_STAGES], s_full, s_free, p_full, pv, o_full, drain;
+  uint64_t kv_full, q_full[K_STAGES], q_empty[K_STAGES], s_full, s_free, d_full[2], p_full[2], pv[2];
+  uint64_t o_full, drain[2];
   uint32_t tmem;
   int abort_flag;
-  float st[K_STAGES][4][COLS];  // -lse_1, -lse_2, -D_1, -D_2 of a tile's queries
+  alignas(16) float st[K_STAGES][4][COLS];  // -lse_1, -lse_2, -D_1, -D_2 of a tile's queries
 };
-constexpr size_t K_SMEM = 1024 + 4 * BIG + K_STAGES * K_STAGE + BIG + sizeof(KShared);
+constexpr size_t K_SMEM = 1024 + 4 * BIG + K_STAGES * K_STAGE + 2 * BIG + sizeof(KShared);
 
 __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw[];
   const Args& a = p.a;
   uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   const uint32_t sk = smem_u32(base), sv = sk + 2 * BIG, sqg = sv + 2 * BIG, sp = sqg + K_STAGES * K_STAGE;
-  KShared& sh = *reinterpret_cast<KShared*>(base + 4 * BIG + K_STAGES * K_STAGE + BIG);
+  KShared& sh = *reinterpret_cast<KShared*>(base + 4 * BIG + K_STAGES * K_STAGE + 2 * BIG);
   volatile int* abort_flag = &sh.abort_flag;
   int* dev_error = p.dev_error;
 
@@ -416,10 +458,14 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
     }
     mbar_init(&sh.s_full, 1);
     mbar_init(&sh.s_free, SOFT);
-    mbar_init(&sh.p_full, SOFT);
-    mbar_init(&sh.pv, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh.d_full[i], 1);
+      mbar_init(&sh.p_full[i], SOFT);
+      mbar_init(&sh.pv[i], 1);
+    }
     mbar_init(&sh.o_full, 1);
-    mbar_init(&sh.drain, 1);
+    mbar_init(&sh.drain[0], 1);
+    mbar_init(&sh.drain[1], 1);
     sh.abort_flag = 0;
     fence_barrier_init();
   }
@@ -450,58 +496,79 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
       tc_fence_after();
       tmem_ld(ts, x);
       tmem_ld(ts + 64, y);
-      tmem_ld(ts + 128, dp);
       tmem_landed(x);
       tmem_landed(y);
-      tmem_landed(dp);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.s_free);
       const float* s = &sh.st[st][0][k4 * 16];
       const f32x2 ll = pair(-lam, -lam);
+      // the first query that sees this key
+      int first = 0;
+      if (a.causal) first = (a.causal == RNN_CAUSAL_START ? key : key - (len - a.tq)) - (q0 + k4 * 16);
+      const bool edge = __any_sync(0xffffffffu, first > 0);
+      auto exps = [&](int c0) {
 #pragma unroll
-      for (int c = 0; c < 16; c += 2) {
-        unpair(fma2(pair(x[c], x[c + 1]), cc, *reinterpret_cast<const f32x2*>(s + c)), x[c], x[c + 1]);
-        unpair(fma2(pair(y[c], y[c + 1]), cc, *reinterpret_cast<const f32x2*>(s + COLS + c)), y[c], y[c + 1]);
-        x[c] = ex2(x[c]);
-        x[c + 1] = ex2(x[c + 1]);
-        y[c] = ex2(y[c]);
-        y[c + 1] = ex2(y[c + 1]);
-      }
-      if (a.causal) {
-        // the first query that sees this key
-        const int first = (a.causal == RNN_CAUSAL_START ? key : key - (len - a.tq)) - (q0 + k4 * 16);
-        if (__any_sync(0xffffffffu, first > 0)) {
+        for (int c = c0; c < c0 + 8; c += 4) {
+          const ulonglong2 n1 = *reinterpret_cast<const ulonglong2*>(s + c);
+          const ulonglong2 n2 = *reinterpret_cast<const ulonglong2*>(s + COLS + c);
+          unpair(fma2(pair(x[c], x[c + 1]), cc, n1.x), x[c], x[c + 1]);
+          unpair(fma2(pair(y[c], y[c + 1]), cc, n2.x), y[c], y[c + 1]);
+          unpair(fma2(pair(x[c + 2], x[c + 3]), cc, n1.y), x[c + 2], x[c + 3]);
+          unpair(fma2(pair(y[c + 2], y[c + 3]), cc, n2.y), y[c + 2], y[c + 3]);
 #pragma unroll
-          for (int c = 0; c < 16; c++)
+          for (int k = c; k < c + 4; k++) {
+            x[k] = ex2(x[k]);
+            y[k] = ex2(y[k]);
+          }
+        }
+        if (__builtin_expect(edge, 0)) {
+#pragma unroll
+          for (int c = c0; c < c0 + 8; c++)
             if (c < first) x[c] = y[c] = 0.0f;
         }
-      }
+      };
       uint32_t u[8], v[8], z[8];
+      ulonglong2 e1, e2;  // -D_1, -D_2 of four queries
+      auto grads = [&](int c0) {
 #pragma unroll
-      for (int c = 0; c < 8; c++) {
-        const f32x2 g = pair(dp[2 * c], dp[2 * c + 1]), x2 = pair(x[2 * c], x[2 * c + 1]);
-        const f32x2 y2 = mul2(pair(y[2 * c], y[2 * c + 1]), ll);  // -lam P_2
-        float r0, r1;
-        unpair(mul2(x2, add2(g, *reinterpret_cast<const f32x2*>(s + 2 * COLS + 2 * c))), r0, r1);
-        u[c] = pack2(r0, r1);
-        unpair(mul2(y2, add2(g, *reinterpret_cast<const f32x2*>(s + 3 * COLS + 2 * c))), r0, r1);
-        v[c] = pack2(r0, r1);
-        unpair(add2(x2, y2), r0, r1);
-        z[c] = pack2(r0, r1);
-      }
-      // the products of the tile before have read the operands
-      if (t > 0 && !warp_wait(&sh.pv, (t - 1) & 1, abort_flag, dev_error)) break;
+        for (int c = c0 / 2; c < c0 / 2 + 4; c++) {
+          if ((c & 1) == 0) {
+            e1 = *reinterpret_cast<const ulonglong2*>(s + 2 * COLS + 2 * c);
+            e2 = *reinterpret_cast<const ulonglong2*>(s + 3 * COLS + 2 * c);
+          }
+          const f32x2 g = pair(dp[2 * c], dp[2 * c + 1]), x2 = pair(x[2 * c], x[2 * c + 1]);
+          const f32x2 y2 = mul2(pair(y[2 * c], y[2 * c + 1]), ll);  // -lam P_2
+          float r0, r1;
+          unpair(mul2(x2, add2(g, c & 1 ? e1.y : e1.x)), r0, r1);
+          u[c] = pack2(r0, r1);
+          unpair(mul2(y2, add2(g, c & 1 ? e2.y : e2.x)), r0, r1);
+          v[c] = pack2(r0, r1);
+          unpair(add2(x2, y2), r0, r1);
+          z[c] = pack2(r0, r1);
+        }
+      };
+      exps(0);
+      exps(8);
+      const uint32_t par = (t >> 1) & 1, td = ts + 128 + (t & 1) * 64;
+      if (!warp_wait(&sh.d_full[t & 1], par, abort_flag, dev_error)) break;
       tc_fence_after();
-      *reinterpret_cast<uint4*>(pc + ch0) = make_uint4(z[0], z[1], z[2], z[3]);
-      *reinterpret_cast<uint4*>(pc + ch1) = make_uint4(z[4], z[5], z[6], z[7]);
+      tmem_ld(td, dp);
+      tmem_landed(dp);
+      grads(0);
+      grads(8);
+      tmem_st(td, u);
+      tmem_st(td + 8, v);
+      // the products of two tiles ago have read the combined map's place
+      if (t > 1 && !warp_wait(&sh.pv[t & 1], par ^ 1, abort_flag, dev_error)) break;
+      uint8_t* pt = pc + (t & 1) * BIG;
+      *reinterpret_cast<uint4*>(pt + ch0) = make_uint4(z[0], z[1], z[2], z[3]);
+      *reinterpret_cast<uint4*>(pt + ch1) = make_uint4(z[4], z[5], z[6], z[7]);
       fence_async_smem();
-      tmem_st(tmem + lanes + 448 + k4 * 8, u);
-      tmem_st(tmem + lanes + 480 + k4 * 8, v);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full);
+      if (lane == 0) mbar_arrive(&sh.p_full[t & 1]);
       if (++st == K_STAGES) st = 0;
       q0 += COLS;
       if (q0 >= qbeg + per * COLS) {
@@ -538,19 +605,37 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == WARP_COPY) {
-      if (elect_one() && nt > 0) {
-        mbar_arrive_expect_tx(&sh.kv_full, (2 + wide) * BIG);
-        for (int h = 0; h < 2; h++) tma_5d(sk + h * BIG, &p.k, 0, h, kvh, key0, b, &sh.kv_full);
-        for (int c = 0; c < wide; c++) tma_5d(sv + c * BIG, &p.v, c * 64, 0, kvh, key0, b, &sh.kv_full);
+      if (nt > 0) {
+        const bool lead = elect_one();
+        if (lead) {
+          mbar_arrive_expect_tx(&sh.kv_full, (2 + wide) * BIG);
+          for (int h = 0; h < 2; h++) tma_5d(sk + h * BIG, &p.k, 0, h, kvh, key0, b, &sh.kv_full);
+          for (int c = 0; c < wide; c++) tma_5d(sv + c * BIG, &p.v, c * 64, 0, kvh, key0, b, &sh.kv_full);
+        }
         int t = 0;
         for (; t < nt; t++) {
           const int st = t % K_STAGES;
-          if (t >= K_STAGES && !wait(&sh.q_empty[st], (t / K_STAGES - 1) & 1, abort_flag, dev_error)) break;
+          if (t >= K_STAGES && !warp_wait(&sh.q_empty[st], (t / K_STAGES - 1) & 1, abort_flag, dev_error)) break;
           const uint32_t dst = sqg + st * K_STAGE;
           const int head = kvh * a.grp + t / per, i0 = qbeg + (t % per) * COLS;
-          mbar_arrive_expect_tx(&sh.q_full[st], (2 + wide) * SMALL);
-          for (int h = 0; h < 2; h++) tma_5d(dst + h * SMALL, &p.q, 0, h, head, i0, b, &sh.q_full[st]);
-          for (int c = 0; c < wide; c++) tma_5d(dst + (2 + c) * SMALL, &p.g, c * 64, 0, head, i0, b, &sh.q_full[st]);
+          if (lead) {
+            mbar_arrive_expect_tx(&sh.q_full[st], (2 + wide) * SMALL);
+            for (int h = 0; h < 2; h++) tma_5d(dst + h * SMALL, &p.q, 0, h, head, i0, b, &sh.q_full[st]);
+            for (int c = 0; c < wide; c++) tma_5d(dst + (2 + c) * SMALL, &p.g, c * 64, 0, head, i0, b, &sh.q_full[st]);
+          }
+          __syncwarp();
+          const long long at = (static_cast<long long>(b) * a.h + head) * 2 * a.tq;
+#pragma unroll
+          for (int c = lane; c < COLS; c += 32) {
+            const int i = i0 + c;
+            const bool in = i < a.tq;
+            sh.st[st][0][c] = in ? -a.flse[at + i] : -CUDART_INF_F;
+            sh.st[st][1][c] = in ? -a.flse[at + a.tq + i] : -CUDART_INF_F;
+            sh.st[st][2][c] = in ? -a.dsum[at + i] : 0.0f;
+            sh.st[st][3][c] = in ? -a.dsum[at + a.tq + i] : 0.0f;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.q_full[st]);
         }
         // what was asked for lands before the block may end, aborting or not
         settle(&sh.kv_full, 0);
@@ -558,24 +643,6 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
       }
       __syncwarp();
     } else if (warp == WARP_AUX) {
-      for (int t = 0; t < nt; t++) {
-        const int st = t % K_STAGES;
-        if (t >= K_STAGES && !warp_wait(&sh.q_empty[st], (t / K_STAGES - 1) & 1, abort_flag, dev_error)) break;
-        const int head = kvh * a.grp + t / per, i0 = qbeg + (t % per) * COLS;
-        const long long at = (static_cast<long long>(b) * a.h + head) * 2 * a.tq;
-#pragma unroll
-        for (int c = lane; c < COLS; c += 32) {
-          const int i = i0 + c;
-          const bool in = i < a.tq;
-          sh.st[st][0][c] = in ? -a.flse[at + i] : -CUDART_INF_F;
-          sh.st[st][1][c] = in ? -a.flse[at + a.tq + i] : -CUDART_INF_F;
-          sh.st[st][2][c] = in ? -a.dsum[at + i] : 0.0f;
-          sh.st[st][3][c] = in ? -a.dsum[at + a.tq + i] : 0.0f;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.q_full[st]);
-      }
-    } else if (warp == WARP_SUM) {
       // dlam: block `head` sums that head's rows in a fixed order
       if (static_cast<int>(blockIdx.x) < a.h && a.tq > 0) {
         const long long cnt = static_cast<long long>(a.n) * a.tq;
@@ -591,58 +658,82 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) a.dlam[blockIdx.x] -= static_cast<float>(sum);
       }
-    } else if (warp == WARP_MMA && nt > 0) {
+    } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
-      const uint32_t id_s = idesc_bf16(ROWS, 64, false), id_k = idesc_bf16(ROWS, 64, true),
-                     id_v = idesc_bf16(ROWS, 2 * a.dh, true);
-      const uint64_t dk = desc_k(sk), dv = desc_k(sv), dqg = desc_k(sqg), dp = desc_k(sp);
-      const uint64_t mq = desc_mn(sqg, 0), mg = desc_mn(sqg + 2 * SMALL, SMALL);
+      const uint32_t id_s = idesc_bf16(ROWS, 64, false);
       auto done = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag, dev_error); };
-      auto scores = [&](int st) {
-        tc_fence_after();
-        const uint64_t q = dqg + st * (K_STAGE / 16);
+      auto landed = [&](int t, int st) { return done(&sh.q_full[st], (t / K_STAGES) & 1); };
+      bool ok = done(&sh.kv_full, 0);
+      int st = 0;
+      if (warp == WARP_SCORE) {
+        const uint64_t dk = desc_k(sk), dqg = desc_k(sqg);
+        for (int t = 0; ok && t < nt; t++) {
+          // the warps have the scores of tile t - 1 in registers
+          if (!(ok = landed(t, st) && (t < 1 || done(&sh.s_free, (t - 1) & 1)))) break;
+          tc_fence_after();
+          const uint64_t q = dqg + st * (K_STAGE / 16);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+          for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int ks = 0; ks < 4; ks++)
-            if (ks < ksteps)
-              mma_ss(tmem + 256 + h * 64, dk + (h * BIG + ks * 32) / 16, q + (h * SMALL + ks * 32) / 16, id_s, ks > 0,
+            for (int ks = 0; ks < 4; ks++)
+              if (ks < ksteps)
+                mma_ss(tmem + 256 + h * 64, dk + (h * BIG + ks * 32) / 16, q + (h * SMALL + ks * 32) / 16, id_s, ks > 0,
+                       lead);
+          commit(&sh.s_full, lead);
+          if (++st == K_STAGES) st = 0;
+        }
+      } else {
+        const uint32_t id_k = idesc_bf16(ROWS, 64, true), id_v = idesc_bf16(ROWS, 2 * a.dh, true);
+        const uint64_t dv = desc_k(sv), dqg = desc_k(sqg), dp = desc_k(sp);
+        const uint64_t mq = desc_mn(sqg, 0), mg = desc_mn(sqg + 2 * SMALL, SMALL);
+        auto slopes = [&](int t, int s1) {
+          const uint64_t q = dqg + s1 * (K_STAGE / 16);
+#pragma unroll
+          for (int ks = 0; ks < 8; ks++)
+            if (ks < dsteps)
+              mma_ss(tmem + 384 + (t & 1) * 64, dv + ((ks >> 2) * BIG + (ks & 3) * 32) / 16,
+                     q + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
+          commit(&sh.d_full[t & 1], lead);
+        };
+        for (int t = 0; ok && t < min(nt, 2); t++)
+          if ((ok = landed(t, t))) {
+            tc_fence_after();
+            slopes(t, t);
+          }
+        int st2 = 2;
+        for (int t = 0; ok && t < nt; t++) {
+          if (!(ok = done(&sh.p_full[t & 1], (t >> 1) & 1))) break;
+          tc_fence_after();
+          const uint64_t q = mq + st * (K_STAGE / 16), g = mg + st * (K_STAGE / 16);
+          const uint64_t pt = dp + (t & 1) * (BIG / 16);
+          const uint32_t ds = tmem + 384 + (t & 1) * 64;
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++)
+              mma_ts(tmem + 128 + m * 64, ds + ks * 16 + m * 8, q + (m * SMALL + ks * 2048) / 16, id_k, t > 0 || ks > 0,
                      lead);
 #pragma unroll
-        for (int ks = 0; ks < 8; ks++)
-          if (ks < dsteps)
-            mma_ss(tmem + 384, dv + ((ks >> 2) * BIG + (ks & 3) * 32) / 16,
-                   q + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
-        commit(&sh.s_full, lead);
-      };
-      bool ok = done(&sh.kv_full, 0) && done(&sh.q_full[0], 0);
-      if (ok) scores(0);
-      int st = 0, st1 = 1;  // stages of tiles t and t + 1
-      for (int t = 0; ok && t < nt; t++) {
-        if (t + 1 < nt) {
-          if (!(ok = done(&sh.q_full[st1], ((t + 1) / K_STAGES) & 1) && done(&sh.s_free, t & 1))) break;
-          scores(st1);
+          for (int ks = 0; ks < 4; ks++) mma_ss(tmem, pt + ks * 2, g + ks * (2048 / 16), id_v, t > 0 || ks > 0, lead);
+          commit(&sh.pv[t & 1], lead);
+          // the scores of tile t are long done: dS came of them
+          commit(&sh.q_empty[st], lead);
+          if (t + 1 == nt) commit(&sh.o_full, lead);
+          if (t + 2 < nt) {
+            // in the place of the dS that the products above have read (they are
+            // of the same accumulator shape, and so executed before)
+            if (!(ok = landed(t + 2, st2))) break;
+            tc_fence_after();
+            slopes(t + 2, st2);
+          }
+          if (++st == K_STAGES) st = 0;
+          if (++st2 == K_STAGES) st2 = 0;
         }
-        if (!(ok = done(&sh.p_full, t & 1))) break;
-        tc_fence_after();
-        const uint64_t q = mq + st * (K_STAGE / 16), g = mg + st * (K_STAGE / 16);
-#pragma unroll
-        for (int m = 0; m < 2; m++)
-#pragma unroll
-          for (int ks = 0; ks < 4; ks++)
-            mma_ts(tmem + 128 + m * 64, tmem + 448 + m * 32 + ks * 8, q + (m * SMALL + ks * 2048) / 16, id_k,
-                   t > 0 || ks > 0, lead);
-#pragma unroll
-        for (int ks = 0; ks < 4; ks++) mma_ss(tmem, dp + ks * 2, g + ks * (2048 / 16), id_v, t > 0 || ks > 0, lead);
-        commit(&sh.pv, lead);
-        commit(&sh.q_empty[st], lead);
-        if (t + 1 == nt) commit(&sh.o_full, lead);
-        if (++st == K_STAGES) st = 0;
-        if (++st1 == K_STAGES) st1 = 0;
       }
       if (!ok) {  // no MMA may write tensor memory after it is released
-        commit(&sh.drain, lead);
-        settle(&sh.drain, 0);
+        uint64_t* drain = &sh.drain[warp == WARP_SCORE];
+        commit(drain, lead);
+        settle(drain, 0);
       }
       __syncwarp();
     }
