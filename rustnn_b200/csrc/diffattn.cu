@@ -555,35 +555,47 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
       cp_wait<0>();
     }
     __syncthreads();
-    for (int r = warp * 16; r < warp * 16 + 16; r++) {
-      const int p = row0 + r;
-      if (p >= rows) break;
-      const int e = p / a.tq, i = p - e * a.tq;
-      const int head = kvh * a.grp + e;
-      const T* o = static_cast<const T*>(a.fo) + b * a.ob + head * a.oh + i * a.orow;
-      const T* o2 = static_cast<const T*>(a.fo2) + ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh);
-      const float lm = __ldg(a.lam + head);
-      float d1 = 0.0f, d2 = 0.0f;
-      for (int c = lane; c < 2 * a.dh; c += 32) {
-        const float g = to_f<T>(sdo[r * PITCH + c]), y = to_f<T>(o2[c]);
-        d2 += g * y;
-        d1 += g * (to_f<T>(o[c]) + lm * y);
+    // eight rows at a time, so that their loads are in flight together
+#pragma unroll 1
+    for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += 8) {
+      float e1[8], e2[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int p = min(row0 + r0 + k, rows - 1);
+        const int e = p / a.tq, i = p - e * a.tq;
+        const int head = kvh * a.grp + e;
+        const T* o = static_cast<const T*>(a.fo) + b * a.ob + head * a.oh + i * a.orow;
+        const T* o2 = static_cast<const T*>(a.fo2) + ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh);
+        const float lm = __ldg(a.lam + head);
+        e1[k] = e2[k] = 0.0f;
+#pragma unroll
+        for (int c0 = 0; c0 < W; c0 += 32) {
+          const int c = c0 + lane;
+          const bool on = c < 2 * a.dh;
+          const float g = on ? to_f<T>(sdo[(r0 + k) * PITCH + c]) : 0.0f, y = on ? to_f<T>(o2[c]) : 0.0f;
+          const float x = on ? to_f<T>(o[c]) : 0.0f;
+          e2[k] += g * y;
+          e1[k] += g * (x + lm * y);
+        }
       }
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) {
-        d1 += __shfl_xor_sync(0xffffffffu, d1, x);
-        d2 += __shfl_xor_sync(0xffffffffu, d2, x);
-      }
-      if (lane == 0) {
-        sd[2 * r] = d1;
-        sd[2 * r + 1] = d2;
+      for (int k = 0; k < 8; k++) {
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+          e1[k] += __shfl_xor_sync(0xffffffffu, e1[k], x);
+          e2[k] += __shfl_xor_sync(0xffffffffu, e2[k], x);
+        }
+        if (lane == 0) {
+          sd[2 * (r0 + k)] = e1[k];
+          sd[2 * (r0 + k) + 1] = e2[k];
+        }
       }
     }
     __syncwarp();
   }
 
   int lim[2];
-  float ls1[2], ls2[2], d1[2], d2[2], dl[2] = {0.0f, 0.0f};
+  float ls1[2], ls2[2], d1[2], d2[2], dl[2] = {0.0f, 0.0f}, pl[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const int r = warp * 16 + (lane >> 2) + 8 * i, p = row0 + r;
@@ -679,6 +691,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
             d2[e >> 1] += y * dp[nb][e];
           } else {
             dl[e >> 1] += y * dp[nb][e];
+            pl[e >> 1] += y;
           }
         }
       if (sums) continue;
@@ -726,7 +739,9 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
 
 #pragma unroll
   for (int h = 0; h < 2; h++) {
-    const float sum = quad_sum(dl[h]);
+    // over the map's own sum: what the log-sum's rounding does to a whole row cancels
+    const float whole = quad_sum(pl[h]), part = quad_sum(dl[h]);
+    const float sum = whole > 0.0f ? part / whole : 0.0f;
     const int p = row0 + warp * 16 + (lane >> 2) + 8 * h;
     if (p >= rows) continue;
     const int e = p / a.tq, i = p - e * a.tq;
@@ -1203,9 +1218,13 @@ extern "C" int rnn_diffattn_bwd_dev(rnn_ctx* ctx, const rnn_diffattn* d, const r
           diff::multiples({a.qb, a.qr, a.qh, a.kb, a.kr, a.kh, a.vb, a.vr, a.vh, a.gb, a.gr, a.gh}, 16 / esz);
   a.pair = a.dh % 2 == 0 && diff::aligned({dq, dk, dv}, 2 * esz) &&
            diff::multiples({a.dqb, a.dqr, a.dqh, a.dkb, a.dkr, a.dkh, a.dvb, a.dvr, a.dvh}, 2);
-  RNN_TRY(ensure_ws(ctx, nrow * 3 * sizeof(float)));
+  const bool tensor = d->dtype == RNN_BF16 && diff::tc_bwd_ok(a);
+  a.kparts = tensor ? diff::tc_bwd_parts(ctx, a) : 1;
+  const size_t sums = (nrow * 3 + 3) / 4 * 4, keep = a.kparts > 1 ? (size_t)a.kparts * a.n * a.hkv * a.tk * 256 : 0;
+  RNN_TRY(ensure_ws(ctx, (sums + keep) * sizeof(float)));
   a.dsum = static_cast<float*>(ctx->ws);
   a.dlrow = a.dsum + 2 * nrow;
-  if (d->dtype == RNN_F32) return diff::bwd_type<float>(ctx, a);
-  return diff::tc_bwd_ok(a) ? diff::tc_bwd(ctx, a) : diff::bwd_type<__nv_bfloat16>(ctx, a);
+  a.kpart = a.dsum + sums;
+  if (tensor) return diff::tc_bwd(ctx, a);
+  return d->dtype == RNN_F32 ? diff::bwd_type<float>(ctx, a) : diff::bwd_type<__nv_bfloat16>(ctx, a);
 }

@@ -42,6 +42,8 @@ struct Args {
   float* dlam;
   float* dsum;   // [n, h, 2, tq]: D_1, D_2
   float* dlrow;  // [h, n * tq]: sum_j P_2 dP of each row, in f32
+  int kparts;    // parts that the queries of a key tile are split into
+  float* kpart;  // [part][n * hkv][tk][256]: dv, dk_1, dk_2 of a part, 64 columns each piece
 };
 
 __device__ __forceinline__ int key_len(const Args& a, int b) {

@@ -235,6 +235,7 @@ bool tc_fwd_ok(const Args& a);
 int tc_fwd(rnn_ctx* ctx, const Args& a);
 bool tc_bwd_ok(const Args& a);
 int tc_bwd(rnn_ctx* ctx, const Args& a);
+int tc_bwd_parts(rnn_ctx* ctx, const Args& a);  // parts (256 floats a key each) that its workspace holds
 // The same of the kernel for a few rows over a long cache, which leaves parts
 // of 128 columns for join_parts when it splits the keys.
 bool dec_ok(const Args& a);

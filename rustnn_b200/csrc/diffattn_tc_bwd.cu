@@ -12,6 +12,7 @@
 // alone left them idle at each of its waits.  Warp 19 clears what lies beyond a
 // sequence's length (queries' kernel) or sums dlam (keys' kernel).
 #include <algorithm>
+#include <cmath>
 
 #include "diffattn_tc.cuh"
 
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     soft_sync();
 
     const f32x2 e1 = pair(-d1, -d1), e2 = pair(-d2, -d2);
-    f32x2 dl = 0ull;
+    f32x2 dl = 0ull, pl = 0ull;
     for (int j = team; j < nt; j += 2) {
       const uint32_t par = (j >> 1) & 1;
       const bool edge = j * COLS + 32 > full;
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
             const int k = h * 4 + e;
             const f32x2 g = pair(dp[2 * e], dp[2 * e + 1]), y2 = pair(y[c][2 * k], y[c][2 * k + 1]);
             dl = fma2(y2, g, dl);
+            pl = add2(pl, y2);
             float r0, r1;
             unpair(mul2(pair(x[c][2 * k], x[c][2 * k + 1]), add2(g, e1)), r0, r1);
             u[k] = pack2(r0, r1);
@@ -256,13 +258,18 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_full[team]);
     }
-    float l0, l1;
+    float l0, l1, p0, p1;
     unpair(dl, l0, l1);
-    sh.part[k4][row].x = l0 + l1;
+    unpair(pl, p0, p1);
+    sh.part[k4][row] = make_float2(l0 + l1, p0 + p1);
     soft_sync();
-    if (in && k4 == 0)
+    if (in && k4 == 0) {
+      // over the map's own sum: what the log-sum's rounding does to a whole row cancels
+      const float part = (sh.part[0][row].x + sh.part[1][row].x) + (sh.part[2][row].x + sh.part[3][row].x);
+      const float whole = (sh.part[0][row].y + sh.part[1][row].y) + (sh.part[2][row].y + sh.part[3][row].y);
       a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
-          (sh.part[0][row].x + sh.part[1][row].x) + (sh.part[2][row].x + sh.part[3][row].x);
+          whole > 0.0f ? part / whole : 0.0f;
+    }
 
     bool ok = true;
     if (nt > 0) {
@@ -447,7 +454,10 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
   } else if (a.causal == RNN_CAUSAL_END) {
     qbeg = min(a.tq, max(0, key0 - (len - a.tq)));
   }
-  const int per = (a.tq - qbeg + COLS - 1) / COLS, nt = per * a.grp;
+  // tiles of all the group's queries, of which this block takes its part
+  const int per = (a.tq - qbeg + COLS - 1) / COLS, all = per * a.grp;
+  const int tbeg = static_cast<int>(static_cast<long long>(all) * blockIdx.y / a.kparts);
+  const int nt = static_cast<int>(static_cast<long long>(all) * (blockIdx.y + 1) / a.kparts) - tbeg;
   const int wide = 2 * a.dh > 64 ? 2 : 1, ksteps = (a.dh + 15) / 16, dsteps = a.dh / 8;
 
   if (tid == 0) {
@@ -487,7 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
     uint8_t* pc = base + 4 * BIG + K_STAGES * K_STAGE + row * 128;
     const int ch0 = ((2 * k4) ^ (row & 7)) << 4, ch1 = ((2 * k4 + 1) ^ (row & 7)) << 4;
 
-    int st = 0, e = 0, q0 = qbeg;
+    int st = 0, e = nt > 0 ? tbeg / per : 0, q0 = nt > 0 ? qbeg + tbeg % per * COLS : 0;
     for (int t = 0; t < nt; t++) {
       const float lam = __ldg(a.lam + kvh * a.grp + e);
       float x[16], y[16], dp[16];
@@ -585,6 +595,9 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
       const bool some = nt > 0 && key < len;
       __nv_bfloat16* odk = static_cast<__nv_bfloat16*>(a.dk) + b * a.dkb + kvh * a.dkh + key * a.dkr;
       __nv_bfloat16* odv = static_cast<__nv_bfloat16*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr;
+      float* part = a.kparts > 1
+                        ? a.kpart + ((static_cast<long long>(blockIdx.y) * nbh + bh) * a.tk + key) * 256 + k4 * 16
+                        : nullptr;
 #pragma unroll
       for (int m = 0; m < 4; m++) {
         float x[16] = {};
@@ -592,7 +605,12 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
           tmem_ld(tmem + lanes + m * 64 + k4 * 16, x);
           tmem_landed(x);
         }
-        if (key < a.tk) {
+        if (key < a.tk && part) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4)
+            *reinterpret_cast<float4*>(part + m * 64 + c) =
+                some ? make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        } else if (key < a.tk) {
           if (m < 2) {
             store16(odv + m * 64 + k4 * 16, x, 1.0f, some, 2 * a.dh - m * 64 - k4 * 16, p.st16);
           } else {
@@ -617,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
           const int st = t % K_STAGES;
           if (t >= K_STAGES && !warp_wait(&sh.q_empty[st], (t / K_STAGES - 1) & 1, abort_flag, dev_error)) break;
           const uint32_t dst = sqg + st * K_STAGE;
-          const int head = kvh * a.grp + t / per, i0 = qbeg + (t % per) * COLS;
+          const int head = kvh * a.grp + (tbeg + t) / per, i0 = qbeg + (tbeg + t) % per * COLS;
           if (lead) {
             mbar_arrive_expect_tx(&sh.q_full[st], (2 + wide) * SMALL);
             for (int h = 0; h < 2; h++) tma_5d(dst + h * SMALL, &p.q, 0, h, head, i0, b, &sh.q_full[st]);
@@ -644,7 +662,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
       __syncwarp();
     } else if (warp == WARP_AUX) {
       // dlam: block `head` sums that head's rows in a fixed order
-      if (static_cast<int>(blockIdx.x) < a.h && a.tq > 0) {
+      if (static_cast<int>(blockIdx.x) < a.h && blockIdx.y == 0 && a.tq > 0) {
         const long long cnt = static_cast<long long>(a.n) * a.tq;
         const float* x = a.dlrow + blockIdx.x * cnt;
         double s[4] = {0.0, 0.0, 0.0, 0.0};
@@ -745,6 +763,40 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
   if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
 }
 
+// Joins the parts of dk and dv in their order: 64 threads a key, four of its 256
+// columns each.
+__global__ void __launch_bounds__(256) join_keys_kernel(Args a) {
+  const long long total = static_cast<long long>(a.n) * a.hkv * a.tk;
+  const long long idx = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (idx >= total) return;
+  const int c = (threadIdx.x & 63) * 4;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int k = 0; k < a.kparts; k++) {
+    const float4 x = *reinterpret_cast<const float4*>(a.kpart + (k * total + idx) * 256 + c);
+    s.x += x.x;
+    s.y += x.y;
+    s.z += x.z;
+    s.w += x.w;
+  }
+  const int key = static_cast<int>(idx % a.tk), bh = static_cast<int>(idx / a.tk);
+  const int b = bh / a.hkv, kvh = bh - b * a.hkv;
+  __nv_bfloat16* o;
+  if (c < 128) {
+    if (c >= 2 * a.dh) return;
+    o = static_cast<__nv_bfloat16*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr + c;
+  } else {
+    const int m = c >= 192 ? 1 : 0, w = c - 128 - m * 64;
+    if (w >= a.dh) return;
+    o = static_cast<__nv_bfloat16*>(a.dk) + b * a.dkb + kvh * a.dkh + key * a.dkr + m * a.dh + w;
+    s = make_float4(s.x * a.scale, s.y * a.scale, s.z * a.scale, s.w * a.scale);
+  }
+  o[0] = __float2bfloat16_rn(s.x);
+  o[1] = __float2bfloat16_rn(s.y);
+  o[2] = __float2bfloat16_rn(s.z);
+  o[3] = __float2bfloat16_rn(s.w);
+}
+
 bool mult8(std::initializer_list<long long> s) {
   for (long long x : s)
     if (x % 8) return false;
@@ -787,9 +839,37 @@ int tc_bwd(rnn_ctx* ctx, const Args& a) {
   RNN_TRY(encode_map(&p.g, a.dout, a.n, a.tq, a.h, 1, 2 * a.dh, a.gb, a.gr, a.gh, COLS));
   RNN_TRY(encode_map(&p.k, a.k, a.n, a.tk, a.hkv, 2, a.dh, a.kb, a.kr, a.kh, ROWS));
   RNN_TRY(encode_map(&p.v, a.v, a.n, a.tk, a.hkv, 1, 2 * a.dh, a.vb, a.vr, a.vh, ROWS));
-  tc_bwd_kv_kernel<<<static_cast<unsigned>(kblocks), THREADS, K_SMEM, ctx->stream>>>(p);
+  tc_bwd_kv_kernel<<<dim3(static_cast<unsigned>(kblocks), a.kparts), THREADS, K_SMEM, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
+  if (a.kparts > 1) {
+    const long long keys = static_cast<long long>(a.n) * a.hkv * a.tk;
+    join_keys_kernel<<<static_cast<unsigned>((keys + 3) / 4), 256, 0, ctx->stream>>>(p.a);
+    RNN_CHECK_LAUNCH();
+  }
   return RNN_OK;
+}
+
+// When the keys alone leave SMs idle (few sequences and key heads), the queries
+// of a key tile are split over blocks.  Time is counted in tiles (about 1.1 us):
+// the waves of blocks, each with its share and a start and end worth six tiles,
+// and the parts' way through memory.  Measured: 5 x 1003 tokens, 2 key heads of
+// 3 queries' heads each (80 key tiles), 75 us whole and 50 in three parts with
+// their join; 2 x 1024, 8 heads (128 key tiles), 63 us whole and 85 in two parts.
+int tc_bwd_parts(rnn_ctx* ctx, const Args& a) {
+  const double blocks = static_cast<double>((a.tk + ROWS - 1) / ROWS) * a.n * a.hkv;
+  const double tiles = static_cast<double>((a.tq + COLS - 1) / COLS) * a.grp;
+  const double pass = 2048.0 * a.n * a.hkv * a.tk / 6.5e12 / 1.1e-6;  // a part written and read
+  int best = 1;
+  double least = 0.0;
+  for (int parts = 1; parts <= 16 && (parts == 1 || tiles >= 4.0 * parts); parts++) {
+    const double waves = std::ceil(blocks * parts / ctx->num_sms);
+    const double time = waves * (tiles / parts + 6.0) + (parts > 1 ? 4.0 + parts * pass : 0.0);
+    if (parts == 1 || time < least) {
+      least = time;
+      best = parts;
+    }
+  }
+  return best;
 }
 
 }  // namespace diff
