@@ -204,10 +204,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
   const int b = bh / a.h, head = bh - b * a.h, kvh = head / a.grp;
   const int i0 = tile * QROWS;
   const int len = key_len(a, b);
-  const int kend = row_limit(a, min(i0 + QROWS, a.tq) - 1, len);
-  const int nt = (kend + KEYS - 1) / KEYS;
+  // this block's part of the keys: all of them, or split_keys (a multiple of KEYS)
+  const int kbeg = static_cast<int>(blockIdx.y) * a.split_keys;
+  const int kend = min(row_limit(a, min(i0 + QROWS, a.tq) - 1, len), kbeg + a.split_keys);
+  const int nt = max(kend - kbeg + KEYS - 1, 0) / KEYS;
   // the last tile may hold rows of a cache beyond the sequence
-  const bool dirty = nt > 0 && nt * KEYS > len && len < a.tk;
+  const bool dirty = nt > 0 && kbeg + nt * KEYS > len && len < a.tk;
   const int wide = 2 * a.dh > 64 ? 2 : 1;  // 64-column parts of v
   const int ksteps = (a.dh + 15) / 16;
 
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
     float m1 = -CUDART_INF_F, m2 = -CUDART_INF_F, l1 = 0.0f, l2 = 0.0f, r = lam;
 
     for (int j = team; j < nt; j += 2) {
-      const int j0 = j * KEYS;
+      const int j0 = kbeg + j * KEYS;
       const bool edge = j0 + KEYS > full;
       const uint32_t par = (j >> 1) & 1;
       float s1[2][32], s2[2][32];
@@ -377,6 +379,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
     __nv_bfloat16* o2 =
         a.o2 ? static_cast<__nv_bfloat16*>(a.o2) + ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh)
              : nullptr;
+    const bool whole = a.nsplit == 1;
+    // a part's sums of the maps' products with v, for join_kernel: A + r B and B
+    const long long idx = (static_cast<long long>(b) * a.hkv + kvh) * (static_cast<long long>(a.grp) * a.tq) +
+                          static_cast<long long>(head - kvh * a.grp) * a.tq + i;
+    const long long at = blockIdx.y * (static_cast<long long>(nbh) * a.tq) + idx;
+    if (!whole && team == 0 && i < a.tq)
+      *reinterpret_cast<float4*>(a.stat + at * 4) = make_float4(last.x, L1, last.y, L2);
     // 16 columns at a time, the two threads of a row in turn
     for (int c = team * 16; ok && c < 2 * a.dh; c += 32) {
       float x[16] = {}, y[16] = {};
@@ -385,6 +394,19 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
         tmem_ld(tmem + lanes + COL_B + c, y);
         tmem_landed(x);
         tmem_landed(y);
+      }
+      if (!whole) {
+        if (i < a.tq) {
+          float4* px = reinterpret_cast<float4*>(a.part + at * 256 + c);
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            px[k] = make_float4(x[4 * k] + last.z * y[4 * k], x[4 * k + 1] + last.z * y[4 * k + 1],
+                                x[4 * k + 2] + last.z * y[4 * k + 2], x[4 * k + 3] + last.z * y[4 * k + 3]);
+            px[32 + k] = make_float4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+          }
+        }
+        __syncwarp();
+        continue;
       }
       uint32_t po[8], p2[8];
 #pragma unroll
@@ -413,7 +435,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
       }
       __syncwarp();
     }
-    if (a.lse && team == 0 && i < a.tq) {
+    if (whole && a.lse && team == 0 && i < a.tq) {
       float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
       s[0] = any ? last.x + log2f(L1) : CUDART_INF_F;
       s[a.tq] = any ? last.y + log2f(L2) : CUDART_INF_F;
@@ -434,9 +456,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
           uint64_t* bar = dirty && j == nt - 1 ? &sh.last_full : &sh.kv_full[st];
           mbar_arrive_expect_tx(bar, (2 + wide) * HALF_BYTES);
           for (int half = 0; half < 2; half++)
-            tma_5d(dst + half * HALF_BYTES, &p.k, 0, half, kvh, j * KEYS, b, bar);
+            tma_5d(dst + half * HALF_BYTES, &p.k, 0, half, kvh, kbeg + j * KEYS, b, bar);
           for (int c = 0; c < wide; c++)
-            tma_5d(dst + (2 + c) * HALF_BYTES, &p.v, c * 64, 0, kvh, j * KEYS, b, bar);
+            tma_5d(dst + (2 + c) * HALF_BYTES, &p.v, c * 64, 0, kvh, kbeg + j * KEYS, b, bar);
         }
         // what was asked for lands before the block may end, aborting or not
         settle(&sh.q_full, 0);
@@ -451,7 +473,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
         if (warp_wait(&sh.last_full, 0, abort_flag, dev_error)) {
           // hidden values may be NaN: P = 0 there, so v has to be finite
           uint8_t* v = base + Q_BYTES + st * STAGE_BYTES + 2 * HALF_BYTES;
-          for (int r = len - j * KEYS; r < KEYS; r++)
+          for (int r = len - kbeg - j * KEYS; r < KEYS; r++)
             for (int c = lane; c < wide * 8; c += 32)
               *reinterpret_cast<uint4*>(v + (c >> 3) * HALF_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           fence_async_smem();
@@ -533,14 +555,93 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
   if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
 }
 
+// Joins the parts that the keys were split into, a warp for each row: the maps'
+// sums meet at the larger maximum.  (The rows here are many and the parts few;
+// for a token over a long cache, where it is the other way round, the parts are
+// shared out over a block.)
+constexpr int JOIN_WARPS = 8;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_rows_kernel(const __grid_constant__ Args a) {
+  const long long total = static_cast<long long>(a.n) * a.h * a.tq;
+  const long long idx = static_cast<long long>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (idx >= total) return;
+  float M1 = -CUDART_INF_F, M2 = -CUDART_INF_F;
+  for (int s = 0; s < a.nsplit; s++) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(a.stat) + s * total + idx);
+    M1 = fmaxf(M1, v.x);
+    M2 = fmaxf(M2, v.z);
+  }
+  const float U1 = M1 == -CUDART_INF_F ? 0.0f : M1, U2 = M2 == -CUDART_INF_F ? 0.0f : M2;
+  float L1 = 0.0f, L2 = 0.0f;
+  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+  const bool mine = lane * 4 < 2 * a.dh;
+#pragma unroll 4
+  for (int s = 0; s < a.nsplit; s++) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(a.stat) + s * total + idx);
+    const float4* part = reinterpret_cast<const float4*>(a.part + (s * total + idx) * 256) + lane;
+    const float w1 = ex2(v.x - U1), w2 = ex2(v.z - U2);
+    L1 += w1 * v.y;
+    L2 += w2 * v.w;
+    if (mine) {
+      const float4 p = part[0], q = part[32];
+      x.x += w1 * p.x, x.y += w1 * p.y, x.z += w1 * p.z, x.w += w1 * p.w;
+      y.x += w2 * q.x, y.y += w2 * q.y, y.z += w2 * q.z, y.w += w2 * q.w;
+    }
+  }
+  const int rows = a.grp * a.tq;
+  const int bh = static_cast<int>(idx / rows), r = static_cast<int>(idx - static_cast<long long>(bh) * rows);
+  const int b = bh / a.hkv, e = r / a.tq, i = r - e * a.tq, head = (bh - b * a.hkv) * a.grp + e;
+  const bool any = L1 > 0.0f && L2 > 0.0f;
+  const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f, f = any ? __ldg(a.lam + head) * i2 : 0.0f;
+  if (mine) {
+    const uint32_t lo = pack2(x.x * i1 - f * y.x, x.y * i1 - f * y.y), hi = pack2(x.z * i1 - f * y.z, x.w * i1 - f * y.w);
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + b * a.ob + head * a.oh + i * a.orow + lane * 4;
+    if (a.pair) {
+      reinterpret_cast<uint32_t*>(o)[0] = lo;
+      reinterpret_cast<uint32_t*>(o)[1] = hi;
+    } else {
+      const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&lo);
+      const __nv_bfloat162 w = *reinterpret_cast<const __nv_bfloat162*>(&hi);
+      o[0] = z.x, o[1] = z.y, o[2] = w.x, o[3] = w.y;
+    }
+    if (a.o2)
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.o2) +
+                                ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + lane * 4) =
+          make_uint2(pack2(y.x * i2, y.y * i2), pack2(y.z * i2, y.w * i2));
+  }
+  if (a.lse && lane < 2) {
+    float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
+    if (lane == 0) s[0] = any ? M1 + log2f(L1) : CUDART_INF_F;
+    else s[a.tq] = any ? M2 + log2f(L2) : CUDART_INF_F;
+  }
+}
+
 }  // namespace
 
+// A block costs about 5 us beside its tiles and holds one head's rows, while the
+// kernels of mma.sync pack the rows of all heads that share keys and run several
+// blocks an SM.  So they keep what is short on both sides (256 x 32 x 32, 4 heads
+// of 32: 20 us against 41 here; 128 x 64 x 64: 19 against 22) and rows too few to
+// fill a tile (64 x 3 x 1024, 32 heads on 4: 96 against 346; 64 x 9 x 512, 8 on
+// 2: 50 against 62).  The rest is faster here: 64 x 24 x 256, 8 of 32: 39 against
+// 51; 128 x 33 x 1000, 8 of 64: 181 against 508; 32 x 1000 x 16: 102 against 131
+// (the others timed with a mask of keys that hides none).
 bool tc_fwd_ok(const Args& a) {
   if (a.dh % 8 || a.dh < 16 || a.dh > 64 || a.kmask || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
-  if (a.tq < 64 || a.tk < 64) return false;
+  if (a.tq < 16 || std::max(a.tq, a.tk) < 64) return false;
   if (reinterpret_cast<uintptr_t>(a.o2) % 16) return false;
   return map_ok(a.q, a.n, a.tq, a.h, a.dh, a.qb, a.qr, a.qh) && map_ok(a.k, a.n, a.tk, a.hkv, a.dh, a.kb, a.kr, a.kh) &&
          map_ok(a.v, a.n, a.tk, a.hkv, 2 * a.dh, a.vb, a.vr, a.vh);
+}
+
+// When the rows leave SMs idle the keys are split over blocks.  A part's start
+// and end and the join cost about seven tiles' time (1.06 us each).  Measured
+// whole and split: 1 x 128 x 8192, 16 heads: 133 and 34 us; 1 x 64 x 16384, 4
+// heads: 293 and 31; 4 x 128 x 1024, 8 heads: 24 and 21; but 2 x 256 x 512, 8
+// heads: 14 and 16 in four parts.
+static long long key_parts(const rnn_ctx* ctx, long long blocks, int tiles) {
+  const long long parts = std::min<long long>(ctx->num_sms / blocks, tiles / 4);
+  return parts > 1 && tiles - tiles / parts > 7 ? parts : 1;
 }
 
 int tc_fwd(rnn_ctx* ctx, const Args& a) {
@@ -556,8 +657,24 @@ int tc_fwd(rnn_ctx* ctx, const Args& a) {
   RNN_REQUIRE(blocks < (1ll << 31), "diffattn: too many rows");
   static std::atomic<unsigned long long> optin{0};
   RNN_TRY(tc::ensure_smem_optin(tc_fwd_kernel, optin, ctx->device, static_cast<int>(FWD_SMEM)));
-  tc_fwd_kernel<<<static_cast<unsigned>(blocks), FWD_THREADS, FWD_SMEM, ctx->stream>>>(p);
+  const int tiles = (a.tk + KEYS - 1) / KEYS;
+  const long long parts = key_parts(ctx, blocks, tiles);
+  p.a.split_keys = static_cast<int>((tiles + parts - 1) / parts) * KEYS;
+  p.a.nsplit = (a.tk + p.a.split_keys - 1) / p.a.split_keys;
+  if (p.a.nsplit > 1) {
+    const size_t rows = static_cast<size_t>(a.n) * a.h * a.tq;
+    RNN_TRY(ensure_ws(ctx, rows * p.a.nsplit * (256 + 4) * sizeof(float)));
+    p.a.part = static_cast<float*>(ctx->ws);
+    p.a.stat = p.a.part + rows * p.a.nsplit * 256;
+  }
+  tc_fwd_kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), FWD_THREADS, FWD_SMEM, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
+  if (p.a.nsplit > 1) {
+    const long long rows = static_cast<long long>(a.n) * a.h * a.tq;
+    join_rows_kernel<<<static_cast<unsigned>((rows + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, ctx->stream>>>(
+        p.a);
+    RNN_CHECK_LAUNCH();
+  }
   return RNN_OK;
 }
 

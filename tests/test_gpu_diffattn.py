@@ -206,6 +206,39 @@ def test_few_rows_over_a_long_cache(ops, n, tq, tk, h, hkv, dh, dtype):
     check_all(ops, q, k, v, lam, dout, causal="end", klen=klen)
 
 
+@pytest.mark.parametrize("causal", [None, "start", "end"])
+@pytest.mark.parametrize("n,tq,tk,h,hkv,dh", [(1, 70, 3000, 2, 1, 40), (3, 20, 1500, 2, 2, 64), (2, 200, 5001, 4, 2, 16),
+                                              (1, 129, 1025, 3, 1, 32)])
+def test_new_rows_over_a_long_cache(ops, n, tq, tk, h, hkv, dh, causal):
+    """A run of new tokens against a cache: rows fill tiles but not the device, so the keys are split over blocks.
+    What lies beyond the lengths is NaN; some parts, and the rows of one sequence, have no keys."""
+    q, k, v, lam, dout = make(n, tq, tk, h, hkv, dh, BF16, tk)
+    check_all(ops, q, k, v, lam, dout, causal=causal)
+    for first in (tk - 1, tk // 2 + 1, 130, 64, 1, 0):
+        klen = torch.tensor([first, tk, 65][:n], dtype=torch.int32, device="cuda")
+        hidden = torch.arange(tk, device="cuda")[None] >= klen[:, None]
+        k2, v2 = k.clone(), v.clone()
+        k2.masked_fill_(hidden[:, :, None, None], math.nan)
+        v2.masked_fill_(hidden[:, :, None, None], -math.inf)
+        o, lse = check_all(ops, q, k2, v2, lam, dout, causal=causal, klen=klen)
+        if first == 0:
+            assert bool((o[0] == 0).all()) and bool((lse[0] == math.inf).all())
+        # any alignment of the output's rows
+        at = torch.full((n, tq, h * 2 * dh + 3), 7.0, device="cuda", dtype=BF16)
+        out = at[..., 1:1 + h * 2 * dh].unflatten(-1, (h, 2 * dh))
+        assert torch.equal(ops.diffattn_forward(q, k2, v2, lam, causal=causal, klen=klen, out=out), o)
+        assert bool((at[..., 0] == 7).all()) and bool((at[..., -2:] == 7).all())
+
+
+def test_nearly_equal_maps_over_a_long_cache(ops):
+    """What is left of the difference keeps the type's precision when the keys are split too."""
+    q, k, v, _, dout = make(1, 130, 3000, 2, 2, 32, BF16, 9)
+    q[..., 32:], k[..., 32:] = q[..., :32], k[..., :32]
+    lam = torch.full((2,), 0.75, device="cuda")
+    want = reference(q, k, v, lam, dout, 32 ** -0.5)[0]
+    assert rel(ops.diffattn_forward(q, k, v, lam), want) < 2.0 ** -8
+
+
 def test_large_scores(ops):
     """Scores far apart, and maps whose sums differ by many orders: no overflow, no loss to the running ratio."""
     q, k, v, lam, dout = make(2, 70, 300, 2, 2, 32, F32, 8)
