@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
   using G = Geo<T, DH>;
   using FR = Frag<T>;
   constexpr int W = G::W, PITCH = G::PITCH, KS = G::KS, SUB = F::SUBK, BN = F::BN;
-  constexpr int NS = SUB / 8, NB = W / 8;
+  constexpr int NS = SUB / 8, NB = W / 8, NSIDE = NS < G::SIDE ? NS : G::SIDE;
   extern __shared__ __align__(16) unsigned char smem[];
   T* sq = reinterpret_cast<T*>(smem);
   T* sk = sq + F::Q_ELEMS;
@@ -163,12 +163,11 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
         const typename FR::A q1 = FR::ldA(sq, PITCH, rw * 16, ks * KS, lane);
         const typename FR::A q2 = FR::ldA(sq, PITCH, rw * 16, DH + ks * KS, lane);
 #pragma unroll
-        for (int nb = 0; nb < NS; nb += 2) {
-          typename FR::B f[2];
-          FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma2(s1[nb], s1[nb + 1], q1, f);
-          FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma2(s2[nb], s2[nb + 1], q2, f);
+        for (int nb = 0; nb < NS; nb += NSIDE) {
+          typename FR::B f[NSIDE], g[NSIDE];
+          FR::ldB_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
+          FR::ldB_nk(g, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
+          FR::mma(s1 + nb, q1, f, s2 + nb, q2, g);
         }
       }
       const bool edge = mask != nullptr || j0 + SUB > full;
@@ -230,16 +229,16 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
       // the step's products start at zero and join the accumulators in one
       // f32 addition, so long sums are not left to the MMA's own rounding
 #pragma unroll
-      for (int nb = 0; nb < NB; nb += 2) {
-        float x[2][4] = {}, y[2][4] = {};
+      for (int nb = 0; nb < NB; nb += G::SIDE) {
+        float x[G::SIDE][4] = {}, y[G::SIDE][4] = {};
 #pragma unroll
         for (int ks = 0; ks < SUB / KS; ks++) {
-          typename FR::B f[2];
-          FR::ldB2_kn(f, v, PITCH, s0 + ks * KS, nb * 8, lane);
-          FR::mma4(x, y, pa[ks], pb[ks], f);
+          typename FR::B f[G::SIDE];
+          FR::ldB_kn(f, v, PITCH, s0 + ks * KS, nb * 8, lane);
+          FR::mma(x, pa[ks], f, y, pb[ks], f);
         }
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < G::SIDE; i++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int h = e >> 1;
@@ -480,7 +479,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
   using G = Geo<T, DH>;
   using FR = Frag<T>;
   constexpr int W = G::W, PITCH = G::PITCH, KS = G::KS, SUB = G::SUB, BN = F::BN;
-  constexpr int NS = SUB / 8, NB = W / 8;
+  constexpr int NS = SUB / 8, NB = W / 8, NSIDE = NS < G::SIDE ? NS : G::SIDE;
   extern __shared__ __align__(16) unsigned char smem[];
   T* sq = reinterpret_cast<T*>(smem);
   T* sdo = sq + F::Q_ELEMS;
@@ -656,22 +655,21 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
         const typename FR::A q1 = FR::ldA(sq, PITCH, warp * 16, ks * KS, lane);
         const typename FR::A q2 = FR::ldA(sq, PITCH, warp * 16, DH + ks * KS, lane);
 #pragma unroll
-        for (int nb = 0; nb < NS; nb += 2) {
-          typename FR::B f[2];
-          FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma2(s1[nb], s1[nb + 1], q1, f);
-          FR::ldB2_nk(f, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma2(s2[nb], s2[nb + 1], q2, f);
+        for (int nb = 0; nb < NS; nb += NSIDE) {
+          typename FR::B f[NSIDE], g[NSIDE];
+          FR::ldB_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
+          FR::ldB_nk(g, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
+          FR::mma(s1 + nb, q1, f, s2 + nb, q2, g);
         }
       }
 #pragma unroll
       for (int ks = 0; ks < W / KS; ks++) {
         const typename FR::A g = FR::ldA(sdo, PITCH, warp * 16, ks * KS, lane);
 #pragma unroll
-        for (int nb = 0; nb < NS; nb += 2) {
-          typename FR::B f[2];
-          FR::ldB2_nk(f, v, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma2(dp[nb], dp[nb + 1], g, f);
+        for (int nb = 0; nb < NS; nb += NSIDE) {
+          typename FR::B f[NSIDE];
+          FR::ldB_nk(f, v, PITCH, s0 + nb * 8, ks * KS, lane);
+          FR::mma(dp + nb, g, f);
         }
       }
       const bool edge = mask != nullptr || j0 + SUB > full;
@@ -718,16 +716,16 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
 #pragma unroll
         for (int ks = 0; ks < SUB / KS; ks++) ds[ks] = m ? FR::from_acc(s2, ks) : FR::from_acc(s1, ks);
 #pragma unroll
-        for (int nb = m * NB / 2; nb < (m + 1) * NB / 2; nb += 2) {
-          float x[2][4] = {};
+        for (int nb = m * NB / 2; nb < (m + 1) * NB / 2; nb += G::HALF_SIDE) {
+          float x[G::HALF_SIDE][4] = {};
 #pragma unroll
           for (int ks = 0; ks < SUB / KS; ks++) {
-            typename FR::B f[2];
-            FR::ldB2_kn(f, k, PITCH, s0 + ks * KS, nb * 8, lane);
-            FR::mma2(x[0], x[1], ds[ks], f);
+            typename FR::B f[G::HALF_SIDE];
+            FR::ldB_kn(f, k, PITCH, s0 + ks * KS, nb * 8, lane);
+            FR::mma(x, ds[ks], f);
           }
 #pragma unroll
-          for (int i = 0; i < 2; i++)
+          for (int i = 0; i < G::HALF_SIDE; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) dq[nb + i][e] += x[i][e];
         }
@@ -783,7 +781,7 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
   using G = Geo<T, DH>;
   using FR = Frag<T>;
   constexpr int W = G::W, PITCH = G::PITCH, KS = G::KS, SUB = G::SUB, BM = F::BM;
-  constexpr int NS = SUB / 8, NB = W / 8;
+  constexpr int NS = SUB / 8, NB = W / 8, NSIDE = NS < G::SIDE ? NS : G::SIDE;
   extern __shared__ __align__(16) unsigned char smem[];
   T* sk = reinterpret_cast<T*>(smem);
   T* sv = sk + F::K_ELEMS;
@@ -903,22 +901,21 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
         const typename FR::A k1 = FR::ldA(sk, PITCH, warp * 16, ks * KS, lane);
         const typename FR::A k2 = FR::ldA(sk, PITCH, warp * 16, DH + ks * KS, lane);
 #pragma unroll
-        for (int nb = 0; nb < NS; nb += 2) {
-          typename FR::B f[2];
-          FR::ldB2_nk(f, q, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma2(s1[nb], s1[nb + 1], k1, f);
-          FR::ldB2_nk(f, q, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma2(s2[nb], s2[nb + 1], k2, f);
+        for (int nb = 0; nb < NS; nb += NSIDE) {
+          typename FR::B f[NSIDE], h[NSIDE];
+          FR::ldB_nk(f, q, PITCH, s0 + nb * 8, ks * KS, lane);
+          FR::ldB_nk(h, q, PITCH, s0 + nb * 8, DH + ks * KS, lane);
+          FR::mma(s1 + nb, k1, f, s2 + nb, k2, h);
         }
       }
 #pragma unroll
       for (int ks = 0; ks < W / KS; ks++) {
         const typename FR::A x = FR::ldA(sv, PITCH, warp * 16, ks * KS, lane);
 #pragma unroll
-        for (int nb = 0; nb < NS; nb += 2) {
-          typename FR::B f[2];
-          FR::ldB2_nk(f, g, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma2(dp[nb], dp[nb + 1], x, f);
+        for (int nb = 0; nb < NS; nb += NSIDE) {
+          typename FR::B f[NSIDE];
+          FR::ldB_nk(f, g, PITCH, s0 + nb * 8, ks * KS, lane);
+          FR::mma(dp + nb, x, f);
         }
       }
       // after this: s1 = dS_1, s2 = dS_2, dp = P_1 - lam P_2 (transposed)
@@ -942,16 +939,16 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
           f[ks] = m == 0 ? FR::from_acc(s1, ks) : m == 1 ? FR::from_acc(s2, ks) : FR::from_acc(dp, ks);
         const T* src = m == 2 ? g : q;
 #pragma unroll
-        for (int nb = (m == 1 ? NB / 2 : 0); nb < (m == 0 ? NB / 2 : NB); nb += 2) {
-          float x[2][4] = {};
+        for (int nb = (m == 1 ? NB / 2 : 0); nb < (m == 0 ? NB / 2 : NB); nb += G::HALF_SIDE) {
+          float x[G::HALF_SIDE][4] = {};
 #pragma unroll
           for (int ks = 0; ks < SUB / KS; ks++) {
-            typename FR::B w[2];
-            FR::ldB2_kn(w, src, PITCH, s0 + ks * KS, nb * 8, lane);
-            FR::mma2(x[0], x[1], f[ks], w);
+            typename FR::B w[G::HALF_SIDE];
+            FR::ldB_kn(w, src, PITCH, s0 + ks * KS, nb * 8, lane);
+            FR::mma(x, f[ks], w);
           }
 #pragma unroll
-          for (int i = 0; i < 2; i++)
+          for (int i = 0; i < G::HALF_SIDE; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               if (m == 2) {
@@ -992,8 +989,10 @@ int fwd_launch(rnn_ctx* ctx, Args a) {
   RNN_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
   static std::atomic<unsigned long long> optin{0};
   RNN_TRY(tc::ensure_smem_optin(fwd_kernel<T, DH, RW>, optin, ctx->device, static_cast<int>(F::SMEM)));
-  // Split the keys when the rows alone do not give every SM a block, in parts
-  // of at least four tiles.
+  // Split the keys when the rows alone do not give every SM a block: in parts of
+  // at least four tiles, or for a token's few rows of one (one row and 777 keys
+  // in f32, two sequences of 4 heads: 10.9 us with parts of a tile, 16.0 of two,
+  // 21.6 of four).
   static std::atomic<int> resident{0};  // blocks of this kernel an SM holds (every device here is the same part)
   int per_sm = resident.load(std::memory_order_relaxed);
   if (per_sm == 0) {
@@ -1002,7 +1001,7 @@ int fwd_launch(rnn_ctx* ctx, Args a) {
   }
   const long long slots = static_cast<long long>(ctx->num_sms) * std::max(1, per_sm);
   const int tiles = (a.tk + F::BN - 1) / F::BN;
-  long long ns = std::min<long long>(slots / std::max(1ll, blocks), tiles / 4);
+  long long ns = std::min<long long>(slots / std::max(1ll, blocks), RW == 1 ? tiles : tiles / 4);
   a.nsplit = static_cast<int>(std::max(1ll, ns));
   a.split_keys = (tiles + a.nsplit - 1) / a.nsplit * F::BN;
   a.nsplit = std::max(1, (a.tk + a.split_keys - 1) / std::max(1, a.split_keys));

@@ -117,7 +117,7 @@ __device__ __forceinline__ void store2(T* p, float x, float y, bool ok0, bool ok
 // three m16n8k8 MMAs (lo*hi, hi*lo, hi*hi) leave an error near 2^-22.
 // In both, `from_acc` turns accumulator blocks into the A operand of the next
 // product without moving data between lanes: for f32 the contraction index is
-// renumbered (lane t holds keys 2t and 2t+1), which `ldB2_kn` matches.
+// renumbered (lane t holds keys 2t and 2t+1), which `ldB_kn` matches.
 
 template <class T>
 struct Frag;
@@ -141,21 +141,29 @@ struct Frag<__nv_bfloat16> {
                  : "r"(p));
     return a;
   }
-  // B operands of columns n0 .. n0+15 (two blocks) from a tile stored [n][k]
-  static __device__ __forceinline__ void ldB2_nk(B (&b)[2], const T* s, int pitch, int n0, int k0, int lane) {
+  // B operands of N blocks of 8 columns (N even) at n0 from a tile stored [n][k]
+  template <int N>
+  static __device__ __forceinline__ void ldB_nk(B (&b)[N], const T* s, int pitch, int n0, int k0, int lane) {
     const int mi = lane >> 3;
-    const uint32_t p = smem_addr(s + (n0 + (mi >> 1) * 8 + (lane & 7)) * pitch + k0 + (mi & 1) * 8);
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(b[0].x[0]), "=r"(b[0].x[1]), "=r"(b[1].x[0]), "=r"(b[1].x[1])
-                 : "r"(p));
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint32_t p = smem_addr(s + (n0 + 8 * i + (mi >> 1) * 8 + (lane & 7)) * pitch + k0 + (mi & 1) * 8);
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(b[i].x[0]), "=r"(b[i].x[1]), "=r"(b[i + 1].x[0]), "=r"(b[i + 1].x[1])
+                   : "r"(p));
+    }
   }
   // the same from a tile stored [k][n]
-  static __device__ __forceinline__ void ldB2_kn(B (&b)[2], const T* s, int pitch, int k0, int n0, int lane) {
+  template <int N>
+  static __device__ __forceinline__ void ldB_kn(B (&b)[N], const T* s, int pitch, int k0, int n0, int lane) {
     const int mi = lane >> 3;
-    const uint32_t p = smem_addr(s + (k0 + (mi & 1) * 8 + (lane & 7)) * pitch + n0 + (mi >> 1) * 8);
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(b[0].x[0]), "=r"(b[0].x[1]), "=r"(b[1].x[0]), "=r"(b[1].x[1])
-                 : "r"(p));
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint32_t p = smem_addr(s + (k0 + (mi & 1) * 8 + (lane & 7)) * pitch + n0 + 8 * i + (mi >> 1) * 8);
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(b[i].x[0]), "=r"(b[i].x[1]), "=r"(b[i + 1].x[0]), "=r"(b[i + 1].x[1])
+                   : "r"(p));
+    }
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -172,15 +180,17 @@ struct Frag<__nv_bfloat16> {
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x[0]), "r"(a.x[1]), "r"(a.x[2]), "r"(a.x[3]), "r"(b.x[0]), "r"(b.x[1]));
   }
-  // two products with one A operand; four with two
-  static __device__ __forceinline__ void mma2(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
-    mma(d0, a, b[0]);
-    mma(d1, a, b[1]);
+  // d += a b for N blocks of columns; and a second such set e += c f
+  template <int N>
+  static __device__ __forceinline__ void mma(float (*d)[4], const A& a, const B (&b)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) mma(d[i], a, b[i]);
   }
-  static __device__ __forceinline__ void mma4(float (&d)[2][4], float (&e)[2][4], const A& a, const A& c,
-                                              const B (&b)[2]) {
-    mma2(d[0], d[1], a, b);
-    mma2(e[0], e[1], c, b);
+  template <int N>
+  static __device__ __forceinline__ void mma(float (*d)[4], const A& a, const B (&b)[N], float (*e)[4], const A& c,
+                                             const B (&f)[N]) {
+    mma(d, a, b);
+    mma(e, c, f);
   }
 };
 
@@ -207,18 +217,20 @@ struct Frag<float> {
     split(p[8 * pitch + 4], a.hi[3], a.lo[3]);
     return a;
   }
-  static __device__ __forceinline__ void ldB2_nk(B (&b)[2], const T* s, int pitch, int n0, int k0, int lane) {
+  template <int N>
+  static __device__ __forceinline__ void ldB_nk(B (&b)[N], const T* s, int pitch, int n0, int k0, int lane) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < N; i++) {
       const T* p = s + (n0 + 8 * i + (lane >> 2)) * pitch + k0 + (lane & 3);
       split(p[0], b[i].hi[0], b[i].lo[0]);
       split(p[4], b[i].hi[1], b[i].lo[1]);
     }
   }
-  static __device__ __forceinline__ void ldB2_kn(B (&b)[2], const T* s, int pitch, int k0, int n0, int lane) {
+  template <int N>
+  static __device__ __forceinline__ void ldB_kn(B (&b)[N], const T* s, int pitch, int k0, int n0, int lane) {
     const T* p = s + (k0 + 2 * (lane & 3)) * pitch + n0 + (lane >> 2);
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < N; i++) {
       split(p[8 * i], b[i].hi[0], b[i].lo[0]);
       split(p[pitch + 8 * i], b[i].hi[1], b[i].lo[1]);
     }
@@ -237,30 +249,32 @@ struct Frag<float> {
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
   }
-  // The three parts of a product depend on one another; several products take
-  // turns so that none waits for its own last part.
-  static __device__ __forceinline__ void mma2(float (&d0)[4], float (&d1)[4], const A& a, const B (&b)[2]) {
-    mma1(d0, a.lo, b[0].hi);
-    mma1(d1, a.lo, b[1].hi);
-    mma1(d0, a.hi, b[0].lo);
-    mma1(d1, a.hi, b[1].lo);
-    mma1(d0, a.hi, b[0].hi);
-    mma1(d1, a.hi, b[1].hi);
+  // The three parts of a product depend on one another; the products of a set
+  // take turns so that none waits for its own last part.
+  template <int N>
+  static __device__ __forceinline__ void mma(float (*d)[4], const A& a, const B (&b)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) mma1(d[i], a.lo, b[i].hi);
+#pragma unroll
+    for (int i = 0; i < N; i++) mma1(d[i], a.hi, b[i].lo);
+#pragma unroll
+    for (int i = 0; i < N; i++) mma1(d[i], a.hi, b[i].hi);
   }
-  static __device__ __forceinline__ void mma4(float (&d)[2][4], float (&e)[2][4], const A& a, const A& c,
-                                              const B (&b)[2]) {
+  template <int N>
+  static __device__ __forceinline__ void mma(float (*d)[4], const A& a, const B (&b)[N], float (*e)[4], const A& c,
+                                             const B (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) mma1(d[i], a.lo, b[i].hi);
+    for (int i = 0; i < N; i++) mma1(d[i], a.lo, b[i].hi);
 #pragma unroll
-    for (int i = 0; i < 2; i++) mma1(e[i], c.lo, b[i].hi);
+    for (int i = 0; i < N; i++) mma1(e[i], c.lo, f[i].hi);
 #pragma unroll
-    for (int i = 0; i < 2; i++) mma1(d[i], a.hi, b[i].lo);
+    for (int i = 0; i < N; i++) mma1(d[i], a.hi, b[i].lo);
 #pragma unroll
-    for (int i = 0; i < 2; i++) mma1(e[i], c.hi, b[i].lo);
+    for (int i = 0; i < N; i++) mma1(e[i], c.hi, f[i].lo);
 #pragma unroll
-    for (int i = 0; i < 2; i++) mma1(d[i], a.hi, b[i].hi);
+    for (int i = 0; i < N; i++) mma1(d[i], a.hi, b[i].hi);
 #pragma unroll
-    for (int i = 0; i < 2; i++) mma1(e[i], c.hi, b[i].hi);
+    for (int i = 0; i < N; i++) mma1(e[i], c.hi, f[i].hi);
   }
 };
 
@@ -275,6 +289,10 @@ struct Geo {
   // keys (or queries) of one register step; 16 where the f32 fragments of a
   // 32-wide step would not fit the register file
   static constexpr int SUB = sizeof(T) == 4 && DH == 64 ? 16 : 32;
+  // column blocks whose products run side by side: few MMAs in a row wait for
+  // one another, as far as registers go
+  static constexpr int SIDE = sizeof(T) == 4 && DH < 64 ? 4 : 2;
+  static constexpr int HALF_SIDE = SIDE < DH / 8 ? SIDE : DH / 8;  // of one half
 };
 
 // Loads ROWS rows of 2*dh columns into a PITCH-wide tile.  row(r) gives the
