@@ -1147,6 +1147,7 @@ bool aligned(std::initializer_list<const void*> ps, size_t bytes) {
 }  // namespace
 
 int join_parts(rnn_ctx* ctx, const Args& a) { return join_launch<__nv_bfloat16, 128>(ctx, a); }
+int join_parts_f32(rnn_ctx* ctx, const Args& a) { return join_launch<float, 64>(ctx, a); }
 
 }  // namespace diff
 }  // namespace rnn
@@ -1171,7 +1172,7 @@ extern "C" int rnn_diffattn_fwd_dev(rnn_ctx* ctx, const rnn_diffattn* d, const v
   a.vec = a.dh % (16 / esz) == 0 && diff::aligned({q, k, v}, 16) &&
           diff::multiples({a.qb, a.qr, a.qh, a.kb, a.kr, a.kh, a.vb, a.vr, a.vh}, 16 / esz);
   a.pair = diff::multiples({a.ob, a.orow, a.oh}, 2) && diff::aligned({o}, 2 * esz);
-  if (d->dtype == RNN_F32) return diff::fwd_type<float>(ctx, a);
+  if (d->dtype == RNN_F32) return diff::f32_tc_ok(a) ? diff::f32_tc_fwd(ctx, a) : diff::fwd_type<float>(ctx, a);
   if (diff::dec_ok(a)) return diff::dec_fwd(ctx, a);
   return diff::tc_fwd_ok(a) ? diff::tc_fwd(ctx, a) : diff::fwd_type<__nv_bfloat16>(ctx, a);
 }

@@ -1,0 +1,520 @@
+// Differential attention in f32 on tcgen05: halves of up to 32 columns, every
+// stride and mask, forward and backward.
+//
+// An f32 operand is split into three bf16 planes, x = h + m + l with h, m, l the
+// rounded value, the rounded rest and its rest (24 bits), and a product is six
+// bf16 MMAs: l h, h l, m m, m h, h m, h h (what is left out is below 2^-24).
+// The small ones come first and every key tile's product starts from zero and
+// joins the f32 accumulators in registers, so that the accumulation in tensor
+// memory rounds few large sums.
+//
+// Operands go through registers to be split, so they are read with plain loads
+// (any stride, masked keys as zeros) and written as 128-byte-swizzled tiles:
+// rows of 64 columns, the two halves of q and k side by side.  A block owns 128
+// packed rows (queries of a key head's group, or keys) and has 8 arithmetic
+// warps, two threads a row with 32 columns each, 7 loading warps and one that
+// issues MMAs.
+#include <algorithm>
+
+#include "diffattn_tc.cuh"
+
+namespace rnn {
+namespace diff {
+namespace {
+
+constexpr int ROWS = 128, COLS = 64;  // of a block; of a step
+constexpr int THREADS = 512;
+constexpr int MATH_WARPS = 8, LOAD_WARPS = 7, WARP_MMA = 15, LOADERS = LOAD_WARPS * 32;
+constexpr uint32_t ROW_PLANE = ROWS * 128, COL_PLANE = COLS * 128;  // bytes
+constexpr uint32_t ROW_TILE = 3 * ROW_PLANE, COL_TILE = 3 * COL_PLANE;
+constexpr int FWD_STAGES = 3, BWD_STAGES = 2;
+
+// Tensor memory columns.  Forward: S_1 S_2 | planes of P_1, P_2 | P_1 v, P_2 v.
+// Queries' backward: S_1 S_2 dP | planes of dS_1, dS_2 | dq.  Keys' backward: the
+// planes of dS_1, dS_2 and P_1 - lam P_2 overwrite S_1, S_2 and dP, each of
+// which has room for three planes | dv, dk.
+constexpr uint32_t MAP = 96;  // three planes of 64 bf16 columns
+constexpr uint32_t FWD_P = 128, FWD_O = FWD_P + 2 * MAP;
+constexpr uint32_t Q_P = 192, Q_O = Q_P + 2 * MAP;
+constexpr uint32_t KV_O = 3 * MAP;
+
+struct Shared {
+  uint64_t rows_full, full[FWD_STAGES], empty[FWD_STAGES], s_full, s_free, p_full, o_full, pair[4], drain;
+  uint32_t tmem;
+  int abort_flag;
+  float2 give[2][2][ROWS];
+  uint32_t seen[FWD_STAGES][2];  // keys of a tile that exist and are not masked
+  float stat[BWD_STAGES][5][COLS];  // lse_1, lse_2, D_1, D_2, limit of a tile's queries
+};
+constexpr size_t FWD_SMEM = 1024 + ROW_TILE + FWD_STAGES * 2 * COL_TILE + sizeof(Shared);
+constexpr size_t BWD_SMEM = 1024 + 2 * ROW_TILE + BWD_STAGES * 2 * COL_TILE + sizeof(Shared);
+
+struct Params {
+  Args a;
+  int* dev_error;  // the context's error word
+  int st16;        // 16-byte stores of the outputs are aligned
+  int st16_2;      // and of o2
+};
+
+// Two values as three planes of bf16 pairs.
+__device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  const f32x2 minus = pair(-1.0f, -1.0f);
+  h = pack2(x, y);
+  f32x2 r = fma2(pair(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), minus, pair(x, y));
+  unpair(r, x, y);
+  m = pack2(x, y);
+  r = fma2(pair(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)), minus, r);
+  unpair(r, x, y);
+  l = pack2(x, y);
+}
+
+// Eight columns (chunk c) of a row of 2*dh values, zeros beyond; p is the row or
+// null.  SPLIT rows (q, k) put the halves at columns 0 and 32.
+template <bool SPLIT>
+__device__ __forceinline__ void load8(float (&x)[8], const float* p, int c, const Args& a) {
+#pragma unroll
+  for (int k = 0; k < 8; k++) x[k] = 0.0f;
+  if (p == nullptr) return;
+  const int w = SPLIT ? (c & 3) * 8 : c * 8, in = (SPLIT ? a.dh : 2 * a.dh) - w;
+  p += w + (SPLIT ? (c >> 2) * a.dh : 0);
+  if (a.vec) {  // dh is a multiple of 4
+    if (in >= 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    }
+    if (in >= 8) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (k < in) x[k] = __ldg(p + k);
+  }
+}
+// Their planes, as chunk c of row r of a tile of R rows.
+template <int R>
+__device__ __forceinline__ void store8(uint8_t* dst, const float (&x)[8], int r, int c) {
+  uint32_t z[3][4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) split3(x[2 * k], x[2 * k + 1], z[0][k], z[1][k], z[2][k]);
+#pragma unroll
+  for (int q = 0; q < 3; q++)
+    *reinterpret_cast<uint4*>(dst + q * (R * 128) + r * 128 + ((c ^ (r & 7)) << 4)) =
+        make_uint4(z[q][0], z[q][1], z[q][2], z[q][3]);
+}
+// The block's own 128 rows, by the arithmetic warps (thread t of 256), which
+// have nothing else to do then.
+template <bool SPLIT, class Row>
+__device__ __forceinline__ void load_rows(uint8_t* dst, const Args& a, int t, float scale, Row row) {
+  constexpr int N = ROWS * 8 / (MATH_WARPS * 32);
+  float x[N][8];
+#pragma unroll
+  for (int u = 0; u < N; u++) load8<SPLIT>(x[u], row((t >> 3) + u * (ROWS / N)), t & 7, a);
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[u][k] *= scale;
+    store8<ROWS>(dst, x[u], (t >> 3) + u * (ROWS / N), t & 7);
+  }
+}
+// Two tiles of a step (k and v, or q and dout), by the loading warps, all loads
+// in flight at once.
+template <class First, class Second>
+__device__ __forceinline__ void load_step(uint8_t* dst, const Args& a, int t, First first, Second second) {
+  constexpr int ITEMS = COLS * 8, N = (2 * ITEMS + LOADERS - 1) / LOADERS;
+  float x[N][8];
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+    const int i = t + u * LOADERS, r = (i & (ITEMS - 1)) >> 3;
+    if (i < ITEMS) {
+      load8<true>(x[u], first(r), i & 7, a);
+    } else if (i < 2 * ITEMS) {
+      load8<false>(x[u], second(r), i & 7, a);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+    const int i = t + u * LOADERS, r = (i & (ITEMS - 1)) >> 3;
+    if (i < 2 * ITEMS) store8<COLS>(dst + (i < ITEMS ? 0 : COL_TILE), x[u], r, i & 7);
+  }
+}
+
+// The planes of 32 values of a row: 16 columns of each plane of the map at `dst`.
+__device__ __forceinline__ void store_planes(uint32_t dst, const float (&s)[32]) {
+#pragma unroll
+  for (int g = 0; g < 2; g++) {
+    uint32_t z[3][8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) split3(s[g * 16 + 2 * k], s[g * 16 + 2 * k + 1], z[0][k], z[1][k], z[2][k]);
+#pragma unroll
+    for (int q = 0; q < 3; q++) tmem_st(dst + q * 32 + g * 8, z[q]);
+  }
+}
+
+// acc <- al acc + 32 columns of tensor memory.
+__device__ __forceinline__ void add_tmem(uint32_t src, float (&acc)[32], float al) {
+  const f32x2 f = pair(al, al);
+#pragma unroll
+  for (int g = 0; g < 2; g++) {
+    float x[16];
+    tmem_ld(src + g * 16, x);
+    tmem_landed(x);
+#pragma unroll
+    for (int k = 0; k < 16; k += 2) {
+      float &u = acc[g * 16 + k], &v = acc[g * 16 + k + 1];
+      unpair(fma2(pair(u, v), f, pair(x[k], x[k + 1])), u, v);
+    }
+  }
+}
+// s <- 2^(s - u); returns the sum.
+__device__ __forceinline__ float exp_sum(float (&s)[32], float u) {
+  const f32x2 uu = pair(-u, -u);
+  f32x2 t[2] = {0ull, 0ull};
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    float &x = s[2 * i], &y = s[2 * i + 1];
+    unpair(add2(pair(x, y), uu), x, y);
+    x = ex2(x);
+    y = ex2(y);
+    t[i & 1] = add2(t[i & 1], pair(x, y));
+  }
+  float x, y;
+  unpair(add2(t[0], t[1]), x, y);
+  return x + y;
+}
+__device__ __forceinline__ float max_of(const float (&s)[32]) {
+  float m[2] = {s[0], s[1]};
+#pragma unroll
+  for (int c = 2; c < 32; c++) m[c & 1] = fmaxf(m[c & 1], s[c]);
+  return fmaxf(m[0], m[1]);
+}
+
+// The six products of two operands in planes, the small ones first.
+template <int KMAX, class Step>
+__device__ __forceinline__ void products(int ksteps, Step step) {
+  constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+  for (int p = 0; p < 6; p++)
+#pragma unroll
+    for (int ks = 0; ks < KMAX; ks++)
+      if (ks < ksteps) step(PA[p], PB[p], ks, p > 0 || ks > 0);
+}
+
+// A warp's 32 rows x 32 columns, a row a thread, to rows in memory: through
+// shared memory, so that eight threads store 128 bytes of a row.  `to` is where
+// the thread's row goes, or null; `in` of its columns exist.
+__device__ __forceinline__ void store_rows(float* patch, const float (&x)[32], int in, bool st16, float* to) {
+  const int lane = threadIdx.x & 31, c = lane & 7;
+#pragma unroll
+  for (int k = 0; k < 8; k++)
+    *reinterpret_cast<float4*>(patch + lane * 32 + ((k ^ (lane & 7)) << 2)) =
+        make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const int r = k * 4 + (lane >> 3);
+    float* p = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), r));
+    if (p == nullptr) continue;
+    const float4 v = *reinterpret_cast<const float4*>(patch + r * 32 + ((c ^ (r & 7)) << 2));
+    p += c * 4;
+    if (st16 && c * 4 + 4 <= in) {
+      *reinterpret_cast<float4*>(p) = v;
+    } else {
+      const float z[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (c * 4 + e < in) p[e] = z[e];
+    }
+  }
+  __syncwarp();
+}
+
+struct Block {
+  Shared& sh;
+  int* dev_error;
+  __device__ __forceinline__ bool done(uint64_t* bar, uint32_t parity) {
+    return warp_wait(bar, parity, &sh.abort_flag, dev_error);
+  }
+  // What the two threads of a row tell each other; `turn` counts the exchanges.
+  __device__ __forceinline__ bool exchange(int& turn, int w, int part, int row, float2 mine, float2& other) {
+    sh.give[turn & 1][part][row] = mine;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.pair[w]);
+    if (!done(&sh.pair[w], turn & 1)) return false;
+    other = sh.give[turn & 1][part ^ 1][row];
+    turn++;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void setup(Shared& sh, int warp) {
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.rows_full, MATH_WARPS);
+    for (int i = 0; i < FWD_STAGES; i++) {
+      mbar_init(&sh.full[i], LOAD_WARPS);
+      mbar_init(&sh.empty[i], 1);
+    }
+    mbar_init(&sh.s_full, 1);
+    mbar_init(&sh.s_free, MATH_WARPS);
+    mbar_init(&sh.p_full, MATH_WARPS);
+    mbar_init(&sh.o_full, 1);
+    for (int i = 0; i < 4; i++) mbar_init(&sh.pair[i], 2);
+    mbar_init(&sh.drain, 1);
+    sh.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == WARP_MMA) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+}
+__device__ __forceinline__ void signal(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// Packed rows of a (sequence, key head): head and query of a row.
+__device__ __forceinline__ const float* packed(const void* base, const Args& a, int p, int rows, long long sb,
+                                               long long sr, long long sh, int b, int kvh) {
+  if (p >= rows) return nullptr;
+  const int e = p / a.tq;
+  return static_cast<const float*>(base) + b * sb + (static_cast<long long>(kvh) * a.grp + e) * sh + (p - e * a.tq) * sr;
+}
+
+// Loads tiles of keys [kbeg, kend) for the kernels that own query rows.
+__device__ __forceinline__ void load_keys(Block& blk, uint8_t* stages, int nstage, const Args& a, int b, int kvh,
+                                          int kbeg, int kend, int nt, int t0) {
+  const float* kp = static_cast<const float*>(a.k) + b * a.kb + kvh * a.kh;
+  const float* vp = static_cast<const float*>(a.v) + b * a.vb + kvh * a.vh;
+  const uint8_t* mask = a.kmask ? a.kmask + b * a.kmb : nullptr;
+  for (int t = 0; t < nt; t++) {
+    const int st = t % nstage, j0 = kbeg + t * COLS;
+    if (t >= nstage && !blk.done(&blk.sh.empty[st], (t / nstage - 1) & 1)) break;
+    auto on = [&](int r) { return j0 + r < kend && (!mask || mask[j0 + r]); };
+    load_step(stages + st * (2 * COL_TILE), a, t0, [&](int r) { return on(r) ? kp + (j0 + r) * a.kr : nullptr; },
+              [&](int r) { return on(r) ? vp + (j0 + r) * a.vr : nullptr; });
+    if (t0 < 64) {
+      const uint32_t bits = __ballot_sync(0xffffffffu, on(t0));
+      if ((t0 & 31) == 0) blk.sh.seen[st][t0 >> 5] = bits;
+    }
+    fence_async_smem();
+    signal(&blk.sh.full[st]);
+  }
+}
+
+__global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  const Args& a = p.a;
+  uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* stages = base + ROW_TILE;
+  Shared& sh = *reinterpret_cast<Shared*>(stages + FWD_STAGES * 2 * COL_TILE);
+  Block blk{sh, p.dev_error};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rows = a.grp * a.tq, nbh = a.n * a.hkv, ntile = (rows + ROWS - 1) / ROWS;
+  const int tile = ntile - 1 - static_cast<int>(blockIdx.x) / nbh;  // longest causal rows first
+  const int bh = static_cast<int>(blockIdx.x) % nbh, b = bh / a.hkv, kvh = bh - b * a.hkv;
+  const int row0 = tile * ROWS, len = key_len(a, b);
+  const int last = min(rows, row0 + ROWS) - 1;
+  // a block that spans a head's end holds that head's last query
+  const int imax = last / a.tq != row0 / a.tq ? a.tq - 1 : last % a.tq;
+  const int kbeg = static_cast<int>(blockIdx.y) * a.split_keys;
+  const int kend = min(row_limit(a, imax, len), kbeg + a.split_keys);
+  const int nt = max(kend - kbeg + COLS - 1, 0) / COLS;
+  setup(sh, warp);
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < MATH_WARPS) {
+    // registers: 512 threads x 128 at launch = 256 x 168 + 256 x 88
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if (nt > 0) {
+      // q in units that make scores exponents of 2
+      load_rows<true>(base, a, tid, a.slog2, [&](int r) { return packed(a.q, a, row0 + r, rows, a.qb, a.qr, a.qh, b, kvh); });
+      fence_async_smem();
+      signal(&sh.rows_full);
+    }
+    const int part = warp >> 2, w = warp & 3, row = w * 32 + lane, r = row0 + row;
+    const uint32_t at = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int e = min(r, rows - 1) / a.tq, i = r - e * a.tq, head = kvh * a.grp + e;
+    const int lim = r < rows ? min(kend, row_limit(a, i, len)) : 0;
+    const int full = __reduce_min_sync(0xffffffffu, lim);
+    float x[32], y[32], m1 = -CUDART_INF_F, m2 = -CUDART_INF_F, l1 = 0.0f, l2 = 0.0f;
+    float al1 = 0.0f, al2 = 0.0f;  // what the sums before the last tile get
+#pragma unroll
+    for (int c = 0; c < 32; c++) x[c] = y[c] = 0.0f;
+    int turn = 0;
+    bool ok = true;
+    for (int t = 0; t < nt; t++) {
+      // the tile's visible keys come from the loading warps, its scores from the MMAs
+      if (!(ok = blk.done(&sh.full[t % FWD_STAGES], (t / FWD_STAGES) & 1) && blk.done(&sh.s_full, t & 1))) break;
+      tc_fence_after();
+      float s1[32], s2[32];
+      tmem_ld(at + part * 32, s1);
+      tmem_ld(at + 64 + part * 32, s2);
+      tmem_landed(s1);
+      tmem_landed(s2);
+      const int j0 = kbeg + t * COLS + part * 32;
+      const uint32_t seen = sh.seen[t % FWD_STAGES][part];
+      tc_fence_before();
+      signal(&sh.s_free);
+      const bool edge = j0 + 32 > full || seen != 0xffffffffu;
+      if (edge) {
+#pragma unroll
+        for (int c = 0; c < 32; c++)
+          if (j0 + c >= lim || !(seen >> c & 1)) s1[c] = s2[c] = -CUDART_INF_F;
+      }
+      float2 top = make_float2(max_of(s1), max_of(s2)), other;
+      if (!(ok = blk.exchange(turn, w, part, row, top, other))) break;
+      top.x = fmaxf(m1, fmaxf(top.x, other.x));
+      top.y = fmaxf(m2, fmaxf(top.y, other.y));
+      // a row without a visible key so far keeps its maximum at -inf
+      const float u1 = top.x == -CUDART_INF_F ? 0.0f : top.x, u2 = top.y == -CUDART_INF_F ? 0.0f : top.y;
+      const float f1 = ex2(m1 - u1), f2 = ex2(m2 - u2);
+      m1 = top.x;
+      m2 = top.y;
+      l1 = l1 * f1 + exp_sum(s1, u1);
+      l2 = l2 * f2 + exp_sum(s2, u2);
+      if (t > 0) {
+        if (!(ok = blk.done(&sh.o_full, (t - 1) & 1))) break;
+        tc_fence_after();
+        add_tmem(at + FWD_O + part * 32, x, al1);
+        add_tmem(at + FWD_O + 64 + part * 32, y, al2);
+      }
+      al1 = f1;
+      al2 = f2;
+      store_planes(at + FWD_P + part * 16, s1);
+      store_planes(at + FWD_P + MAP + part * 16, s2);
+      tmem_wait_st();
+      tc_fence_before();
+      signal(&sh.p_full);
+    }
+    if (ok && nt > 0 && (ok = blk.done(&sh.o_full, (nt - 1) & 1))) {
+      tc_fence_after();
+      add_tmem(at + FWD_O + part * 32, x, al1);
+      add_tmem(at + FWD_O + 64 + part * 32, y, al2);
+    }
+    float2 other;
+    if (ok && blk.exchange(turn, w, part, row, make_float2(l1, l2), other)) {
+      // the same order of the two sums in both threads
+      const float L1 = part ? other.x + l1 : l1 + other.x, L2 = part ? other.y + l2 : l2 + other.y;
+      float* patch = reinterpret_cast<float*>(base) + warp * 1024;  // q is no longer read
+      if (a.nsplit > 1) {
+        const long long to = (static_cast<long long>(blockIdx.y) * nbh + bh) * rows + r;
+        float* q = r < rows ? a.part + to * 128 + part * 32 : nullptr;
+        store_rows(patch, x, 32, true, q);
+        store_rows(patch, y, 32, true, q ? q + 64 : nullptr);
+        if (part == 0 && r < rows) *reinterpret_cast<float4*>(a.stat + to * 4) = make_float4(m1, L1, m2, L2);
+      } else {
+        const bool any = L1 > 0.0f && L2 > 0.0f;
+        const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f;
+        const float lam = any ? __ldg(a.lam + head) : 0.0f;
+#pragma unroll
+        for (int c = 0; c < 32; c++) {
+          y[c] = any ? y[c] * i2 : 0.0f;
+          x[c] = any ? x[c] * i1 - lam * y[c] : 0.0f;
+        }
+        const int in = 2 * a.dh - part * 32;
+        store_rows(patch, x, in, p.st16,
+                   r < rows ? static_cast<float*>(a.o) + b * a.ob + head * a.oh + i * a.orow + part * 32 : nullptr);
+        if (a.o2)
+          store_rows(patch, y, in, p.st16_2,
+                     r < rows ? static_cast<float*>(a.o2) +
+                                    ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + part * 32
+                              : nullptr);
+        if (a.lse && part == 0 && r < rows) {
+          float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
+          s[0] = any ? m1 + log2f(L1) : CUDART_INF_F;
+          s[a.tq] = any ? m2 + log2f(L2) : CUDART_INF_F;
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < WARP_MMA) {
+      const int t0 = tid - MATH_WARPS * 32;
+      if (nt > 0) load_keys(blk, stages, FWD_STAGES, a, b, kvh, kbeg, kend, nt, t0);
+    } else if (nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_o = idesc_bf16(ROWS, 64, true);
+      const uint64_t dq = desc_k(smem_u32(base)), dk = desc_k(smem_u32(stages));
+      const uint64_t dv = desc_mn(smem_u32(stages) + COL_TILE, 0);
+      const int ksteps = (a.dh + 15) / 16;
+      bool ok = blk.done(&sh.rows_full, 0);
+      for (int t = 0; ok && t <= nt; t++) {
+        if (t < nt) {
+          const int st = t % FWD_STAGES;
+          if (!(ok = blk.done(&sh.full[st], (t / FWD_STAGES) & 1) && (t == 0 || blk.done(&sh.s_free, (t - 1) & 1)))) break;
+          tc_fence_after();
+          const uint64_t k = dk + st * (2 * COL_TILE / 16);
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+            products<2>(ksteps, [&](int pa, int pb, int ks, bool acc) {
+              mma_ss(tmem + m * 64, dq + (pa * ROW_PLANE + m * 64 + ks * 32) / 16,
+                     k + (pb * COL_PLANE + m * 64 + ks * 32) / 16, id_s, acc, lead);
+            });
+          commit(&sh.s_full, lead);
+        }
+        if (t > 0) {
+          const int st = (t - 1) % FWD_STAGES;
+          if (!(ok = blk.done(&sh.p_full, (t - 1) & 1))) break;
+          tc_fence_after();
+          const uint64_t v = dv + st * (2 * COL_TILE / 16);
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+            products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+              mma_ts(tmem + FWD_O + m * 64, tmem + FWD_P + m * MAP + pa * 32 + ks * 8,
+                     v + (pb * COL_PLANE + ks * 2048) / 16, id_o, acc, lead);
+            });
+          commit(&sh.empty[st], lead);
+          commit(&sh.o_full, lead);
+        }
+      }
+      if (!ok) {  // no MMA may write tensor memory after it is released
+        commit(&sh.drain, lead);
+        settle(&sh.drain, 0);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace
+
+bool f32_tc_ok(const Args& a) { return a.dh <= 32 && static_cast<long long>(a.grp) * a.tq >= 64 && a.tk >= 32; }
+
+int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
+  Params p;
+  p.a = a;
+  p.dev_error = ctx->dev_error;
+  auto m4 = [](long long s) { return s % 4 == 0; };
+  p.st16 = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && m4(a.ob) && m4(a.orow) && m4(a.oh);
+  p.st16_2 = reinterpret_cast<uintptr_t>(a.o2) % 16 == 0 && a.dh % 2 == 0;
+  const long long rows = static_cast<long long>(a.grp) * a.tq, nbh = static_cast<long long>(a.n) * a.hkv;
+  const long long blocks = (rows + ROWS - 1) / ROWS * nbh;
+  RNN_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  const int tiles = (a.tk + COLS - 1) / COLS;
+  const long long parts = std::max(1ll, std::min<long long>(ctx->num_sms / blocks, tiles / 4));
+  p.a.split_keys = static_cast<int>((tiles + parts - 1) / parts) * COLS;
+  p.a.nsplit = (a.tk + p.a.split_keys - 1) / p.a.split_keys;
+  if (p.a.nsplit > 1) {
+    const size_t all = static_cast<size_t>(p.a.nsplit) * nbh * rows;
+    RNN_TRY(ensure_ws(ctx, all * (128 + 4) * sizeof(float)));
+    p.a.part = static_cast<float*>(ctx->ws);
+    p.a.stat = p.a.part + all * 128;
+  }
+  static std::atomic<unsigned long long> optin{0};
+  RNN_TRY(tc::ensure_smem_optin(f32_fwd_kernel, optin, ctx->device, static_cast<int>(FWD_SMEM)));
+  f32_fwd_kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), THREADS, FWD_SMEM, ctx->stream>>>(p);
+  RNN_CHECK_LAUNCH();
+  return p.a.nsplit > 1 ? join_parts_f32(ctx, p.a) : RNN_OK;
+}
+
+}  // namespace diff
+}  // namespace rnn
