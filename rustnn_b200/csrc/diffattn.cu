@@ -1226,5 +1226,6 @@ extern "C" int rnn_diffattn_bwd_dev(rnn_ctx* ctx, const rnn_diffattn* d, const r
   a.dlrow = a.dsum + 2 * nrow;
   a.kpart = a.dsum + sums;
   if (tensor) return diff::tc_bwd(ctx, a);
-  return d->dtype == RNN_F32 ? diff::bwd_type<float>(ctx, a) : diff::bwd_type<__nv_bfloat16>(ctx, a);
+  if (d->dtype == RNN_F32) return diff::f32_tc_ok(a) ? diff::f32_tc_bwd(ctx, a) : diff::bwd_type<float>(ctx, a);
+  return diff::bwd_type<__nv_bfloat16>(ctx, a);
 }

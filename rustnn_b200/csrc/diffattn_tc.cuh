@@ -244,6 +244,7 @@ int join_parts(rnn_ctx* ctx, const Args& a);
 // The same in f32, whose parts have 64 columns.
 bool f32_tc_ok(const Args& a);
 int f32_tc_fwd(rnn_ctx* ctx, const Args& a);
+int f32_tc_bwd(rnn_ctx* ctx, const Args& a);
 int join_parts_f32(rnn_ctx* ctx, const Args& a);
 
 }  // namespace diff

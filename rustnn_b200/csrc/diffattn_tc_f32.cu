@@ -44,7 +44,8 @@ struct Shared {
   int abort_flag;
   float2 give[2][2][ROWS];
   uint32_t seen[FWD_STAGES][2];  // keys of a tile that exist and are not masked
-  float stat[BWD_STAGES][5][COLS];  // lse_1, lse_2, D_1, D_2, limit of a tile's queries
+  alignas(16) float stat[BWD_STAGES][5][COLS];  // lse_1, lse_2, D_1, D_2, limit of a tile's queries
+  int least[BWD_STAGES][2];                     // least limit of 32 of them
 };
 constexpr size_t FWD_SMEM = 1024 + ROW_TILE + FWD_STAGES * 2 * COL_TILE + sizeof(Shared);
 constexpr size_t BWD_SMEM = 1024 + 2 * ROW_TILE + BWD_STAGES * 2 * COL_TILE + sizeof(Shared);
@@ -54,6 +55,7 @@ struct Params {
   int* dev_error;  // the context's error word
   int st16;        // 16-byte stores of the outputs are aligned
   int st16_2;      // and of o2
+  int ld16;        // 16-byte loads of dout, o and o2 are aligned
 };
 
 // Two values as three planes of bf16 pairs.
@@ -485,6 +487,448 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
   if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
 }
 
+// A row's 32 values of the map's exponent to the map: s <- 2^(s - u).
+__device__ __forceinline__ void exp_row(float (&s)[32], float u) {
+  const f32x2 uu = pair(-u, -u);
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    float &x = s[2 * i], &y = s[2 * i + 1];
+    unpair(add2(pair(x, y), uu), x, y);
+    x = ex2(x);
+    y = ex2(y);
+  }
+}
+// sum of x y over a row's 32 values
+__device__ __forceinline__ float dot_row(const float (&x)[32], const float (&y)[32]) {
+  f32x2 t[2] = {0ull, 0ull};
+#pragma unroll
+  for (int i = 0; i < 16; i++) t[i & 1] = fma2(pair(x[2 * i], x[2 * i + 1]), pair(y[2 * i], y[2 * i + 1]), t[i & 1]);
+  float u, v;
+  unpair(add2(t[0], t[1]), u, v);
+  return u + v;
+}
+// s <- s (dp - d)
+__device__ __forceinline__ void times_rest(float (&s)[32], const float (&dp)[32], float d) {
+  const f32x2 dd = pair(-d, -d);
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+    unpair(mul2(pair(s[2 * i], s[2 * i + 1]), add2(pair(dp[2 * i], dp[2 * i + 1]), dd)), s[2 * i], s[2 * i + 1]);
+}
+
+// dq of 128 packed rows, D_1 and D_2 of each (for the keys' kernel), and the row
+// sums of P_2 dP over those of P_2.
+__global__ void __launch_bounds__(THREADS, 1) f32_bwd_q_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  const Args& a = p.a;
+  uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* stages = base + 2 * ROW_TILE;
+  Shared& sh = *reinterpret_cast<Shared*>(stages + BWD_STAGES * 2 * COL_TILE);
+  Block blk{sh, p.dev_error};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rows = a.grp * a.tq, nbh = a.n * a.hkv, ntile = (rows + ROWS - 1) / ROWS;
+  const int tile = ntile - 1 - static_cast<int>(blockIdx.x) / nbh;
+  const int bh = static_cast<int>(blockIdx.x) % nbh, b = bh / a.hkv, kvh = bh - b * a.hkv;
+  const int row0 = tile * ROWS, len = key_len(a, b);
+  const int last = min(rows, row0 + ROWS) - 1;
+  const int imax = last / a.tq != row0 / a.tq ? a.tq - 1 : last % a.tq;
+  const int kend = row_limit(a, imax, len);
+  const int nt = (kend + COLS - 1) / COLS;
+  setup(sh, warp);
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < MATH_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if (nt > 0) {
+      load_rows<true>(base, a, tid, a.slog2,
+                      [&](int r) { return packed(a.q, a, row0 + r, rows, a.qb, a.qr, a.qh, b, kvh); });
+      load_rows<false>(base + ROW_TILE, a, tid, 1.0f,
+                       [&](int r) { return packed(a.dout, a, row0 + r, rows, a.gb, a.gr, a.gh, b, kvh); });
+      fence_async_smem();
+      signal(&sh.rows_full);
+    }
+    const int part = warp >> 2, w = warp & 3, row = w * 32 + lane, r = row0 + row;
+    const uint32_t at = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int e = min(r, rows - 1) / a.tq, i = r - e * a.tq, head = kvh * a.grp + e;
+    const int lim = r < rows ? min(kend, row_limit(a, i, len)) : 0;
+    const int full = __reduce_min_sync(0xffffffffu, lim);
+    float ls1 = CUDART_INF_F, ls2 = CUDART_INF_F, d1 = 0.0f, d2 = 0.0f, dl = 0.0f, pl = 0.0f;
+    int turn = 0;
+    bool ok = true;
+    if (r < rows) {
+      const float* s = a.flse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
+      ls1 = s[0];
+      ls2 = s[a.tq];
+    }
+    // D_1 = do . (o + lam o2) and D_2 = do . o2; rows that see one tile of keys
+    // sum P dP there instead (dS of a lone key comes out as 0).
+    if (nt > 1) {
+      if (r < rows) {
+        const float* g = packed(a.dout, a, r, rows, a.gb, a.gr, a.gh, b, kvh) + part * 32;
+        const float* o = static_cast<const float*>(a.fo) + b * a.ob + head * a.oh + i * a.orow + part * 32;
+        const float* o2 = static_cast<const float*>(a.fo2) +
+                          ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + part * 32;
+        const int in = min(2 * a.dh - part * 32, 32);
+        if (p.ld16) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            if (c < in) {
+              const float4 x = __ldg(reinterpret_cast<const float4*>(g + c));
+              const float4 y = __ldg(reinterpret_cast<const float4*>(o + c));
+              const float4 z = __ldg(reinterpret_cast<const float4*>(o2 + c));
+              d1 += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+              d2 += x.x * z.x + x.y * z.y + x.z * z.z + x.w * z.w;
+            }
+        } else {
+          for (int c = 0; c < in; c++) {
+            d1 += g[c] * o[c];
+            d2 += g[c] * o2[c];
+          }
+        }
+        d1 += __ldg(a.lam + head) * d2;
+      }
+      float2 other;
+      ok = blk.exchange(turn, w, part, row, make_float2(d1, d2), other);
+      if (ok) {
+        d1 += other.x;
+        d2 += other.y;
+      }
+    }
+    float dq[32];
+#pragma unroll
+    for (int c = 0; c < 32; c++) dq[c] = 0.0f;
+    for (int t = 0; ok && t < nt; t++) {
+      const int st = t % BWD_STAGES;
+      if (!(ok = blk.done(&sh.full[st], (t / BWD_STAGES) & 1) && blk.done(&sh.s_full, t & 1))) break;
+      tc_fence_after();
+      float s1[32], s2[32], dp[32];
+      tmem_ld(at + part * 32, s1);
+      tmem_ld(at + 64 + part * 32, s2);
+      tmem_ld(at + 128 + part * 32, dp);
+      tmem_landed(s1);
+      tmem_landed(s2);
+      tmem_landed(dp);
+      const int j0 = t * COLS + part * 32;
+      const uint32_t seen = sh.seen[st][part];
+      tc_fence_before();
+      signal(&sh.s_free);
+      if (j0 + 32 > full || seen != 0xffffffffu) {
+#pragma unroll
+        for (int c = 0; c < 32; c++)
+          if (j0 + c >= lim || !(seen >> c & 1)) s1[c] = s2[c] = -CUDART_INF_F;
+      }
+      exp_row(s1, ls1);
+      pl += exp_sum(s2, ls2);
+      const float dlt = dot_row(s2, dp);
+      dl += dlt;
+      if (nt == 1) {
+        float2 other;
+        d1 = dot_row(s1, dp);
+        if (!(ok = blk.exchange(turn, w, part, row, make_float2(d1, dlt), other))) break;
+        d1 += other.x;
+        d2 = dlt + other.y;
+      }
+      times_rest(s1, dp, d1);
+      times_rest(s2, dp, d2);
+      if (t > 0) {
+        if (!(ok = blk.done(&sh.o_full, (t - 1) & 1))) break;
+        tc_fence_after();
+        add_tmem(at + Q_O + part * 32, dq, 1.0f);
+      }
+      store_planes(at + Q_P + part * 16, s1);
+      store_planes(at + Q_P + MAP + part * 16, s2);
+      tmem_wait_st();
+      tc_fence_before();
+      signal(&sh.p_full);
+    }
+    if (ok && nt > 0 && (ok = blk.done(&sh.o_full, (nt - 1) & 1))) {
+      tc_fence_after();
+      add_tmem(at + Q_O + part * 32, dq, 1.0f);
+    }
+    float2 other;
+    if (ok && blk.exchange(turn, w, part, row, make_float2(dl, pl), other)) {
+      if (part == 0 && r < rows) {
+        // over the map's own sum: what the log-sum's rounding does to a whole row cancels
+        const float whole = pl + other.y;
+        float* s = a.dsum + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
+        s[0] = d1;
+        s[a.tq] = d2;
+        a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
+            whole > 0.0f ? (dl + other.x) / whole : 0.0f;
+      }
+      const float f = part ? -a.scale * __ldg(a.lam + head) : a.scale;
+#pragma unroll
+      for (int c = 0; c < 32; c++) dq[c] *= f;
+      store_rows(reinterpret_cast<float*>(base) + warp * 1024, dq, a.dh, p.st16,
+                 r < rows ? static_cast<float*>(a.dq) + b * a.dqb + head * a.dqh + i * a.dqr + part * a.dh : nullptr);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < WARP_MMA) {
+      if (nt > 0) load_keys(blk, stages, BWD_STAGES, a, b, kvh, 0, kend, nt, tid - MATH_WARPS * 32);
+    } else if (nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_o = idesc_bf16(ROWS, 32, true);
+      const uint64_t dq = desc_k(smem_u32(base)), dg = desc_k(smem_u32(base) + ROW_TILE);
+      const uint64_t dk = desc_k(smem_u32(stages)), dv = desc_k(smem_u32(stages) + COL_TILE);
+      const uint64_t dkn = desc_mn(smem_u32(stages), 0);
+      const int ksteps = (a.dh + 15) / 16, vsteps = (2 * a.dh + 15) / 16;
+      bool ok = blk.done(&sh.rows_full, 0);
+      for (int t = 0; ok && t <= nt; t++) {
+        if (t < nt) {
+          const int st = t % BWD_STAGES;
+          if (!(ok = blk.done(&sh.full[st], (t / BWD_STAGES) & 1) && (t == 0 || blk.done(&sh.s_free, (t - 1) & 1)))) break;
+          tc_fence_after();
+          const uint64_t k = dk + st * (2 * COL_TILE / 16), v = dv + st * (2 * COL_TILE / 16);
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+            products<2>(ksteps, [&](int pa, int pb, int ks, bool acc) {
+              mma_ss(tmem + m * 64, dq + (pa * ROW_PLANE + m * 64 + ks * 32) / 16,
+                     k + (pb * COL_PLANE + m * 64 + ks * 32) / 16, id_s, acc, lead);
+            });
+          products<4>(vsteps, [&](int pa, int pb, int ks, bool acc) {
+            mma_ss(tmem + 128, dg + (pa * ROW_PLANE + ks * 32) / 16, v + (pb * COL_PLANE + ks * 32) / 16, id_s, acc, lead);
+          });
+          commit(&sh.s_full, lead);
+        }
+        if (t > 0) {
+          const int st = (t - 1) % BWD_STAGES;
+          if (!(ok = blk.done(&sh.p_full, (t - 1) & 1))) break;
+          tc_fence_after();
+          const uint64_t k = dkn + st * (2 * COL_TILE / 16);
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+            products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+              mma_ts(tmem + Q_O + m * 32, tmem + Q_P + m * MAP + pa * 32 + ks * 8,
+                     k + (pb * COL_PLANE + m * 64 + ks * 2048) / 16, id_o, acc, lead);
+            });
+          commit(&sh.empty[st], lead);
+          commit(&sh.o_full, lead);
+        }
+      }
+      if (!ok) {
+        commit(&sh.drain, lead);
+        settle(&sh.drain, 0);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+}
+
+// dk and dv of 128 keys, over the queries of the group's heads: the transposed
+// maps come from k q^T and v do^T, so that keys stay in the rows.
+__global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  const Args& a = p.a;
+  uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* stages = base + 2 * ROW_TILE;
+  Shared& sh = *reinterpret_cast<Shared*>(stages + BWD_STAGES * 2 * COL_TILE);
+  Block blk{sh, p.dev_error};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nbh = a.n * a.hkv, nkt = (a.tk + ROWS - 1) / ROWS;
+  const bool work = static_cast<int>(blockIdx.x) < nkt * nbh;  // else a block for dlam only
+  const int kt = work ? static_cast<int>(blockIdx.x) / nbh : 0;  // the earliest keys, which most queries see, first
+  const int bh = static_cast<int>(blockIdx.x) % nbh, b = bh / a.hkv, kvh = bh - b * a.hkv;
+  const int key0 = kt * ROWS, len = key_len(a, b);
+  const uint8_t* mask = a.kmask ? a.kmask + b * a.kmb : nullptr;
+  // queries before `qbeg` see none of these keys
+  int qbeg = 0;
+  if (!work || key0 >= len) {
+    qbeg = a.tq;
+  } else if (a.causal == RNN_CAUSAL_START) {
+    qbeg = min(a.tq, key0);
+  } else if (a.causal == RNN_CAUSAL_END) {
+    qbeg = min(a.tq, max(0, key0 - (len - a.tq)));
+  }
+  const int per = (a.tq - qbeg + COLS - 1) / COLS, nt = per * a.grp;
+  setup(sh, warp);
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < MATH_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if (nt > 0) {
+      auto row = [&](const void* q, long long sb, long long sr, long long sh_, int r) -> const float* {
+        const int j = key0 + r;
+        return j < len && (!mask || mask[j]) ? static_cast<const float*>(q) + b * sb + kvh * sh_ + j * sr : nullptr;
+      };
+      load_rows<true>(base, a, tid, a.slog2, [&](int r) { return row(a.k, a.kb, a.kr, a.kh, r); });
+      load_rows<false>(base + ROW_TILE, a, tid, 1.0f, [&](int r) { return row(a.v, a.vb, a.vr, a.vh, r); });
+      fence_async_smem();
+      signal(&sh.rows_full);
+    }
+    const int part = warp >> 2, w = warp & 3, row = w * 32 + lane, key = key0 + row;
+    const uint32_t at = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    // what a query has to see for this key to count
+    const int need = key < len && (!mask || mask[key]) ? key : 0x7fffffff;
+    const int most = __reduce_max_sync(0xffffffffu, need);
+    float dv[32], dk[32];
+#pragma unroll
+    for (int c = 0; c < 32; c++) dv[c] = dk[c] = 0.0f;
+    int turn = 0;
+    bool ok = true;
+    for (int t = 0; t < nt; t++) {
+      const int st = t % BWD_STAGES;
+      if (!(ok = blk.done(&sh.full[st], (t / BWD_STAGES) & 1) && blk.done(&sh.s_full, t & 1))) break;
+      tc_fence_after();
+      float s1[32], s2[32], dp[32];
+      tmem_ld(at + part * 32, s1);
+      tmem_ld(at + MAP + part * 32, s2);
+      tmem_ld(at + 2 * MAP + part * 32, dp);
+      tmem_landed(s1);
+      tmem_landed(s2);
+      tmem_landed(dp);
+      tc_fence_before();
+      // the planes overwrite what both threads of a row have now read
+      float2 other;
+      if (!(ok = blk.exchange(turn, w, part, row, make_float2(0.0f, 0.0f), other))) break;
+      tc_fence_after();
+      const float* stat = &sh.stat[st][0][part * 32];
+      const float lam = __ldg(a.lam + kvh * a.grp + t / per);
+      if (most >= sh.least[st][part]) {
+#pragma unroll
+        for (int c = 0; c < 32; c++)
+          if (need >= __float_as_int(stat[4 * COLS + c])) s1[c] = s2[c] = -CUDART_INF_F;
+      }
+      // after this: s1 = dS_1, s2 = dS_2, dp = P_1 - lam P_2
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const float4 ls1 = *reinterpret_cast<const float4*>(stat + c);
+        const float4 ls2 = *reinterpret_cast<const float4*>(stat + COLS + c);
+        const float4 d1 = *reinterpret_cast<const float4*>(stat + 2 * COLS + c);
+        const float4 d2 = *reinterpret_cast<const float4*>(stat + 3 * COLS + c);
+        const float l1[4] = {ls1.x, ls1.y, ls1.z, ls1.w}, l2[4] = {ls2.x, ls2.y, ls2.z, ls2.w};
+        const float e1[4] = {d1.x, d1.y, d1.z, d1.w}, e2[4] = {d2.x, d2.y, d2.z, d2.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float x = ex2(s1[c + k] - l1[k]), y = lam * ex2(s2[c + k] - l2[k]);
+          s1[c + k] = x * (dp[c + k] - e1[k]);
+          s2[c + k] = y * (e2[k] - dp[c + k]);
+          dp[c + k] = x - y;
+        }
+      }
+      if (t > 0) {
+        if (!(ok = blk.done(&sh.o_full, (t - 1) & 1))) break;
+        tc_fence_after();
+        add_tmem(at + KV_O + part * 32, dv, 1.0f);
+        add_tmem(at + KV_O + 64 + part * 32, dk, 1.0f);
+      }
+      store_planes(at + part * 16, s1);
+      store_planes(at + MAP + part * 16, s2);
+      store_planes(at + 2 * MAP + part * 16, dp);
+      tmem_wait_st();
+      tc_fence_before();
+      signal(&sh.p_full);
+    }
+    if (ok && nt > 0 && (ok = blk.done(&sh.o_full, (nt - 1) & 1))) {
+      tc_fence_after();
+      add_tmem(at + KV_O + part * 32, dv, 1.0f);
+      add_tmem(at + KV_O + 64 + part * 32, dk, 1.0f);
+    }
+    if (ok && work) {
+      float* patch = reinterpret_cast<float*>(base) + warp * 1024;
+      store_rows(patch, dv, 2 * a.dh - part * 32, p.st16,
+                 key < a.tk ? static_cast<float*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr + part * 32 : nullptr);
+#pragma unroll
+      for (int c = 0; c < 32; c++) dk[c] *= a.scale;
+      store_rows(patch, dk, a.dh, p.st16,
+                 key < a.tk ? static_cast<float*>(a.dk) + b * a.dkb + kvh * a.dkh + key * a.dkr + part * a.dh : nullptr);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < WARP_MMA) {
+      const int t0 = tid - MATH_WARPS * 32;
+      const float* qp = static_cast<const float*>(a.q) + b * a.qb + static_cast<long long>(kvh) * a.grp * a.qh;
+      const float* gp = static_cast<const float*>(a.dout) + b * a.gb + static_cast<long long>(kvh) * a.grp * a.gh;
+      for (int t = 0; t < nt; t++) {
+        const int st = t % BWD_STAGES, e = t / per, i0 = qbeg + (t - e * per) * COLS;
+        if (t >= BWD_STAGES && !blk.done(&sh.empty[st], (t / BWD_STAGES - 1) & 1)) break;
+        load_step(stages + st * (2 * COL_TILE), a, t0,
+                  [&](int r) { return i0 + r < a.tq ? qp + e * a.qh + (i0 + r) * a.qr : nullptr; },
+                  [&](int r) { return i0 + r < a.tq ? gp + e * a.gh + (i0 + r) * a.gr : nullptr; });
+        if (t0 < COLS) {
+          const int i = i0 + t0;
+          const bool in = i < a.tq;
+          const long long from = (static_cast<long long>(b) * a.h + kvh * a.grp + e) * 2 * a.tq + i;
+          const int lim = in ? row_limit(a, i, len) : 0;
+          sh.stat[st][0][t0] = in ? a.flse[from] : CUDART_INF_F;
+          sh.stat[st][1][t0] = in ? a.flse[from + a.tq] : CUDART_INF_F;
+          sh.stat[st][2][t0] = in ? a.dsum[from] : 0.0f;
+          sh.stat[st][3][t0] = in ? a.dsum[from + a.tq] : 0.0f;
+          sh.stat[st][4][t0] = __int_as_float(lim);
+          const int least = __reduce_min_sync(0xffffffffu, lim);
+          if ((t0 & 31) == 0) sh.least[st][t0 >> 5] = least;
+        }
+        fence_async_smem();
+        signal(&sh.full[st]);
+      }
+      // dlam: block `head` sums that head's rows in a fixed order
+      if (warp == MATH_WARPS && static_cast<int>(blockIdx.x) < a.h && a.tq > 0) {
+        const long long cnt = static_cast<long long>(a.n) * a.tq;
+        const float* x = a.dlrow + blockIdx.x * cnt;
+        double sum = 0.0;
+#pragma unroll 8
+        for (long long i = lane; i < cnt; i += 32) sum += x[i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) a.dlam[blockIdx.x] -= static_cast<float>(sum);
+      }
+    } else if (nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_v = idesc_bf16(ROWS, 64, true);
+      const uint32_t id_k = idesc_bf16(ROWS, 32, true);
+      const uint64_t dk = desc_k(smem_u32(base)), dv = desc_k(smem_u32(base) + ROW_TILE);
+      const uint64_t dq = desc_k(smem_u32(stages)), dg = desc_k(smem_u32(stages) + COL_TILE);
+      const uint64_t dqn = desc_mn(smem_u32(stages), 0), dgn = desc_mn(smem_u32(stages) + COL_TILE, 0);
+      const int ksteps = (a.dh + 15) / 16, vsteps = (2 * a.dh + 15) / 16;
+      bool ok = blk.done(&sh.rows_full, 0);
+      for (int t = 0; ok && t < nt; t++) {
+        const int st = t % BWD_STAGES;
+        // the products of the step before have read the planes in the scores' place
+        if (!(ok = blk.done(&sh.full[st], (t / BWD_STAGES) & 1) && (t == 0 || blk.done(&sh.o_full, (t - 1) & 1)))) break;
+        tc_fence_after();
+        const uint32_t off = st * (2 * COL_TILE / 16);
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+          products<2>(ksteps, [&](int pa, int pb, int ks, bool acc) {
+            mma_ss(tmem + m * MAP, dk + (pa * ROW_PLANE + m * 64 + ks * 32) / 16,
+                   dq + off + (pb * COL_PLANE + m * 64 + ks * 32) / 16, id_s, acc, lead);
+          });
+        products<4>(vsteps, [&](int pa, int pb, int ks, bool acc) {
+          mma_ss(tmem + 2 * MAP, dv + (pa * ROW_PLANE + ks * 32) / 16, dg + off + (pb * COL_PLANE + ks * 32) / 16, id_s,
+                 acc, lead);
+        });
+        commit(&sh.s_full, lead);
+        if (!(ok = blk.done(&sh.p_full, t & 1))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+          products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+            mma_ts(tmem + KV_O + 64 + m * 32, tmem + m * MAP + pa * 32 + ks * 8,
+                   dqn + off + (pb * COL_PLANE + m * 64 + ks * 2048) / 16, id_k, acc, lead);
+          });
+        products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+          mma_ts(tmem + KV_O, tmem + 2 * MAP + pa * 32 + ks * 8, dgn + off + (pb * COL_PLANE + ks * 2048) / 16, id_v, acc,
+                 lead);
+        });
+        commit(&sh.empty[st], lead);
+        commit(&sh.o_full, lead);
+      }
+      if (!ok) {
+        commit(&sh.drain, lead);
+        settle(&sh.drain, 0);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+}
+
 }  // namespace
 
 bool f32_tc_ok(const Args& a) { return a.dh <= 32 && static_cast<long long>(a.grp) * a.tq >= 64 && a.tk >= 32; }
@@ -514,6 +958,33 @@ int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
   f32_fwd_kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), THREADS, FWD_SMEM, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
   return p.a.nsplit > 1 ? join_parts_f32(ctx, p.a) : RNN_OK;
+}
+
+int f32_tc_bwd(rnn_ctx* ctx, const Args& a) {
+  Params p;
+  p.a = a;
+  p.dev_error = ctx->dev_error;
+  auto a16 = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  auto m4 = [](std::initializer_list<long long> s) {
+    for (long long x : s)
+      if (x % 4) return false;
+    return true;
+  };
+  p.st16 = a.dh % 4 == 0 && a16(a.dq) && a16(a.dk) && a16(a.dv) &&
+           m4({a.dqb, a.dqr, a.dqh, a.dkb, a.dkr, a.dkh, a.dvb, a.dvr, a.dvh});
+  p.ld16 = a.vec && a16(a.fo) && a16(a.fo2) && m4({a.ob, a.orow, a.oh});
+  const long long rows = static_cast<long long>(a.grp) * a.tq, nbh = static_cast<long long>(a.n) * a.hkv;
+  const long long qblocks = (rows + ROWS - 1) / ROWS * nbh;
+  const long long kblocks = std::max<long long>((a.tk + ROWS - 1ll) / ROWS * nbh, a.h);
+  RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  static std::atomic<unsigned long long> optin_q{0}, optin_k{0};
+  RNN_TRY(tc::ensure_smem_optin(f32_bwd_q_kernel, optin_q, ctx->device, static_cast<int>(BWD_SMEM)));
+  RNN_TRY(tc::ensure_smem_optin(f32_bwd_kv_kernel, optin_k, ctx->device, static_cast<int>(BWD_SMEM)));
+  f32_bwd_q_kernel<<<static_cast<unsigned>(qblocks), THREADS, BWD_SMEM, ctx->stream>>>(p);
+  RNN_CHECK_LAUNCH();
+  f32_bwd_kv_kernel<<<static_cast<unsigned>(kblocks), THREADS, BWD_SMEM, ctx->stream>>>(p);
+  RNN_CHECK_LAUNCH();
+  return RNN_OK;
 }
 
 }  // namespace diff
