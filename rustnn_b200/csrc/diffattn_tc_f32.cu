@@ -15,6 +15,7 @@
 // warps, two threads a row with 32 columns each, 7 loading warps and one that
 // issues MMAs.
 #include <algorithm>
+#include <type_traits>
 
 #include "diffattn_tc.cuh"
 
@@ -30,21 +31,25 @@ constexpr uint32_t ROW_TILE = 3 * ROW_PLANE, COL_TILE = 3 * COL_PLANE;
 constexpr int FWD_STAGES = 3, BWD_STAGES = 2;
 
 // Tensor memory columns.  Forward: S_1 S_2 | planes of P_1, P_2 | P_1 v, P_2 v.
-// Queries' backward: S_1 S_2 dP | planes of dS_1, dS_2 | dq.  Keys' backward: the
-// planes of dS_1, dS_2 and P_1 - lam P_2 overwrite S_1, S_2 and dP, each of
-// which has room for three planes | dv, dk.
-constexpr uint32_t MAP = 96;  // three planes of 64 bf16 columns
+// Queries' backward: S_1 S_2 dP | planes of dS_1, dS_2 | dq.  Keys' backward:
+// four places for three planes each, of which the first three take S_1, S_2 and
+// dP first, from column 16 on, so that a thread's planes overwrite its own
+// scores alone: P_1 - lam P_2 takes S_2's place, dS_1 dP's, dS_2 the fourth |
+// dv, dk.
+constexpr uint32_t MAP = 96, PART = 48;  // three planes of 64 bf16 values; of a thread's 32
+// where the 16 values of step ks of a plane start
+__device__ __forceinline__ uint32_t plane_at(int plane, int ks) { return PART * (ks >> 1) + 16 * plane + 8 * (ks & 1); }
 constexpr uint32_t FWD_P = 128, FWD_O = FWD_P + 2 * MAP;
 constexpr uint32_t Q_P = 192, Q_O = Q_P + 2 * MAP;
-constexpr uint32_t KV_O = 3 * MAP;
+constexpr uint32_t KV_O = 4 * MAP, KV_S = 16;
 
 struct Shared {
-  uint64_t rows_full, full[FWD_STAGES], empty[FWD_STAGES], s_full, s_free, p_full, o_full, pair[4], drain;
+  uint64_t rows_full, d_full, full[FWD_STAGES], empty[FWD_STAGES], s_full, s_free, dp_full, p_full, ds_full, o_full, pair[4], drain;
   uint32_t tmem;
   int abort_flag;
-  float2 give[2][2][ROWS];
+  float2 give[2][2][ROWS], d[ROWS];
   uint32_t seen[FWD_STAGES][2];  // keys of a tile that exist and are not masked
-  alignas(16) float stat[BWD_STAGES][5][COLS];  // lse_1, lse_2, D_1, D_2, limit of a tile's queries
+  alignas(16) float stat[BWD_STAGES][5][COLS];  // -lse_1, -lse_2, -D_1, -D_2, limit of a tile's queries
   int least[BWD_STAGES][2];                     // least limit of 32 of them
 };
 constexpr size_t FWD_SMEM = 1024 + ROW_TILE + FWD_STAGES * 2 * COL_TILE + sizeof(Shared);
@@ -71,27 +76,21 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& 
 }
 
 // Eight columns (chunk c) of a row of 2*dh values, zeros beyond; p is the row or
-// null.  SPLIT rows (q, k) put the halves at columns 0 and 32.
-template <bool SPLIT>
-__device__ __forceinline__ void load8(float (&x)[8], const float* p, int c, const Args& a) {
-#pragma unroll
-  for (int k = 0; k < 8; k++) x[k] = 0.0f;
-  if (p == nullptr) return;
-  const int w = SPLIT ? (c & 3) * 8 : c * 8, in = (SPLIT ? a.dh : 2 * a.dh) - w;
-  p += w + (SPLIT ? (c >> 2) * a.dh : 0);
-  if (a.vec) {  // dh is a multiple of 4
-    if (in >= 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    }
-    if (in >= 8) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-    }
+// null.  SPLIT rows (q, k) put the halves at columns 0 and 32.  VEC: 16-byte
+// loads are aligned and dh is a multiple of 4.
+template <bool SPLIT, bool VEC>
+__device__ __forceinline__ void load8(float (&x)[8], const float* p, int c, int dh) {
+  const int w = SPLIT ? (c & 3) * 8 : c * 8, in = p == nullptr ? 0 : (SPLIT ? dh : 2 * dh) - w;
+  p += w + (SPLIT ? (c >> 2) * dh : 0);
+  if (VEC) {
+    float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
+    if (in >= 4) u = __ldg(reinterpret_cast<const float4*>(p));
+    if (in >= 8) v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+    x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; k++)
-      if (k < in) x[k] = __ldg(p + k);
+    for (int k = 0; k < 8; k++) x[k] = k < in ? __ldg(p + k) : 0.0f;
   }
 }
 // Their planes, as chunk c of row r of a tile of R rows.
@@ -106,43 +105,91 @@ __device__ __forceinline__ void store8(uint8_t* dst, const float (&x)[8], int r,
         make_uint4(z[q][0], z[q][1], z[q][2], z[q][3]);
 }
 // The block's own 128 rows, by the arithmetic warps (thread t of 256), which
-// have nothing else to do then.
-template <bool SPLIT, class Row>
-__device__ __forceinline__ void load_rows(uint8_t* dst, const Args& a, int t, float scale, Row row) {
-  constexpr int N = ROWS * 8 / (MATH_WARPS * 32);
-  float x[N][8];
+// have nothing else to do then: a thread takes chunk t % 8 of four rows.
+constexpr int OWN = ROWS * 8 / (MATH_WARPS * 32);
+__device__ __forceinline__ int own_row(int t, int u) { return (t >> 3) + u * (ROWS / OWN); }
+
+// Rows of two tensors, the first scaled; x(u) and y(u) give the places of the
+// thread's row u.  Aligned loads are all in flight at once; the others take one
+// row after the other, which keeps the code that runs once per block short.
+template <bool TWO, class X, class Y>
+__device__ __forceinline__ void load_own(uint8_t* dst, const Args& a, int t, float scale, X x, Y y) {
+  auto put = [&](float (&v)[8], uint8_t* to, int u, float f) {
 #pragma unroll
-  for (int u = 0; u < N; u++) load8<SPLIT>(x[u], row((t >> 3) + u * (ROWS / N)), t & 7, a);
+    for (int k = 0; k < 8; k++) v[k] *= f;
+    store8<ROWS>(to, v, own_row(t, u), t & 7);
+  };
+  if (a.vec) {
+    float v[OWN][8], w[OWN][8];
 #pragma unroll
-  for (int u = 0; u < N; u++) {
+    for (int u = 0; u < OWN; u++) load8<true, true>(v[u], x(u), t & 7, a.dh);
 #pragma unroll
-    for (int k = 0; k < 8; k++) x[u][k] *= scale;
-    store8<ROWS>(dst, x[u], (t >> 3) + u * (ROWS / N), t & 7);
-  }
-}
-// Two tiles of a step (k and v, or q and dout), by the loading warps, all loads
-// in flight at once.
-template <class First, class Second>
-__device__ __forceinline__ void load_step(uint8_t* dst, const Args& a, int t, First first, Second second) {
-  constexpr int ITEMS = COLS * 8, N = (2 * ITEMS + LOADERS - 1) / LOADERS;
-  float x[N][8];
+    for (int u = 0; TWO && u < OWN; u++) load8<false, true>(w[u], y(u), t & 7, a.dh);
 #pragma unroll
-  for (int u = 0; u < N; u++) {
-    const int i = t + u * LOADERS, r = (i & (ITEMS - 1)) >> 3;
-    if (i < ITEMS) {
-      load8<true>(x[u], first(r), i & 7, a);
-    } else if (i < 2 * ITEMS) {
-      load8<false>(x[u], second(r), i & 7, a);
+    for (int u = 0; u < OWN; u++) put(v[u], dst, u, scale);
+#pragma unroll
+    for (int u = 0; TWO && u < OWN; u++) put(w[u], dst + ROW_TILE, u, 1.0f);
+  } else {
+#pragma unroll 1
+    for (int u = 0; u < OWN; u++) {
+      float v[8];
+      load8<true, false>(v, x(u), t & 7, a.dh);
+      put(v, dst, u, scale);
+      if (TWO) {
+        load8<false, false>(v, y(u), t & 7, a.dh);
+        put(v, dst + ROW_TILE, u, 1.0f);
+      }
     }
   }
-#pragma unroll
-  for (int u = 0; u < N; u++) {
-    const int i = t + u * LOADERS, r = (i & (ITEMS - 1)) >> 3;
-    if (i < 2 * ITEMS) store8<COLS>(dst + (i < ITEMS ? 0 : COL_TILE), x[u], r, i & 7);
-  }
+}
+// A packed row's place, or null: head e of the group and query i, from `base` on.
+__device__ __forceinline__ const float* packed(const float* base, const Args& a, int r, int rows, long long sr,
+                                               long long sh) {
+  const int e = r / a.tq;
+  return r < rows ? base + e * sh + (r - e * a.tq) * sr : nullptr;
 }
 
-// The planes of 32 values of a row: 16 columns of each plane of the map at `dst`.
+// Two tiles of a step (k and v, or q and dout), by the loading warps.  ready()
+// waits until their place is free, false if it never is; aligned loads go before
+// it, so that only the stores follow.
+template <class First, class Second, class Ready>
+__device__ __forceinline__ bool load_step(uint8_t* dst, const Args& a, int t, First first, Second second, Ready ready) {
+  constexpr int ITEMS = COLS * 8, N = (2 * ITEMS + LOADERS - 1) / LOADERS;
+  if (a.vec) {
+    float x[N][8];
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      const int i = t + u * LOADERS, r = (i & (ITEMS - 1)) >> 3;
+      if (i < ITEMS) {
+        load8<true, true>(x[u], first(r), i & 7, a.dh);
+      } else if (i < 2 * ITEMS) {
+        load8<false, true>(x[u], second(r), i & 7, a.dh);
+      }
+    }
+    if (!ready()) return false;
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      const int i = t + u * LOADERS, r = (i & (ITEMS - 1)) >> 3;
+      if (i < 2 * ITEMS) store8<COLS>(dst + (i < ITEMS ? 0 : COL_TILE), x[u], r, i & 7);
+    }
+  } else {
+    if (!ready()) return false;
+#pragma unroll 1
+    for (int i = t; i < 2 * ITEMS; i += LOADERS) {
+      const int r = (i & (ITEMS - 1)) >> 3;
+      float x[8];
+      if (i < ITEMS) {
+        load8<true, false>(x, first(r), i & 7, a.dh);
+      } else {
+        load8<false, false>(x, second(r), i & 7, a.dh);
+      }
+      store8<COLS>(dst + (i < ITEMS ? 0 : COL_TILE), x, r, i & 7);
+    }
+  }
+  return true;
+}
+
+// The planes of a thread's 32 values of a map: its 48 columns of the map's 96.
 __device__ __forceinline__ void store_planes(uint32_t dst, const float (&s)[32]) {
 #pragma unroll
   for (int g = 0; g < 2; g++) {
@@ -150,7 +197,7 @@ __device__ __forceinline__ void store_planes(uint32_t dst, const float (&s)[32])
 #pragma unroll
     for (int k = 0; k < 8; k++) split3(s[g * 16 + 2 * k], s[g * 16 + 2 * k + 1], z[0][k], z[1][k], z[2][k]);
 #pragma unroll
-    for (int q = 0; q < 3; q++) tmem_st(dst + q * 32 + g * 8, z[q]);
+    for (int q = 0; q < 3; q++) tmem_st(dst + q * 16 + g * 8, z[q]);
   }
 }
 
@@ -213,20 +260,27 @@ __device__ __forceinline__ void store_rows(float* patch, const float (&x)[32], i
     *reinterpret_cast<float4*>(patch + lane * 32 + ((k ^ (lane & 7)) << 2)) =
         make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
   __syncwarp();
+  float* p[8];
+  float4 v[8];
 #pragma unroll
   for (int k = 0; k < 8; k++) {
     const int r = k * 4 + (lane >> 3);
-    float* p = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), r));
-    if (p == nullptr) continue;
-    const float4 v = *reinterpret_cast<const float4*>(patch + r * 32 + ((c ^ (r & 7)) << 2));
-    p += c * 4;
-    if (st16 && c * 4 + 4 <= in) {
-      *reinterpret_cast<float4*>(p) = v;
-    } else {
-      const float z[4] = {v.x, v.y, v.z, v.w};
+    p[k] = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), r));
+    v[k] = *reinterpret_cast<const float4*>(patch + r * 32 + ((c ^ (r & 7)) << 2));
+  }
+  in -= c * 4;
+  if (st16) {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (p[k] != nullptr && in >= 4) *reinterpret_cast<float4*>(p[k] + c * 4) = v[k];
+  }
+  if (!st16 || (in > 0 && in < 4)) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float z[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        if (c * 4 + e < in) p[e] = z[e];
+        if (p[k] != nullptr && e < in) p[k][c * 4 + e] = z[e];
     }
   }
   __syncwarp();
@@ -253,13 +307,16 @@ struct Block {
 __device__ __forceinline__ void setup(Shared& sh, int warp) {
   if (threadIdx.x == 0) {
     mbar_init(&sh.rows_full, MATH_WARPS);
+    mbar_init(&sh.d_full, MATH_WARPS);
     for (int i = 0; i < FWD_STAGES; i++) {
       mbar_init(&sh.full[i], LOAD_WARPS);
       mbar_init(&sh.empty[i], 1);
     }
     mbar_init(&sh.s_full, 1);
     mbar_init(&sh.s_free, MATH_WARPS);
+    mbar_init(&sh.dp_full, 1);
     mbar_init(&sh.p_full, MATH_WARPS);
+    mbar_init(&sh.ds_full, MATH_WARPS);
     mbar_init(&sh.o_full, 1);
     for (int i = 0; i < 4; i++) mbar_init(&sh.pair[i], 2);
     mbar_init(&sh.drain, 1);
@@ -279,14 +336,6 @@ __device__ __forceinline__ void signal(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// Packed rows of a (sequence, key head): head and query of a row.
-__device__ __forceinline__ const float* packed(const void* base, const Args& a, int p, int rows, long long sb,
-                                               long long sr, long long sh, int b, int kvh) {
-  if (p >= rows) return nullptr;
-  const int e = p / a.tq;
-  return static_cast<const float*>(base) + b * sb + (static_cast<long long>(kvh) * a.grp + e) * sh + (p - e * a.tq) * sr;
-}
-
 // Loads tiles of keys [kbeg, kend) for the kernels that own query rows.
 __device__ __forceinline__ void load_keys(Block& blk, uint8_t* stages, int nstage, const Args& a, int b, int kvh,
                                           int kbeg, int kend, int nt, int t0) {
@@ -295,12 +344,13 @@ __device__ __forceinline__ void load_keys(Block& blk, uint8_t* stages, int nstag
   const uint8_t* mask = a.kmask ? a.kmask + b * a.kmb : nullptr;
   for (int t = 0; t < nt; t++) {
     const int st = t % nstage, j0 = kbeg + t * COLS;
-    if (t >= nstage && !blk.done(&blk.sh.empty[st], (t / nstage - 1) & 1)) break;
     auto on = [&](int r) { return j0 + r < kend && (!mask || mask[j0 + r]); };
-    load_step(stages + st * (2 * COL_TILE), a, t0, [&](int r) { return on(r) ? kp + (j0 + r) * a.kr : nullptr; },
-              [&](int r) { return on(r) ? vp + (j0 + r) * a.vr : nullptr; });
-    if (t0 < 64) {
-      const uint32_t bits = __ballot_sync(0xffffffffu, on(t0));
+    const uint32_t bits = __ballot_sync(0xffffffffu, t0 < COLS && on(t0));
+    if (!load_step(stages + st * (2 * COL_TILE), a, t0, [&](int r) { return on(r) ? kp + (j0 + r) * a.kr : nullptr; },
+                   [&](int r) { return on(r) ? vp + (j0 + r) * a.vr : nullptr; },
+                   [&] { return t < nstage || blk.done(&blk.sh.empty[st], (t / nstage - 1) & 1); }))
+      break;
+    if (t0 < COLS) {
       if ((t0 & 31) == 0) blk.sh.seen[st][t0 >> 5] = bits;
     }
     fence_async_smem();
@@ -333,8 +383,9 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
     // registers: 512 threads x 128 at launch = 256 x 168 + 256 x 88
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     if (nt > 0) {
-      // q in units that make scores exponents of 2
-      load_rows<true>(base, a, tid, a.slog2, [&](int r) { return packed(a.q, a, row0 + r, rows, a.qb, a.qr, a.qh, b, kvh); });
+      const float* q = static_cast<const float*>(a.q) + b * a.qb + static_cast<long long>(kvh) * a.grp * a.qh;
+      auto at_q = [&](int u) { return packed(q, a, row0 + own_row(tid, u), rows, a.qr, a.qh); };
+      load_own<false>(base, a, tid, a.slog2, at_q, at_q);  // in units that make scores exponents of 2
       fence_async_smem();
       signal(&sh.rows_full);
     }
@@ -387,8 +438,8 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
       }
       al1 = f1;
       al2 = f2;
-      store_planes(at + FWD_P + part * 16, s1);
-      store_planes(at + FWD_P + MAP + part * 16, s2);
+      store_planes(at + FWD_P + part * PART, s1);
+      store_planes(at + FWD_P + MAP + part * PART, s2);
       tmem_wait_st();
       tc_fence_before();
       signal(&sh.p_full);
@@ -467,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
 #pragma unroll
           for (int m = 0; m < 2; m++)
             products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
-              mma_ts(tmem + FWD_O + m * 64, tmem + FWD_P + m * MAP + pa * 32 + ks * 8,
+              mma_ts(tmem + FWD_O + m * 64, tmem + FWD_P + m * MAP + plane_at(pa, ks),
                      v + (pb * COL_PLANE + ks * 2048) / 16, id_o, acc, lead);
             });
           commit(&sh.empty[st], lead);
@@ -539,12 +590,46 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_q_kernel(const __grid_cons
   if (warp < MATH_WARPS) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     if (nt > 0) {
-      load_rows<true>(base, a, tid, a.slog2,
-                      [&](int r) { return packed(a.q, a, row0 + r, rows, a.qb, a.qr, a.qh, b, kvh); });
-      load_rows<false>(base + ROW_TILE, a, tid, 1.0f,
-                       [&](int r) { return packed(a.dout, a, row0 + r, rows, a.gb, a.gr, a.gh, b, kvh); });
+      const long long h0 = static_cast<long long>(kvh) * a.grp;
+      const float* q = static_cast<const float*>(a.q) + b * a.qb + h0 * a.qh;
+      const float* g = static_cast<const float*>(a.dout) + b * a.gb + h0 * a.gh;
+      load_own<true>(base, a, tid, a.slog2, [&](int u) { return packed(q, a, row0 + own_row(tid, u), rows, a.qr, a.qh); },
+                     [&](int u) { return packed(g, a, row0 + own_row(tid, u), rows, a.gr, a.gh); });
       fence_async_smem();
       signal(&sh.rows_full);
+      // D_1 = do . (o + lam o2) and D_2 = do . o2; rows that see one tile of keys
+      // sum P dP instead (dS of a lone key comes out as 0).
+      if (nt > 1) {
+        const float* o = static_cast<const float*>(a.fo) + b * a.ob + h0 * a.oh;
+        const float* o2 = static_cast<const float*>(a.fo2) + (static_cast<long long>(b) * a.tq * a.h + h0) * (2 * a.dh);
+        auto load = [&](float (&x)[8], const float* q, auto vec) { load8<false, decltype(vec)::value>(x, q, tid & 7, a.dh); };
+        auto sums = [&](int u, auto vec) {
+          const int r = row0 + own_row(tid, u), e = r < rows ? r / a.tq : -1, i = r - e * a.tq;
+          float x[8], y[8], z[8], d = 0.0f, d2 = 0.0f;
+          load(x, e < 0 ? nullptr : g + e * a.gh + i * a.gr, vec);
+          load(y, e < 0 ? nullptr : o + e * a.oh + i * a.orow, vec);
+          load(z, e < 0 ? nullptr : o2 + (static_cast<long long>(i) * a.h + e) * (2 * a.dh), vec);
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            d += x[k] * y[k];
+            d2 += x[k] * z[k];
+          }
+#pragma unroll
+          for (int k = 1; k < 8; k <<= 1) {
+            d += __shfl_xor_sync(0xffffffffu, d, k);
+            d2 += __shfl_xor_sync(0xffffffffu, d2, k);
+          }
+          if ((tid & 7) == 0 && e >= 0) sh.d[r - row0] = make_float2(d + __ldg(a.lam + kvh * a.grp + e) * d2, d2);
+        };
+        if (p.ld16) {
+#pragma unroll
+          for (int u = 0; u < OWN; u++) sums(u, std::true_type());
+        } else {
+#pragma unroll 1
+          for (int u = 0; u < OWN; u++) sums(u, std::false_type());
+        }
+        signal(&sh.d_full);
+      }
     }
     const int part = warp >> 2, w = warp & 3, row = w * 32 + lane, r = row0 + row;
     const uint32_t at = tmem + (static_cast<uint32_t>(w * 32) << 16);
@@ -559,38 +644,11 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_q_kernel(const __grid_cons
       ls1 = s[0];
       ls2 = s[a.tq];
     }
-    // D_1 = do . (o + lam o2) and D_2 = do . o2; rows that see one tile of keys
-    // sum P dP there instead (dS of a lone key comes out as 0).
     if (nt > 1) {
-      if (r < rows) {
-        const float* g = packed(a.dout, a, r, rows, a.gb, a.gr, a.gh, b, kvh) + part * 32;
-        const float* o = static_cast<const float*>(a.fo) + b * a.ob + head * a.oh + i * a.orow + part * 32;
-        const float* o2 = static_cast<const float*>(a.fo2) +
-                          ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + part * 32;
-        const int in = min(2 * a.dh - part * 32, 32);
-        if (p.ld16) {
-#pragma unroll
-          for (int c = 0; c < 32; c += 4)
-            if (c < in) {
-              const float4 x = __ldg(reinterpret_cast<const float4*>(g + c));
-              const float4 y = __ldg(reinterpret_cast<const float4*>(o + c));
-              const float4 z = __ldg(reinterpret_cast<const float4*>(o2 + c));
-              d1 += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
-              d2 += x.x * z.x + x.y * z.y + x.z * z.z + x.w * z.w;
-            }
-        } else {
-          for (int c = 0; c < in; c++) {
-            d1 += g[c] * o[c];
-            d2 += g[c] * o2[c];
-          }
-        }
-        d1 += __ldg(a.lam + head) * d2;
-      }
-      float2 other;
-      ok = blk.exchange(turn, w, part, row, make_float2(d1, d2), other);
-      if (ok) {
-        d1 += other.x;
-        d2 += other.y;
+      ok = blk.done(&sh.d_full, 0);
+      if (ok && r < rows) {
+        d1 = sh.d[row].x;
+        d2 = sh.d[row].y;
       }
     }
     float dq[32];
@@ -634,8 +692,8 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_q_kernel(const __grid_cons
         tc_fence_after();
         add_tmem(at + Q_O + part * 32, dq, 1.0f);
       }
-      store_planes(at + Q_P + part * 16, s1);
-      store_planes(at + Q_P + MAP + part * 16, s2);
+      store_planes(at + Q_P + part * PART, s1);
+      store_planes(at + Q_P + MAP + part * PART, s2);
       tmem_wait_st();
       tc_fence_before();
       signal(&sh.p_full);
@@ -698,7 +756,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_q_kernel(const __grid_cons
 #pragma unroll
           for (int m = 0; m < 2; m++)
             products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
-              mma_ts(tmem + Q_O + m * 32, tmem + Q_P + m * MAP + pa * 32 + ks * 8,
+              mma_ts(tmem + Q_O + m * 32, tmem + Q_P + m * MAP + plane_at(pa, ks),
                      k + (pb * COL_PLANE + m * 64 + ks * 2048) / 16, id_o, acc, lead);
             });
           commit(&sh.empty[st], lead);
@@ -754,8 +812,8 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
         const int j = key0 + r;
         return j < len && (!mask || mask[j]) ? static_cast<const float*>(q) + b * sb + kvh * sh_ + j * sr : nullptr;
       };
-      load_rows<true>(base, a, tid, a.slog2, [&](int r) { return row(a.k, a.kb, a.kr, a.kh, r); });
-      load_rows<false>(base + ROW_TILE, a, tid, 1.0f, [&](int r) { return row(a.v, a.vb, a.vr, a.vh, r); });
+      load_own<true>(base, a, tid, a.slog2, [&](int u) { return row(a.k, a.kb, a.kr, a.kh, own_row(tid, u)); },
+                     [&](int u) { return row(a.v, a.vb, a.vr, a.vh, own_row(tid, u)); });
       fence_async_smem();
       signal(&sh.rows_full);
     }
@@ -767,47 +825,35 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
     float dv[32], dk[32];
 #pragma unroll
     for (int c = 0; c < 32; c++) dv[c] = dk[c] = 0.0f;
-    int turn = 0;
     bool ok = true;
     for (int t = 0; t < nt; t++) {
       const int st = t % BWD_STAGES;
       if (!(ok = blk.done(&sh.full[st], (t / BWD_STAGES) & 1) && blk.done(&sh.s_full, t & 1))) break;
       tc_fence_after();
-      float s1[32], s2[32], dp[32];
-      tmem_ld(at + part * 32, s1);
-      tmem_ld(at + MAP + part * 32, s2);
-      tmem_ld(at + 2 * MAP + part * 32, dp);
+      float s1[32], s2[32];
+      tmem_ld(at + KV_S + part * 32, s1);
+      tmem_ld(at + MAP + KV_S + part * 32, s2);
       tmem_landed(s1);
       tmem_landed(s2);
-      tmem_landed(dp);
-      tc_fence_before();
-      // the planes overwrite what both threads of a row have now read
-      float2 other;
-      if (!(ok = blk.exchange(turn, w, part, row, make_float2(0.0f, 0.0f), other))) break;
-      tc_fence_after();
       const float* stat = &sh.stat[st][0][part * 32];
       const float lam = __ldg(a.lam + kvh * a.grp + t / per);
+      const f32x2 ll = pair(-lam, -lam);  // s2 is -lam P_2
       if (most >= sh.least[st][part]) {
 #pragma unroll
         for (int c = 0; c < 32; c++)
           if (need >= __float_as_int(stat[4 * COLS + c])) s1[c] = s2[c] = -CUDART_INF_F;
       }
-      // after this: s1 = dS_1, s2 = dS_2, dp = P_1 - lam P_2
+      float z[32];  // P_1 - lam P_2
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 ls1 = *reinterpret_cast<const float4*>(stat + c);
-        const float4 ls2 = *reinterpret_cast<const float4*>(stat + COLS + c);
-        const float4 d1 = *reinterpret_cast<const float4*>(stat + 2 * COLS + c);
-        const float4 d2 = *reinterpret_cast<const float4*>(stat + 3 * COLS + c);
-        const float l1[4] = {ls1.x, ls1.y, ls1.z, ls1.w}, l2[4] = {ls2.x, ls2.y, ls2.z, ls2.w};
-        const float e1[4] = {d1.x, d1.y, d1.z, d1.w}, e2[4] = {d2.x, d2.y, d2.z, d2.w};
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float x = ex2(s1[c + k] - l1[k]), y = lam * ex2(s2[c + k] - l2[k]);
-          s1[c + k] = x * (dp[c + k] - e1[k]);
-          s2[c + k] = y * (e2[k] - dp[c + k]);
-          dp[c + k] = x - y;
-        }
+      for (int c = 0; c < 32; c += 2) {
+        const f32x2 l1 = *reinterpret_cast<const f32x2*>(stat + c), l2 = *reinterpret_cast<const f32x2*>(stat + COLS + c);
+        float x, y, u, v;
+        unpair(add2(pair(s1[c], s1[c + 1]), l1), x, y);
+        unpair(add2(pair(s2[c], s2[c + 1]), l2), u, v);
+        const f32x2 p1 = pair(ex2(x), ex2(y)), p2 = mul2(pair(ex2(u), ex2(v)), ll);
+        unpair(p1, s1[c], s1[c + 1]);
+        unpair(p2, s2[c], s2[c + 1]);
+        unpair(add2(p1, p2), z[c], z[c + 1]);
       }
       if (t > 0) {
         if (!(ok = blk.done(&sh.o_full, (t - 1) & 1))) break;
@@ -815,12 +861,28 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
         add_tmem(at + KV_O + part * 32, dv, 1.0f);
         add_tmem(at + KV_O + 64 + part * 32, dk, 1.0f);
       }
-      store_planes(at + part * 16, s1);
-      store_planes(at + MAP + part * 16, s2);
-      store_planes(at + 2 * MAP + part * 16, dp);
+      store_planes(at + MAP + part * PART, z);
       tmem_wait_st();
       tc_fence_before();
       signal(&sh.p_full);
+      if (!(ok = blk.done(&sh.dp_full, t & 1))) break;
+      tc_fence_after();
+      tmem_ld(at + 2 * MAP + KV_S + part * 32, z);
+      tmem_landed(z);
+      // s1 = dS_1, s2 = dS_2
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        const f32x2 d1 = *reinterpret_cast<const f32x2*>(stat + 2 * COLS + c);
+        const f32x2 d2 = *reinterpret_cast<const f32x2*>(stat + 3 * COLS + c);
+        const f32x2 dp = pair(z[c], z[c + 1]);
+        unpair(mul2(pair(s1[c], s1[c + 1]), add2(dp, d1)), s1[c], s1[c + 1]);
+        unpair(mul2(pair(s2[c], s2[c + 1]), add2(dp, d2)), s2[c], s2[c + 1]);
+      }
+      store_planes(at + 2 * MAP + part * PART, s1);
+      store_planes(at + 3 * MAP + part * PART, s2);
+      tmem_wait_st();
+      tc_fence_before();
+      signal(&sh.ds_full);
     }
     if (ok && nt > 0 && (ok = blk.done(&sh.o_full, (nt - 1) & 1))) {
       tc_fence_after();
@@ -844,19 +906,22 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
       const float* gp = static_cast<const float*>(a.dout) + b * a.gb + static_cast<long long>(kvh) * a.grp * a.gh;
       for (int t = 0; t < nt; t++) {
         const int st = t % BWD_STAGES, e = t / per, i0 = qbeg + (t - e * per) * COLS;
-        if (t >= BWD_STAGES && !blk.done(&sh.empty[st], (t / BWD_STAGES - 1) & 1)) break;
-        load_step(stages + st * (2 * COL_TILE), a, t0,
-                  [&](int r) { return i0 + r < a.tq ? qp + e * a.qh + (i0 + r) * a.qr : nullptr; },
-                  [&](int r) { return i0 + r < a.tq ? gp + e * a.gh + (i0 + r) * a.gr : nullptr; });
+        const int i = i0 + t0;
+        const bool in = t0 < COLS && i < a.tq;
+        const long long from = (static_cast<long long>(b) * a.h + kvh * a.grp + e) * 2 * a.tq + i;
+        const float l1 = in ? a.flse[from] : CUDART_INF_F, l2 = in ? a.flse[from + a.tq] : CUDART_INF_F;
+        const float d1 = in ? a.dsum[from] : 0.0f, d2 = in ? a.dsum[from + a.tq] : 0.0f;
+        const int lim = in ? row_limit(a, i, len) : 0;
+        if (!load_step(stages + st * (2 * COL_TILE), a, t0,
+                       [&](int r) { return i0 + r < a.tq ? qp + e * a.qh + (i0 + r) * a.qr : nullptr; },
+                       [&](int r) { return i0 + r < a.tq ? gp + e * a.gh + (i0 + r) * a.gr : nullptr; },
+                       [&] { return t < BWD_STAGES || blk.done(&sh.empty[st], (t / BWD_STAGES - 1) & 1); }))
+          break;
         if (t0 < COLS) {
-          const int i = i0 + t0;
-          const bool in = i < a.tq;
-          const long long from = (static_cast<long long>(b) * a.h + kvh * a.grp + e) * 2 * a.tq + i;
-          const int lim = in ? row_limit(a, i, len) : 0;
-          sh.stat[st][0][t0] = in ? a.flse[from] : CUDART_INF_F;
-          sh.stat[st][1][t0] = in ? a.flse[from + a.tq] : CUDART_INF_F;
-          sh.stat[st][2][t0] = in ? a.dsum[from] : 0.0f;
-          sh.stat[st][3][t0] = in ? a.dsum[from + a.tq] : 0.0f;
+          sh.stat[st][0][t0] = -l1;
+          sh.stat[st][1][t0] = -l2;
+          sh.stat[st][2][t0] = -d1;
+          sh.stat[st][3][t0] = -d2;
           sh.stat[st][4][t0] = __int_as_float(lim);
           const int least = __reduce_min_sync(0xffffffffu, lim);
           if ((t0 & 31) == 0) sh.least[st][t0 >> 5] = least;
@@ -884,36 +949,49 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
       const uint64_t dqn = desc_mn(smem_u32(stages), 0), dgn = desc_mn(smem_u32(stages) + COL_TILE, 0);
       const int ksteps = (a.dh + 15) / 16, vsteps = (2 * a.dh + 15) / 16;
       bool ok = blk.done(&sh.rows_full, 0);
-      for (int t = 0; ok && t < nt; t++) {
+      auto scores = [&](int t) {
         const int st = t % BWD_STAGES;
-        // the products of the step before have read the planes in the scores' place
-        if (!(ok = blk.done(&sh.full[st], (t / BWD_STAGES) & 1) && (t == 0 || blk.done(&sh.o_full, (t - 1) & 1)))) break;
+        if (!blk.done(&sh.full[st], (t / BWD_STAGES) & 1)) return false;
         tc_fence_after();
         const uint32_t off = st * (2 * COL_TILE / 16);
 #pragma unroll
         for (int m = 0; m < 2; m++)
           products<2>(ksteps, [&](int pa, int pb, int ks, bool acc) {
-            mma_ss(tmem + m * MAP, dk + (pa * ROW_PLANE + m * 64 + ks * 32) / 16,
+            mma_ss(tmem + m * MAP + KV_S, dk + (pa * ROW_PLANE + m * 64 + ks * 32) / 16,
                    dq + off + (pb * COL_PLANE + m * 64 + ks * 32) / 16, id_s, acc, lead);
           });
-        products<4>(vsteps, [&](int pa, int pb, int ks, bool acc) {
-          mma_ss(tmem + 2 * MAP, dv + (pa * ROW_PLANE + ks * 32) / 16, dg + off + (pb * COL_PLANE + ks * 32) / 16, id_s,
-                 acc, lead);
-        });
         commit(&sh.s_full, lead);
+        return true;
+      };
+      ok = ok && scores(0);
+      for (int t = 0; ok && t < nt; t++) {
+        const uint32_t off = (t % BWD_STAGES) * (2 * COL_TILE / 16);
+        // dP overwrites dS_1 of the step before
+        if (t > 0 && !(ok = blk.done(&sh.o_full, (t - 1) & 1))) break;
+        tc_fence_after();
+        products<4>(vsteps, [&](int pa, int pb, int ks, bool acc) {
+          mma_ss(tmem + 2 * MAP + KV_S, dv + (pa * ROW_PLANE + ks * 32) / 16, dg + off + (pb * COL_PLANE + ks * 32) / 16,
+                 id_s, acc, lead);
+        });
+        commit(&sh.dp_full, lead);
         if (!(ok = blk.done(&sh.p_full, t & 1))) break;
+        tc_fence_after();
+        products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+          mma_ts(tmem + KV_O, tmem + MAP + plane_at(pa, ks), dgn + off + (pb * COL_PLANE + ks * 2048) / 16, id_v, acc, lead);
+        });
+        // The next scores take the places of the last ones, which are in
+        // registers, and of the planes that dv reads: MMAs of one accumulator
+        // shape (128 x 64) execute in the order of issue.
+        if (t + 1 < nt && !(ok = scores(t + 1))) break;
+        if (!(ok = blk.done(&sh.ds_full, t & 1))) break;
         tc_fence_after();
 #pragma unroll
         for (int m = 0; m < 2; m++)
           products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
-            mma_ts(tmem + KV_O + 64 + m * 32, tmem + m * MAP + pa * 32 + ks * 8,
+            mma_ts(tmem + KV_O + 64 + m * 32, tmem + (2 + m) * MAP + plane_at(pa, ks),
                    dqn + off + (pb * COL_PLANE + m * 64 + ks * 2048) / 16, id_k, acc, lead);
           });
-        products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
-          mma_ts(tmem + KV_O, tmem + 2 * MAP + pa * 32 + ks * 8, dgn + off + (pb * COL_PLANE + ks * 2048) / 16, id_v, acc,
-                 lead);
-        });
-        commit(&sh.empty[st], lead);
+        commit(&sh.empty[t % BWD_STAGES], lead);
         commit(&sh.o_full, lead);
       }
       if (!ok) {
