@@ -459,6 +459,73 @@ int join_launch(rnn_ctx* ctx, const Args& a) {
   return RNN_OK;
 }
 
+// Joins the parts that the keys were split into, a warp for each row: the maps'
+// sums meet at the larger maximum.  (The rows here are many and the parts few;
+// for a token over a long cache, where it is the other way round, the parts are
+// shared out over a block.)
+constexpr int JOIN_WARPS = 8;
+template <class T, int W>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_rows_kernel(const __grid_constant__ Args a) {
+  const long long total = static_cast<long long>(a.n) * a.h * a.tq;
+  const long long idx = static_cast<long long>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (idx >= total) return;
+  float M1 = -CUDART_INF_F, M2 = -CUDART_INF_F;
+  for (int s = 0; s < a.nsplit; s++) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(a.stat) + s * total + idx);
+    M1 = fmaxf(M1, v.x);
+    M2 = fmaxf(M2, v.z);
+  }
+  const float U1 = M1 == -CUDART_INF_F ? 0.0f : M1, U2 = M2 == -CUDART_INF_F ? 0.0f : M2;
+  float L1 = 0.0f, L2 = 0.0f;
+  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+  const bool mine = lane * 4 < 2 * a.dh;
+#pragma unroll 4
+  for (int s = 0; s < a.nsplit; s++) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(a.stat) + s * total + idx);
+    const float4* part = reinterpret_cast<const float4*>(a.part + (s * total + idx) * (2 * W)) + lane;
+    const float w1 = ex2(v.x - U1), w2 = ex2(v.z - U2);
+    L1 += w1 * v.y;
+    L2 += w2 * v.w;
+    if (mine) {
+      const float4 p = part[0], q = part[W / 4];
+      x.x += w1 * p.x, x.y += w1 * p.y, x.z += w1 * p.z, x.w += w1 * p.w;
+      y.x += w2 * q.x, y.y += w2 * q.y, y.z += w2 * q.z, y.w += w2 * q.w;
+    }
+  }
+  const int rows = a.grp * a.tq;
+  const int bh = static_cast<int>(idx / rows), r = static_cast<int>(idx - static_cast<long long>(bh) * rows);
+  const int b = bh / a.hkv, e = r / a.tq, i = r - e * a.tq, head = (bh - b * a.hkv) * a.grp + e;
+  const bool any = L1 > 0.0f && L2 > 0.0f;
+  const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f, f = any ? __ldg(a.lam + head) * i2 : 0.0f;
+  if (mine) {
+    T* o = static_cast<T*>(a.o) + b * a.ob + head * a.oh + i * a.orow + lane * 4;
+    const int in = 2 * a.dh - lane * 4;  // at least 2
+    store2(o, x.x * i1 - f * y.x, x.y * i1 - f * y.y, true, true, a.pair);
+    store2(o + 2, x.z * i1 - f * y.z, x.w * i1 - f * y.w, in > 2, in > 3, a.pair);
+    if (a.o2) {
+      T* o2 = static_cast<T*>(a.o2) + ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + lane * 4;
+      store2(o2, y.x * i2, y.y * i2, true, true, true);
+      store2(o2 + 2, y.z * i2, y.w * i2, in > 2, in > 3, true);
+    }
+  }
+  if (a.lse && lane < 2) {
+    float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
+    if (lane == 0) s[0] = any ? M1 + log2f(L1) : CUDART_INF_F;
+    else s[a.tq] = any ? M2 + log2f(L2) : CUDART_INF_F;
+  }
+}
+
+template <class T, int W>
+int join_rows_launch(rnn_ctx* ctx, const Args& a) {
+  const long long rows = static_cast<long long>(a.n) * a.h * a.tq;
+  RNN_REQUIRE(rows < (1ll << 31), "diffattn: too many rows to join");
+  join_rows_kernel<T, W>
+      <<<static_cast<unsigned>((rows + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, ctx->stream>>>(a);
+  RNN_CHECK_LAUNCH();
+  return RNN_OK;
+}
+
 // ----------------------------------------------------------------- backward
 
 template <class T, int DH>
@@ -1147,7 +1214,8 @@ bool aligned(std::initializer_list<const void*> ps, size_t bytes) {
 }  // namespace
 
 int join_parts(rnn_ctx* ctx, const Args& a) { return join_launch<__nv_bfloat16, 128>(ctx, a); }
-int join_parts_f32(rnn_ctx* ctx, const Args& a) { return join_launch<float, 64>(ctx, a); }
+int join_rows_bf16(rnn_ctx* ctx, const Args& a) { return join_rows_launch<__nv_bfloat16, 128>(ctx, a); }
+int join_rows_f32(rnn_ctx* ctx, const Args& a) { return join_rows_launch<float, 64>(ctx, a); }
 
 }  // namespace diff
 }  // namespace rnn

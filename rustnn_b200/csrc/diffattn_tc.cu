@@ -555,67 +555,6 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
   if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
 }
 
-// Joins the parts that the keys were split into, a warp for each row: the maps'
-// sums meet at the larger maximum.  (The rows here are many and the parts few;
-// for a token over a long cache, where it is the other way round, the parts are
-// shared out over a block.)
-constexpr int JOIN_WARPS = 8;
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_rows_kernel(const __grid_constant__ Args a) {
-  const long long total = static_cast<long long>(a.n) * a.h * a.tq;
-  const long long idx = static_cast<long long>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (idx >= total) return;
-  float M1 = -CUDART_INF_F, M2 = -CUDART_INF_F;
-  for (int s = 0; s < a.nsplit; s++) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(a.stat) + s * total + idx);
-    M1 = fmaxf(M1, v.x);
-    M2 = fmaxf(M2, v.z);
-  }
-  const float U1 = M1 == -CUDART_INF_F ? 0.0f : M1, U2 = M2 == -CUDART_INF_F ? 0.0f : M2;
-  float L1 = 0.0f, L2 = 0.0f;
-  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
-  const bool mine = lane * 4 < 2 * a.dh;
-#pragma unroll 4
-  for (int s = 0; s < a.nsplit; s++) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(a.stat) + s * total + idx);
-    const float4* part = reinterpret_cast<const float4*>(a.part + (s * total + idx) * 256) + lane;
-    const float w1 = ex2(v.x - U1), w2 = ex2(v.z - U2);
-    L1 += w1 * v.y;
-    L2 += w2 * v.w;
-    if (mine) {
-      const float4 p = part[0], q = part[32];
-      x.x += w1 * p.x, x.y += w1 * p.y, x.z += w1 * p.z, x.w += w1 * p.w;
-      y.x += w2 * q.x, y.y += w2 * q.y, y.z += w2 * q.z, y.w += w2 * q.w;
-    }
-  }
-  const int rows = a.grp * a.tq;
-  const int bh = static_cast<int>(idx / rows), r = static_cast<int>(idx - static_cast<long long>(bh) * rows);
-  const int b = bh / a.hkv, e = r / a.tq, i = r - e * a.tq, head = (bh - b * a.hkv) * a.grp + e;
-  const bool any = L1 > 0.0f && L2 > 0.0f;
-  const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f, f = any ? __ldg(a.lam + head) * i2 : 0.0f;
-  if (mine) {
-    const uint32_t lo = pack2(x.x * i1 - f * y.x, x.y * i1 - f * y.y), hi = pack2(x.z * i1 - f * y.z, x.w * i1 - f * y.w);
-    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + b * a.ob + head * a.oh + i * a.orow + lane * 4;
-    if (a.pair) {
-      reinterpret_cast<uint32_t*>(o)[0] = lo;
-      reinterpret_cast<uint32_t*>(o)[1] = hi;
-    } else {
-      const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&lo);
-      const __nv_bfloat162 w = *reinterpret_cast<const __nv_bfloat162*>(&hi);
-      o[0] = z.x, o[1] = z.y, o[2] = w.x, o[3] = w.y;
-    }
-    if (a.o2)
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.o2) +
-                                ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + lane * 4) =
-          make_uint2(pack2(y.x * i2, y.y * i2), pack2(y.z * i2, y.w * i2));
-  }
-  if (a.lse && lane < 2) {
-    float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-    if (lane == 0) s[0] = any ? M1 + log2f(L1) : CUDART_INF_F;
-    else s[a.tq] = any ? M2 + log2f(L2) : CUDART_INF_F;
-  }
-}
-
 }  // namespace
 
 // A block costs about 5 us beside its tiles and holds one head's rows, while the
@@ -669,13 +608,7 @@ int tc_fwd(rnn_ctx* ctx, const Args& a) {
   }
   tc_fwd_kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), FWD_THREADS, FWD_SMEM, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
-  if (p.a.nsplit > 1) {
-    const long long rows = static_cast<long long>(a.n) * a.h * a.tq;
-    join_rows_kernel<<<static_cast<unsigned>((rows + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, ctx->stream>>>(
-        p.a);
-    RNN_CHECK_LAUNCH();
-  }
-  return RNN_OK;
+  return p.a.nsplit > 1 ? join_rows_bf16(ctx, p.a) : RNN_OK;
 }
 
 }  // namespace diff

@@ -241,11 +241,13 @@ int tc_bwd_parts(rnn_ctx* ctx, const Args& a);  // parts (256 floats a key each)
 bool dec_ok(const Args& a);
 int dec_fwd(rnn_ctx* ctx, const Args& a);
 int join_parts(rnn_ctx* ctx, const Args& a);
-// The same in f32, whose parts have 64 columns.
+// The tensor-core kernels in f32 (halves of up to 32 columns).
 bool f32_tc_ok(const Args& a);
 int f32_tc_fwd(rnn_ctx* ctx, const Args& a);
 int f32_tc_bwd(rnn_ctx* ctx, const Args& a);
-int join_parts_f32(rnn_ctx* ctx, const Args& a);
+// Joins parts of many rows: 128 columns in bf16, 64 in f32.
+int join_rows_bf16(rnn_ctx* ctx, const Args& a);
+int join_rows_f32(rnn_ctx* ctx, const Args& a);
 
 }  // namespace diff
 }  // namespace rnn

@@ -1009,7 +1009,17 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
 
 }  // namespace
 
-bool f32_tc_ok(const Args& a) { return a.dh <= 32 && static_cast<long long>(a.grp) * a.tq >= 64 && a.tk >= 32; }
+// A block starts and ends in about 9 us beside 2 us a tile, more than the
+// kernels of mma.sync, which keep what is small (forward and backward of 128 x 64
+// x 64, 4 heads of 32: 28 and 70 us against 38 and 83 here).  Here are faster: 64
+// x 128 x 128: 25 and 62 against 47 and 116; 32 x 256 x 256: 34 and 91 against 82
+// and 206; 64 x 64 x 256: 35 and 91 against 43 and 103; 1 x 64 x 5000: 25 and 283
+// against 26 and 524.  Halves of more than 32 columns would not leave room for
+// two stages of tiles beside the block's rows.
+bool f32_tc_ok(const Args& a) {
+  const long long rows = static_cast<long long>(a.grp) * a.tq;
+  return a.dh <= 32 && rows >= 64 && rows * a.tk >= 64 * 128;
+}
 
 int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
   Params p;
@@ -1035,7 +1045,7 @@ int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
   RNN_TRY(tc::ensure_smem_optin(f32_fwd_kernel, optin, ctx->device, static_cast<int>(FWD_SMEM)));
   f32_fwd_kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), THREADS, FWD_SMEM, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
-  return p.a.nsplit > 1 ? join_parts_f32(ctx, p.a) : RNN_OK;
+  return p.a.nsplit > 1 ? join_rows_f32(ctx, p.a) : RNN_OK;
 }
 
 int f32_tc_bwd(rnn_ctx* ctx, const Args& a) {

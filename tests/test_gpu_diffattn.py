@@ -230,6 +230,39 @@ def test_new_rows_over_a_long_cache(ops, n, tq, tk, h, hkv, dh, causal):
         assert bool((at[..., 0] == 7).all()) and bool((at[..., -2:] == 7).all())
 
 
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("causal", [None, "start", "end"])
+@pytest.mark.parametrize("n,tq,tk,h,hkv,dh", [(2, 128, 128, 2, 2, 32), (3, 130, 257, 2, 1, 32), (2, 70, 1000, 2, 2, 7),
+                                              (1, 33, 2000, 4, 1, 20), (2, 500, 65, 2, 2, 12)])
+def test_f32_over_tiles(ops, n, tq, tk, h, hkv, dh, causal, shift):
+    """f32 calls of several tiles: any width and alignment, lengths and masked keys with anything in them, rows packed
+    across heads, keys split over blocks."""
+    q, k, v, lam, dout = make(n, tq, tk, h, hkv, dh, F32, 31)
+
+    def moved(x):  # the same values at an address that allows no wide loads
+        return torch.zeros(x.numel() + shift, device="cuda")[shift:].view(x.shape).copy_(x)
+
+    q, k, v, dout = (moved(x) for x in (q, k, v, dout))
+    check_all(ops, q, k, v, lam, dout, causal=causal)
+    klen = torch.tensor([tk - 3, 0, 64][:n], dtype=torch.int32, device="cuda")
+    kmask = torch.rand(n, tk, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)) < 0.7
+    hidden = (torch.arange(tk, device="cuda")[None] >= klen[:, None]) | ~kmask
+    k.masked_fill_(hidden[:, :, None, None], math.nan)
+    v.masked_fill_(hidden[:, :, None, None], math.inf)
+    check_all(ops, q, k, v, lam, dout, causal=causal, klen=klen, kmask=kmask)
+
+
+def test_f32_keeps_its_precision(ops):
+    """Products of three bf16 planes leave 2^-24: far below what a product of fewer parts would."""
+    q, k, v, lam, dout = make(2, 256, 300, 2, 2, 32, F32, 3)
+    want = reference(q, k, v, lam, dout, 32 ** -0.5)
+    got = run_all(ops, q, k, v, lam, dout)
+    # 300 terms added in f32: 2^-24 sqrt(300) / 2 = 5e-7; gradients pass two such sums
+    assert rel(got[0], want[0]) < 5e-7 and rel(got[1], want[1]) < 5e-7
+    for x, y in zip(got[3:6], want[2:5]):
+        assert rel(x, y) < 1e-6
+
+
 def test_nearly_equal_maps_over_a_long_cache(ops):
     """What is left of the difference keeps the type's precision when the keys are split too."""
     q, k, v, _, dout = make(1, 130, 3000, 2, 2, 32, BF16, 9)
