@@ -613,7 +613,19 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
   // it matters where few keys are averaged: rows that see one register step of
   // keys sum P dP there (dS of a lone key comes out as 0), and in bf16 rows of
   // up to 128 keys sum it in a pass of its own.
-  const bool one_step = kend <= SUB, own_pass = !one_step && sizeof(T) == 2 && kend <= 128;
+  const bool one_step = kend <= SUB;
+  bool own_pass = !one_step && sizeof(T) == 2 && kend <= 128;
+  if (sizeof(T) == 2 && mask && kend > 128) {  // few of many keys
+    __shared__ int count;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    int c = 0;
+    for (int j = tid; j < kend; j += THREADS) c += mask[j] != 0;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0 && c) atomicAdd(&count, c);
+    __syncthreads();
+    own_pass = count <= 128;
+  }
   if (!one_step && !own_pass) {
     if (ntk > 0) {
       cp_wait<1>();

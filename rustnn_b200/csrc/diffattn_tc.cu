@@ -7,8 +7,8 @@
 // run while the tensor cores form scores and the products with v for the other.
 // Warp 8 copies tiles; warps 9 and 10 issue MMAs, 10 the scores of the first map,
 // 9 the others (an issuing warp stalls while the tensor cores are busy, and one
-// warp alone left them idle at each of its waits); warp 11 clears what lies
-// beyond a sequence's length.  Tensor memory (512 columns):
+// warp alone left them idle at each of its waits); warp 11 clears values
+// that are masked or beyond a sequence's length.  Tensor memory (512 columns):
 //   [0, 128)    A = sum (P_1 - r P_2) v        [128, 256)  B = sum P_2 v
 //   [256, 384)  S_1 | S_2 of even tiles        [384, 512)  the same of odd tiles
 // The bf16 maps overwrite S_2 alone: S_1 of a team's next tile is formed as soon
@@ -88,20 +88,25 @@ struct alignas(64) FwdParams {
 };
 
 struct FwdShared {
-  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], last_full, s1_full[2], s2_full[2], s1_free[2], p_full[2];
+  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], landed[STAGES], s1_full[2], s2_full[2], s1_free[2], p_full[2];
   uint64_t pv_last, o_full, tok[4], drain[2];
   uint32_t tmem;
   int abort_flag;
+  uint2 seen[STAGES];    // masked calls: which keys of a tile count
   float4 ref[QROWS];     // a row's m_1, m_2, r
   float4 sum[2][QROWS];  // m_1, l_1, m_2, l_2 of a team
 };
 constexpr size_t FWD_SMEM = 1024 + Q_BYTES + STAGES * STAGE_BYTES + sizeof(FwdShared);
 
 // What a thread does with its row's 64 scores of one map.
-__device__ __forceinline__ void mask_scores(float (&s)[2][32], int visible) {
+__device__ __forceinline__ void mask_scores(float (&s)[2][32], int visible, uint2 seen) {
+  if (visible < KEYS) {
+    seen.x &= visible >= 32 ? 0xffffffffu : visible > 0 ? (1u << visible) - 1 : 0u;
+    seen.y &= visible > 32 ? (1u << (visible - 32)) - 1 : 0u;
+  }
 #pragma unroll
   for (int c = 0; c < KEYS; c++)
-    if (c >= visible) s[c >> 5][c & 31] = -CUDART_INF_F;
+    if (!((c < 32 ? seen.x : seen.y) >> (c & 31) & 1)) s[c >> 5][c & 31] = -CUDART_INF_F;
 }
 __device__ __forceinline__ float max_of(const float (&s)[2][32]) {
   float m[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
@@ -131,14 +136,14 @@ __device__ __forceinline__ float exp_sum(float (&s)[2][32], float c2, float u) {
 // it matters: when a row has no reference yet (u = -inf) or the sum shows that
 // a score passed it by about 2^20; rows beyond that get their tile's maximum.
 __device__ __forceinline__ float exponentials(uint32_t t, float (&s)[2][32], float& u, float c2, bool edge,
-                                              int visible) {
+                                              int visible, uint2 seen) {
   bool look = __any_sync(0xffffffffu, u == -CUDART_INF_F && visible > 0);
   while (true) {
     tmem_ld(t, s[0]);
     tmem_ld(t + 32, s[1]);
     tmem_landed(s[0]);
     tmem_landed(s[1]);
-    if (__builtin_expect(edge, 0)) mask_scores(s, visible);
+    if (__builtin_expect(edge, 0)) mask_scores(s, visible, seen);
     if (__builtin_expect(look, 0)) {
       const float top = max_of(s) * c2;
       if (u == -CUDART_INF_F || top > u + RAISE) u = top;
@@ -188,6 +193,7 @@ __device__ __forceinline__ bool check_at(int j) { return j == 0 || (j >= 3 && (j
 
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+template <bool MASK>
 __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_constant__ FwdParams p) {
   extern __shared__ uint8_t raw[];
   const Args& a = p.a;
@@ -208,8 +214,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
   const int kbeg = static_cast<int>(blockIdx.y) * a.split_keys;
   const int kend = min(row_limit(a, min(i0 + QROWS, a.tq) - 1, len), kbeg + a.split_keys);
   const int nt = max(kend - kbeg + KEYS - 1, 0) / KEYS;
-  // the last tile may hold rows of a cache beyond the sequence
-  const bool dirty = nt > 0 && kbeg + nt * KEYS > len && len < a.tk;
+  // Values that a row must not meet are cleared: the last tile's that lie in a
+  // cache beyond the sequence, any tile's that are masked.
+  const uint8_t* mask = MASK ? a.kmask + b * a.kmb : nullptr;
+  const int clear0 = MASK ? 0 : nt > 0 && kbeg + nt * KEYS > len && len < a.tk ? nt - 1 : nt;  // first tile to be cleared
+  // phase of a tile's arrival: a stage's uses so far, of one barrier or the other
+  auto clears = [&](int j) { return j >= clear0 && clear0 > 0 ? 0u : static_cast<uint32_t>(j / STAGES) & 1u; };
   const int wide = 2 * a.dh > 64 ? 2 : 1;  // 64-column parts of v
   const int ksteps = (a.dh + 15) / 16;
 
@@ -218,8 +228,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
     for (int i = 0; i < STAGES; i++) {
       mbar_init(&sh.kv_full[i], 1);
       mbar_init(&sh.kv_empty[i], 1);
+      mbar_init(&sh.landed[i], 1);
     }
-    mbar_init(&sh.last_full, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh.s1_full[i], 1);
       mbar_init(&sh.s2_full[i], 1);
@@ -258,21 +268,27 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
 
     for (int j = team; j < nt; j += 2) {
       const int j0 = kbeg + j * KEYS;
-      const bool edge = j0 + KEYS > full;
+      bool edge = j0 + KEYS > full;
       const uint32_t par = (j >> 1) & 1;
       float s1[2][32], s2[2][32];
       // the references the exponentials are taken at: the row's, as far as this
       // team knows them
       float u1 = m1, u2 = m2;
+      uint2 seen = make_uint2(0xffffffffu, 0xffffffffu);
+      if (MASK) {  // from the clearing warp
+        if (!warp_wait(&sh.kv_full[j % STAGES], (j / STAGES) & 1, abort_flag, dev_error)) break;
+        seen = sh.seen[j % STAGES];
+        edge |= (seen.x & seen.y) != 0xffffffffu;
+      }
       if (!warp_wait(&sh.s1_full[team], par, abort_flag, dev_error)) break;
       tc_fence_after();
-      const float sum1 = exponentials(ts, s1, u1, c2, edge, lim - j0);
+      const float sum1 = exponentials(ts, s1, u1, c2, edge, lim - j0, seen);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.s1_free[team]);
       if (!warp_wait(&sh.s2_full[team], par, abort_flag, dev_error)) break;
       tc_fence_after();
-      const float sum2 = exponentials(ts + 64, s2, u2, c2, edge, lim - j0);
+      const float sum2 = exponentials(ts + 64, s2, u2, c2, edge, lim - j0, seen);
 
       // The row's references as tile j - 1 left them.  Where they are what the
       // exponentials were taken at (nearly always), only the sums go on; else
@@ -453,7 +469,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
           if (j >= STAGES && !wait(&sh.kv_empty[st], (j / STAGES - 1) & 1, abort_flag, dev_error)) break;
           const uint32_t dst = skv + st * STAGE_BYTES;
           // a tile to be cleared lands for the clearing warp, which passes it on
-          uint64_t* bar = dirty && j == nt - 1 ? &sh.last_full : &sh.kv_full[st];
+          uint64_t* bar = j >= clear0 ? &sh.landed[st] : &sh.kv_full[st];
           mbar_arrive_expect_tx(bar, (2 + wide) * HALF_BYTES);
           for (int half = 0; half < 2; half++)
             tma_5d(dst + half * HALF_BYTES, &p.k, 0, half, kvh, kbeg + j * KEYS, b, bar);
@@ -463,23 +479,22 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
         // what was asked for lands before the block may end, aborting or not
         settle(&sh.q_full, 0);
         for (int t = max(0, j - STAGES); t < j; t++)
-          settle(dirty && t == nt - 1 ? &sh.last_full : &sh.kv_full[t % STAGES],
-                 dirty && t == nt - 1 ? 0 : (t / STAGES) & 1);
+          settle(t >= clear0 ? &sh.landed[t % STAGES] : &sh.kv_full[t % STAGES], clears(t));
       }
       __syncwarp();
     } else if (warp == WARP_CLEAR) {
-      if (dirty) {
-        const int j = nt - 1, st = j % STAGES;
-        if (warp_wait(&sh.last_full, 0, abort_flag, dev_error)) {
-          // hidden values may be NaN: P = 0 there, so v has to be finite
-          uint8_t* v = base + Q_BYTES + st * STAGE_BYTES + 2 * HALF_BYTES;
-          for (int r = len - kbeg - j * KEYS; r < KEYS; r++)
-            for (int c = lane; c < wide * 8; c += 32)
-              *reinterpret_cast<uint4*>(v + (c >> 3) * HALF_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.kv_full[st]);
-        }
+      Seen keys;
+      if (clear0 < nt) keys.load(mask, kbeg + clear0 * KEYS, len);
+      for (int j = clear0; j < nt; j++) {
+        const int st = j % STAGES;
+        const uint2 seen = keys.bits();
+        if (j + 1 < nt) keys.load(mask, kbeg + (j + 1) * KEYS, len);
+        if (!warp_wait(&sh.landed[st], clears(j), abort_flag, dev_error)) break;
+        clear_hidden(base + Q_BYTES + st * STAGE_BYTES + 2 * HALF_BYTES, seen, wide);
+        if (lane == 0) sh.seen[st] = seen;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.kv_full[st]);
       }
     } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
@@ -566,7 +581,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
 // 51; 128 x 33 x 1000, 8 of 64: 181 against 508; 32 x 1000 x 16: 102 against 131
 // (the others timed with a mask of keys that hides none).
 bool tc_fwd_ok(const Args& a) {
-  if (a.dh % 8 || a.dh < 16 || a.dh > 64 || a.kmask || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
+  if (a.dh % 8 || a.dh < 16 || a.dh > 64 || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
   if (a.tq < 16 || std::max(a.tq, a.tk) < 64) return false;
   if (reinterpret_cast<uintptr_t>(a.o2) % 16) return false;
   return map_ok(a.q, a.n, a.tq, a.h, a.dh, a.qb, a.qr, a.qh) && map_ok(a.k, a.n, a.tk, a.hkv, a.dh, a.kb, a.kr, a.kh) &&
@@ -594,8 +609,9 @@ int tc_fwd(rnn_ctx* ctx, const Args& a) {
   RNN_TRY(encode_map(&p.v, a.v, a.n, a.tk, a.hkv, 1, 2 * a.dh, a.vb, a.vr, a.vh, KEYS));
   const long long blocks = (a.tq + QROWS - 1ll) / QROWS * a.n * a.h;
   RNN_REQUIRE(blocks < (1ll << 31), "diffattn: too many rows");
-  static std::atomic<unsigned long long> optin{0};
-  RNN_TRY(tc::ensure_smem_optin(tc_fwd_kernel, optin, ctx->device, static_cast<int>(FWD_SMEM)));
+  static std::atomic<unsigned long long> optin[2];
+  const auto kernel = a.kmask ? tc_fwd_kernel<true> : tc_fwd_kernel<false>;
+  RNN_TRY(tc::ensure_smem_optin(kernel, optin[a.kmask != nullptr], ctx->device, static_cast<int>(FWD_SMEM)));
   const int tiles = (a.tk + KEYS - 1) / KEYS;
   const long long parts = key_parts(ctx, blocks, tiles);
   p.a.split_keys = static_cast<int>((tiles + parts - 1) / parts) * KEYS;
@@ -606,7 +622,7 @@ int tc_fwd(rnn_ctx* ctx, const Args& a) {
     p.a.part = static_cast<float*>(ctx->ws);
     p.a.stat = p.a.part + rows * p.a.nsplit * 256;
   }
-  tc_fwd_kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), FWD_THREADS, FWD_SMEM, ctx->stream>>>(p);
+  kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), FWD_THREADS, FWD_SMEM, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
   return p.a.nsplit > 1 ? join_rows_bf16(ctx, p.a) : RNN_OK;
 }

@@ -221,6 +221,33 @@ __device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
   }
 }
 
+// Which of a tile's 64 keys from j0 on exist and are not masked (the whole warp
+// calls): load() asks memory for them, so that it can run ahead, bits() answers.
+struct Seen {
+  bool lo, hi;
+  __device__ __forceinline__ void load(const uint8_t* mask, int j0, int len) {
+    const int j = j0 + (threadIdx.x & 31);
+    lo = j < len && (mask == nullptr || mask[j] != 0);
+    hi = j + 32 < len && (mask == nullptr || mask[j + 32] != 0);
+  }
+  __device__ __forceinline__ uint2 bits() const {
+    return make_uint2(__ballot_sync(0xffffffffu, lo), __ballot_sync(0xffffffffu, hi));
+  }
+};
+// Clears the rows of a 64-row tile that `seen` leaves out: `parts` pieces of 128
+// bytes a row, 8192 bytes apart.  What is hidden may be NaN, and meets P = 0 in a
+// product.
+__device__ __forceinline__ void clear_hidden(uint8_t* tile, uint2 seen, int parts) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int half = 0; half < 2; half++)
+    for (uint32_t gone = ~(half ? seen.y : seen.x); gone; gone &= gone - 1) {
+      const int r = half * 32 + __ffs(gone) - 1;
+      for (int c = lane; c < parts * 8; c += 32)
+        *reinterpret_cast<uint4*>(tile + (c >> 3) * 8192 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+}
+
 // Tensor map of a bf16 view [n, t, heads, 2 halves, dh] read in boxes of 64
 // columns of one half and `rows` rows; columns beyond dh and rows beyond t are
 // zero.  The contiguous 2*dh columns of v and dout are read with halves == 1.

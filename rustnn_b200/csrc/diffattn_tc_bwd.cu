@@ -9,8 +9,8 @@
 // them.  Warp 16 copies tiles (and in the keys' kernel brings the queries'
 // log-sums and D).  Two warps issue MMAs, 17 the products with dS and dP, 18 the
 // scores: an issuing warp stalls while the tensor cores are busy, and one warp
-// alone left them idle at each of its waits.  Warp 19 clears what lies beyond a
-// sequence's length (queries' kernel) or sums dlam (keys' kernel).
+// alone left them idle at each of its waits.  Warp 19 clears what is masked or
+// lies beyond a sequence's length (queries' kernel) or sums dlam (keys' kernel).
 #include <algorithm>
 #include <cmath>
 
@@ -60,14 +60,17 @@ __device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&v)[16], 
 constexpr int Q_STAGES = 4;
 constexpr uint32_t Q_STAGE = 4 * SMALL;  // k halves, v parts
 struct QShared {
-  uint64_t q_full, kv_full[Q_STAGES], kv_empty[Q_STAGES], last_full, s_full[2], s_free[2], d_full[2], p_full[2];
+  uint64_t q_full, kv_full[Q_STAGES], kv_empty[Q_STAGES], landed[Q_STAGES], s_full[2], s_free[2], d_full[2], p_full[2];
   uint64_t o_full, drain[2];
   uint32_t tmem;
   int abort_flag;
+  uint2 seen[Q_STAGES];  // masked calls: which keys of a tile count
+  int count;             // and how many of all
   float2 part[4][ROWS];
 };
 constexpr size_t Q_SMEM = 1024 + 4 * BIG + Q_STAGES * Q_STAGE + sizeof(QShared);
 
+template <bool MASK>
 __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw[];
   const Args& a = p.a;
@@ -86,7 +89,13 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
   const int len = key_len(a, b);
   const int kend = row_limit(a, min(i0 + ROWS, a.tq) - 1, len);
   const int nt = (kend + COLS - 1) / COLS;
-  const bool dirty = nt > 0 && nt * COLS > len && len < a.tk;
+  // tiles from clear0 on have hidden keys and values to be cleared, as in the forward pass
+  const uint8_t* mask = MASK ? a.kmask + b * a.kmb : nullptr;
+  const int clear0 = MASK ? 0 : nt > 0 && nt * COLS > len && len < a.tk ? nt - 1 : nt;
+  auto clears = [&](int t) { return t >= clear0 && clear0 > 0 ? 0u : static_cast<uint32_t>(t / Q_STAGES) & 1u; };
+  // Where a mask leaves few keys of many, their D comes from a pass of its own
+  // over the tiles: step t is tile t - lead_in, or t while t < lead_in.
+  int lead_in = 0;
   const int wide = 2 * a.dh > 64 ? 2 : 1, ksteps = (a.dh + 15) / 16, dsteps = a.dh / 8;
 
   if (tid == 0) {
@@ -94,8 +103,8 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     for (int i = 0; i < Q_STAGES; i++) {
       mbar_init(&sh.kv_full[i], 1);
       mbar_init(&sh.kv_empty[i], 1);
+      mbar_init(&sh.landed[i], 1);
     }
-    mbar_init(&sh.last_full, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.s_free[i], 8);
@@ -106,6 +115,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     mbar_init(&sh.drain[0], 1);
     mbar_init(&sh.drain[1], 1);
     sh.abort_flag = 0;
+    if (MASK) sh.count = 0;
     fence_barrier_init();
   }
   if (warp == WARP_MMA) {
@@ -116,6 +126,15 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  if (MASK && nt > 2) {
+    int c = 0;
+    for (int j = tid; j < kend; j += THREADS) c += mask[j] != 0;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0 && c) atomicAdd(&sh.count, c);
+    __syncthreads();
+    if (sh.count <= 128) lead_in = nt;
+  }
+  const int steps = nt + lead_in;
 
   // registers: 640 threads x 96 at launch = 512 x 104 + 128 x 64
   if (warp < SOFT) {
@@ -133,7 +152,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     const f32x2 cc = pair(c2, c2), n1 = pair(-ls1, -ls1), n2 = pair(-ls2, -ls2);
 
     // both maps' entries of 16 columns from the scores
-    auto maps = [&](uint32_t t, float (&x)[16], float (&y)[16], int visible, bool edge) {
+    auto maps = [&](uint32_t t, float (&x)[16], float (&y)[16], int visible, bool edge, uint32_t seen) {
       tmem_ld(t, x);
       tmem_ld(t + 64, y);
       tmem_landed(x);
@@ -150,14 +169,16 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       if (__builtin_expect(edge, 0)) {
 #pragma unroll
         for (int c = 0; c < 16; c++)
-          if (c >= visible) x[c] = y[c] = 0.0f;
+          if (c >= visible || !(seen >> c & 1)) x[c] = y[c] = 0.0f;
       }
     };
+    // which of this thread's 32 keys of step t count
+    auto counts = [&](int t) { return !MASK ? 0xffffffffu : half ? sh.seen[t % Q_STAGES].y : sh.seen[t % Q_STAGES].x; };
 
     // D_1 and D_2: from o and o2, or, where a row sees at most two tiles, from
     // P dP itself (see diffattn.cu on what their rounding does to short rows).
     float d1 = 0.0f, d2 = 0.0f;
-    if (nt > 2) {
+    if (nt > 2 && lead_in == 0) {
       if (in) {
         const int c0 = k4 * (a.dh / 2);
         const __nv_bfloat16* po = static_cast<const __nv_bfloat16*>(a.fo) + b * a.ob + head * a.oh + i * a.orow + c0;
@@ -183,14 +204,15 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
           }
         }
       }
-    } else if (team < nt) {
+    } else if (lead_in == 0 && team < nt) {
+      warp_wait(&sh.kv_full[team], 0, abort_flag, dev_error);
       warp_wait(&sh.s_full[team], 0, abort_flag, dev_error);
       warp_wait(&sh.d_full[team], 0, abort_flag, dev_error);
       tc_fence_after();
 #pragma unroll 1
       for (int c = 0; c < 32; c += 16) {
         float x[16], y[16], dp[16];
-        maps(ts + c, x, y, lim - team * COLS - c, true);
+        maps(ts + c, x, y, lim - team * COLS - c, true, counts(team) >> c);
         tmem_ld(ts + 128 + c, dp);
         tmem_landed(dp);
 #pragma unroll
@@ -200,35 +222,69 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
         }
       }
     }
-    sh.part[k4][row] = make_float2(d1, d2);
-    soft_sync();
-    d1 = d2 = 0.0f;
+    f32x2 e1, e2;  // -D_1, -D_2
+    // sums the row's four shares of D
+    auto settle_d = [&] {
+      sh.part[k4][row] = make_float2(d1, d2);
+      soft_sync();
+      d1 = d2 = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      d1 += sh.part[k][row].x;
-      d2 += sh.part[k][row].y;
-    }
-    if (in && k4 == 0) {
-      a.dsum[stat] = d1;
-      a.dsum[stat + a.tq] = d2;
-    }
-    soft_sync();
-
-    const f32x2 e1 = pair(-d1, -d1), e2 = pair(-d2, -d2);
+      for (int k = 0; k < 4; k++) {
+        d1 += sh.part[k][row].x;
+        d2 += sh.part[k][row].y;
+      }
+      if (in && k4 == 0) {
+        a.dsum[stat] = d1;
+        a.dsum[stat + a.tq] = d2;
+      }
+      soft_sync();
+      e1 = pair(-d1, -d1);
+      e2 = pair(-d2, -d2);
+    };
+    if (lead_in == 0) settle_d();
     f32x2 dl = 0ull, pl = 0ull;
-    for (int j = team; j < nt; j += 2) {
-      const uint32_t par = (j >> 1) & 1;
-      const bool edge = j * COLS + 32 > full;
+    bool settled = lead_in == 0;
+    for (int t = team; t < steps; t += 2) {
+      const uint32_t par = (t >> 1) & 1;
+      const int j = t < lead_in ? t : t - lead_in;
+      if (MASK && !settled && t >= lead_in) {
+        settle_d();
+        settled = true;
+      }
+      bool edge = j * COLS + 32 > full;
+      uint32_t seen = 0xffffffffu;
+      if (MASK) {  // from the clearing warp
+        if (!warp_wait(&sh.kv_full[t % Q_STAGES], (t / Q_STAGES) & 1, abort_flag, dev_error)) break;
+        seen = counts(t);
+        edge |= seen != 0xffffffffu;
+      }
       float x[2][16], y[2][16];
       if (!warp_wait(&sh.s_full[team], par, abort_flag, dev_error)) break;
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 2; c++) maps(ts + c * 16, x[c], y[c], lim - j * COLS - c * 16, edge);
+      for (int c = 0; c < 2; c++) maps(ts + c * 16, x[c], y[c], lim - j * COLS - c * 16, edge, seen >> (c * 16));
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.s_free[team]);
       if (!warp_wait(&sh.d_full[team], par, abort_flag, dev_error)) break;
       tc_fence_after();
+      if (MASK && t < lead_in) {
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float dp[16];
+          tmem_ld(ts + 128 + c * 16, dp);
+          tmem_landed(dp);
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            d1 += x[c][e] * dp[e];
+            d2 += y[c][e] * dp[e];
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[team]);
+        continue;
+      }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         uint32_t u[8], v[8];
@@ -258,6 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_full[team]);
     }
+    if (MASK && !settled) settle_d();  // every soft warp does, an aborting one too
     float l0, l1, p0, p1;
     unpair(dl, l0, l1);
     unpair(pl, p0, p1);
@@ -296,37 +353,36 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
         mbar_arrive_expect_tx(&sh.q_full, (2 + wide) * BIG);
         for (int h = 0; h < 2; h++) tma_5d(sq + h * BIG, &p.q, 0, h, head, i0, b, &sh.q_full);
         for (int c = 0; c < wide; c++) tma_5d(sg + c * BIG, &p.g, c * 64, 0, head, i0, b, &sh.q_full);
-        int j = 0;
-        for (; j < nt; j++) {
-          const int st = j % Q_STAGES;
-          if (j >= Q_STAGES && !wait(&sh.kv_empty[st], (j / Q_STAGES - 1) & 1, abort_flag, dev_error)) break;
+        int t = 0;
+        for (; t < steps; t++) {
+          const int st = t % Q_STAGES, j = t < lead_in ? t : t - lead_in;
+          if (t >= Q_STAGES && !wait(&sh.kv_empty[st], (t / Q_STAGES - 1) & 1, abort_flag, dev_error)) break;
           const uint32_t dst = skv + st * Q_STAGE;
           // a tile to be cleared lands for the clearing warp, which passes it on
-          uint64_t* bar = dirty && j == nt - 1 ? &sh.last_full : &sh.kv_full[st];
+          uint64_t* bar = t >= clear0 ? &sh.landed[st] : &sh.kv_full[st];
           mbar_arrive_expect_tx(bar, (2 + wide) * SMALL);
           for (int h = 0; h < 2; h++) tma_5d(dst + h * SMALL, &p.k, 0, h, kvh, j * COLS, b, bar);
           for (int c = 0; c < wide; c++) tma_5d(dst + (2 + c) * SMALL, &p.v, c * 64, 0, kvh, j * COLS, b, bar);
         }
         // what was asked for lands before the block may end, aborting or not
         settle(&sh.q_full, 0);
-        for (int t = max(0, j - Q_STAGES); t < j; t++)
-          settle(dirty && t == nt - 1 ? &sh.last_full : &sh.kv_full[t % Q_STAGES],
-                 dirty && t == nt - 1 ? 0 : (t / Q_STAGES) & 1);
+        for (int i = max(0, t - Q_STAGES); i < t; i++)
+          settle(i >= clear0 ? &sh.landed[i % Q_STAGES] : &sh.kv_full[i % Q_STAGES], clears(i));
       }
       __syncwarp();
     } else if (warp == WARP_AUX) {
-      if (dirty) {
-        const int j = nt - 1, st = j % Q_STAGES;
-        if (warp_wait(&sh.last_full, 0, abort_flag, dev_error)) {
-          // hidden keys and values may be NaN: both meet P = 0 in a product
-          uint8_t* kv = base + 4 * BIG + st * Q_STAGE;
-          for (int r = len - j * COLS; r < COLS; r++)
-            for (int c = lane; c < (2 + wide) * 8; c += 32)
-              *reinterpret_cast<uint4*>(kv + (c >> 3) * SMALL + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.kv_full[st]);
-        }
+      Seen keys;
+      if (clear0 < nt) keys.load(mask, clear0 * COLS, len);
+      for (int t = clear0; t < steps; t++) {
+        const int st = t % Q_STAGES, next = t + 1 < lead_in ? t + 1 : t + 1 - lead_in;
+        const uint2 seen = keys.bits();
+        if (t + 1 < steps) keys.load(mask, next * COLS, len);
+        if (!warp_wait(&sh.landed[st], clears(t), abort_flag, dev_error)) break;
+        clear_hidden(base + 4 * BIG + st * Q_STAGE, seen, 2 + wide);
+        if (lane == 0) sh.seen[st] = seen;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.kv_full[st]);
       }
     } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
@@ -337,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       int st = 0;
       if (warp == WARP_SCORE) {
         const uint64_t dq = desc_k(sq), dkv = desc_k(skv);
-        for (int j = 0; ok && j < nt; j++) {
+        for (int j = 0; ok && j < steps; j++) {
           // the team has the scores of tile j - 2 in registers
           if (!(ok = landed(j, st) && (j < 2 || done(&sh.s_free[j & 1], ((j >> 1) - 1) & 1)))) break;
           tc_fence_after();
@@ -367,26 +423,29 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
                      kv + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
           commit(&sh.d_full[j & 1], lead);
         };
-        for (int j = 0; ok && j < min(nt, 2); j++)
+        for (int j = 0; ok && j < min(steps, 2); j++)
           if ((ok = landed(j, j))) {
             tc_fence_after();
             slopes(j, j);
           }
         int st2 = 2;
-        for (int j = 0; ok && j < nt; j++) {
-          if (!(ok = (j + 2 >= nt || landed(j + 2, st2)) && done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
+        for (int j = 0; ok && j < steps; j++) {
+          if (!(ok = (j + 2 >= steps || landed(j + 2, st2)) && done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
           tc_fence_after();
           const uint64_t k = dmn + st * (Q_STAGE / 16);
           const uint32_t s = tmem + 256 + (j & 1) * 192;
+          if (!MASK || j >= lead_in) {
 #pragma unroll
-          for (int m = 0; m < 2; m++)
+            for (int m = 0; m < 2; m++)
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++)
-              mma_ts(tmem + m * 64, s + ks * 16 + m * 8, k + (m * SMALL + ks * 2048) / 16, id_o, j > 0 || ks > 0, lead);
+              for (int ks = 0; ks < 4; ks++)
+                mma_ts(tmem + m * 64, s + ks * 16 + m * 8, k + (m * SMALL + ks * 2048) / 16, id_o, j > lead_in || ks > 0,
+                       lead);
+          }
           // the scores of tile j are long done: dS came of them
           commit(&sh.kv_empty[st], lead);
-          if (j + 1 == nt) commit(&sh.o_full, lead);
-          if (j + 2 < nt) slopes(j + 2, st2);
+          if (j + 1 == steps) commit(&sh.o_full, lead);
+          if (j + 2 < steps) slopes(j + 2, st2);
           if (++st == Q_STAGES) st = 0;
           if (++st2 == Q_STAGES) st2 = 0;
         }
@@ -592,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_kv_kernel(const __grid_cons
       tc_fence_after();
     }
     if (ok && work) {
-      const bool some = nt > 0 && key < len;
+      const bool some = nt > 0 && key < len && (!a.kmask || a.kmask[b * a.kmb + key]);
       __nv_bfloat16* odk = static_cast<__nv_bfloat16*>(a.dk) + b * a.dkb + kvh * a.dkh + key * a.dkr;
       __nv_bfloat16* odv = static_cast<__nv_bfloat16*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr;
       float* part = a.kparts > 1
@@ -811,7 +870,7 @@ bool mult8(std::initializer_list<long long> s) {
 // (4 x 4 x 4096, 32 heads on 4: 132 us against 468; 64 x 24 x 256, 8 heads of 32:
 // 84 against 88; 32 x 1000 x 16, 8 of 64: 163 against 281).
 bool tc_bwd_ok(const Args& a) {
-  if (a.dh % 8 || a.dh < 16 || a.dh > 64 || a.kmask || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
+  if (a.dh % 8 || a.dh < 16 || a.dh > 64 || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
   if (std::max(a.tq, a.tk) < 64) return false;
   if (reinterpret_cast<uintptr_t>(a.fo) % 16 || reinterpret_cast<uintptr_t>(a.fo2) % 16) return false;
   if (!mult8({a.ob, a.orow, a.oh})) return false;
@@ -830,14 +889,15 @@ int tc_bwd(rnn_ctx* ctx, const Args& a) {
   const long long qblocks = (a.tq + ROWS - 1ll) / ROWS * a.n * a.h;
   const long long kblocks = std::max<long long>((a.tk + ROWS - 1ll) / ROWS * a.n * a.hkv, a.h);
   RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31), "diffattn: too many rows");
-  static std::atomic<unsigned long long> optin_q{0}, optin_k{0};
-  RNN_TRY(tc::ensure_smem_optin(tc_bwd_q_kernel, optin_q, ctx->device, static_cast<int>(Q_SMEM)));
+  static std::atomic<unsigned long long> optin_q[2], optin_k{0};
+  const auto q_kernel = a.kmask ? tc_bwd_q_kernel<true> : tc_bwd_q_kernel<false>;
+  RNN_TRY(tc::ensure_smem_optin(q_kernel, optin_q[a.kmask != nullptr], ctx->device, static_cast<int>(Q_SMEM)));
   RNN_TRY(tc::ensure_smem_optin(tc_bwd_kv_kernel, optin_k, ctx->device, static_cast<int>(K_SMEM)));
   RNN_TRY(encode_map(&p.q, a.q, a.n, a.tq, a.h, 2, a.dh, a.qb, a.qr, a.qh, ROWS));
   RNN_TRY(encode_map(&p.g, a.dout, a.n, a.tq, a.h, 1, 2 * a.dh, a.gb, a.gr, a.gh, ROWS));
   RNN_TRY(encode_map(&p.k, a.k, a.n, a.tk, a.hkv, 2, a.dh, a.kb, a.kr, a.kh, COLS));
   RNN_TRY(encode_map(&p.v, a.v, a.n, a.tk, a.hkv, 1, 2 * a.dh, a.vb, a.vr, a.vh, COLS));
-  tc_bwd_q_kernel<<<static_cast<unsigned>(qblocks), THREADS, Q_SMEM, ctx->stream>>>(p);
+  q_kernel<<<static_cast<unsigned>(qblocks), THREADS, Q_SMEM, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
   // the keys' kernel owns 128 keys and reads the queries 64 at a time
   RNN_TRY(encode_map(&p.q, a.q, a.n, a.tq, a.h, 2, a.dh, a.qb, a.qr, a.qh, COLS));

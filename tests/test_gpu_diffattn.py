@@ -28,6 +28,12 @@ def ops():
     return _ops
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(ops):
+    yield
+    ops.default_context(0).synchronize()  # raises what a kernel has recorded
+
+
 def visible(n, tq, tk, causal, klen, kmask):
     i, j = torch.arange(tq, device="cuda")[:, None], torch.arange(tk, device="cuda")[None]
     length = (klen.long().clamp(0, tk) if klen is not None else torch.full((n,), tk, device="cuda"))[:, None, None]
@@ -261,6 +267,38 @@ def test_f32_keeps_its_precision(ops):
     assert rel(got[0], want[0]) < 5e-7 and rel(got[1], want[1]) < 5e-7
     for x, y in zip(got[3:6], want[2:5]):
         assert rel(x, y) < 1e-6
+
+
+@pytest.mark.parametrize("causal", [None, "start", "end"])
+@pytest.mark.parametrize("tq,tk,h,hkv,dh", [(300, 700, 2, 1, 40), (130, 1000, 2, 2, 64), (700, 700, 2, 2, 32),
+                                            (70, 90, 2, 1, 24), (200, 200, 2, 2, 5)])
+def test_masked_keys_over_many_tiles(ops, tq, tk, h, hkv, dh, causal):
+    """bf16 with key masks: some keys, whole tiles, all but three keys, all but one, or all of them hidden, and NaN or
+    infinite; with lengths besides."""
+    n = 6
+    q, k, v, lam, dout = make(n, tq, tk, h, hkv, dh, BF16, 23)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    kmask = torch.rand(n, tk, device="cuda", generator=g) < 0.7
+    kmask[1, :67] = False
+    kmask[2] = False
+    kmask[2, [1, tk // 2, tk - 60]] = True
+    kmask[3] = False
+    kmask[4] = False
+    kmask[4, tk // 3] = True
+    klen = torch.tensor([tk, tk - 5, tk, tk, tk, tk // 2 + 3], dtype=torch.int32, device="cuda")
+    hidden = (torch.arange(tk, device="cuda")[None] >= klen[:, None]) | ~kmask
+    k.masked_fill_(hidden[:, :, None, None], math.nan)
+    v.masked_fill_(hidden[:, :, None, None], math.inf)
+    o, lse = check_all(ops, q, k, v, lam, dout, causal=causal, klen=klen, kmask=kmask)
+    assert bool((o[3] == 0).all()) and bool((lse[3] == math.inf).all())
+    want = reference(q, k, v, lam, dout, dh ** -0.5, causal, klen, kmask)
+    got = run_all(ops, q, k, v, lam, dout, causal=causal, klen=klen, kmask=kmask)
+    for b in (0, 1, 2, 5):  # each sequence by itself, whose rows outweigh none
+        for x, y in zip((got[0], got[3], got[4], got[5]), (want[0], want[2], want[3], want[4])):
+            assert rel(x[b], y[b]) < 2 * TOL[BF16], (b, rel(x[b], y[b]))
+    # one key: dq and dk are 0 but for what two roundings of P dP - D leave
+    for x, y in ((got[3], dout), (got[4], dout)):
+        assert float(x[4].double().norm()) < 1e-5 * float(y[4].double().norm()) * float(q[4].double().norm())
 
 
 def test_nearly_equal_maps_over_a_long_cache(ops):
