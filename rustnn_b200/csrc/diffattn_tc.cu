@@ -99,14 +99,11 @@ struct FwdShared {
 constexpr size_t FWD_SMEM = 1024 + Q_BYTES + STAGES * STAGE_BYTES + sizeof(FwdShared);
 
 // What a thread does with its row's 64 scores of one map.
+template <bool MASK>
 __device__ __forceinline__ void mask_scores(float (&s)[2][32], int visible, uint2 seen) {
-  if (visible < KEYS) {
-    seen.x &= visible >= 32 ? 0xffffffffu : visible > 0 ? (1u << visible) - 1 : 0u;
-    seen.y &= visible > 32 ? (1u << (visible - 32)) - 1 : 0u;
-  }
 #pragma unroll
   for (int c = 0; c < KEYS; c++)
-    if (!((c < 32 ? seen.x : seen.y) >> (c & 31) & 1)) s[c >> 5][c & 31] = -CUDART_INF_F;
+    if (c >= visible || (MASK && !((c < 32 ? seen.x : seen.y) >> (c & 31) & 1))) s[c >> 5][c & 31] = -CUDART_INF_F;
 }
 __device__ __forceinline__ float max_of(const float (&s)[2][32]) {
   float m[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
@@ -135,6 +132,7 @@ __device__ __forceinline__ float exp_sum(float (&s)[2][32], float c2, float u) {
 // to s, at reference u; returns their sum.  The maximum is only looked for where
 // it matters: when a row has no reference yet (u = -inf) or the sum shows that
 // a score passed it by about 2^20; rows beyond that get their tile's maximum.
+template <bool MASK>
 __device__ __forceinline__ float exponentials(uint32_t t, float (&s)[2][32], float& u, float c2, bool edge,
                                               int visible, uint2 seen) {
   bool look = __any_sync(0xffffffffu, u == -CUDART_INF_F && visible > 0);
@@ -143,7 +141,7 @@ __device__ __forceinline__ float exponentials(uint32_t t, float (&s)[2][32], flo
     tmem_ld(t + 32, s[1]);
     tmem_landed(s[0]);
     tmem_landed(s[1]);
-    if (__builtin_expect(edge, 0)) mask_scores(s, visible, seen);
+    if (__builtin_expect(edge, 0)) mask_scores<MASK>(s, visible, seen);
     if (__builtin_expect(look, 0)) {
       const float top = max_of(s) * c2;
       if (u == -CUDART_INF_F || top > u + RAISE) u = top;
@@ -282,13 +280,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
       }
       if (!warp_wait(&sh.s1_full[team], par, abort_flag, dev_error)) break;
       tc_fence_after();
-      const float sum1 = exponentials(ts, s1, u1, c2, edge, lim - j0, seen);
+      const float sum1 = exponentials<MASK>(ts, s1, u1, c2, edge, lim - j0, seen);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.s1_free[team]);
       if (!warp_wait(&sh.s2_full[team], par, abort_flag, dev_error)) break;
       tc_fence_after();
-      const float sum2 = exponentials(ts + 64, s2, u2, c2, edge, lim - j0, seen);
+      const float sum2 = exponentials<MASK>(ts + 64, s2, u2, c2, edge, lim - j0, seen);
 
       // The row's references as tile j - 1 left them.  Where they are what the
       // exponentials were taken at (nearly always), only the sums go on; else

@@ -319,8 +319,9 @@ def _rope(x, pos, inv_freq, pairs, interleaved, backward, out, ctx):
     pp = _plain(pos, "pos", _I32, (rows, len(counts)), device)
     fp = _plain(inv_freq, "inv_freq", _F32, (total,), device)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
-        ys, yp = (heads * dh, dh), out.data_ptr()
+        ys = (heads * dh, dh, 1)
+        out = torch.empty_strided(shape, ys, dtype=dtype, device=device)
+        yp = out.data_ptr()
     else:
         _, ys, yp = _view(out, "out", 3, dtype, shape, device)
     call("rnn_rope_dev", _ctx_of(x, ctx), _DTYPES[dtype], xp, xs[0], xs[1], rows, heads, dh, pp, len(counts), counts, fp,
@@ -348,6 +349,15 @@ def rope_backward(dy, pos, inv_freq, pairs, interleaved=False, out=None, ctx=Non
 _CAUSAL = {None: 0, "start": 1, "end": 2}
 
 
+def _fresh(shape, dtype, device):
+    """A new contiguous tensor of four axes, its strides and address (with the
+    strides given, an allocation takes half the time)."""
+    _, t, h, w = shape
+    strides = (t * h * w, h * w, w, 1)
+    x = torch.empty_strided(shape, strides, dtype=dtype, device=device)
+    return x, strides, x.data_ptr()
+
+
 def _diffattn(q, k, v, lam, o, scale, causal, klen, kmask):
     """Checks a differential attention call, allocating o if it is None;
     (description, o, addresses of q, k, v, lam, o)."""
@@ -360,8 +370,7 @@ def _diffattn(q, k, v, lam, o, scale, causal, klen, kmask):
         raise RnnError(f"k: shape {tuple(kshape)}, expected ({n}, *, *, {w})")
     _, vs, vp = _view(v, "v", 4, dtype, kshape, device)
     if o is None:
-        o = torch.empty(shape, device=device, dtype=dtype)
-        os, op = (tq * h * w, h * w, w), o.data_ptr()
+        o, os, op = _fresh(shape, dtype, device)
     else:
         _, os, op = _view(o, "out", 4, dtype, shape, device)
     lp = _plain(lam, "lam", _F32, (h,), device)
@@ -394,7 +403,7 @@ def diffattn_forward(q, k, v, lam, scale=None, causal=None, klen=None, kmask=Non
     d, out, ptrs = _diffattn(q, k, v, lam, out, scale, causal, klen, kmask)
     o2 = lse = None
     if save:
-        o2 = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        o2 = _fresh(q.shape, q.dtype, q.device)[0]
         lse = torch.empty((d.n, d.h, 2, d.tq), device=q.device, dtype=torch.float32)
     call("rnn_diffattn_fwd_dev", _ctx_of(q, ctx), d, *ptrs, None if o2 is None else o2.data_ptr(),
          None if lse is None else lse.data_ptr())
@@ -415,14 +424,13 @@ def diffattn_backward(dout, q, k, v, lam, o, o2, lse, dlam, scale=None, causal=N
     o2p = _plain(o2, "o2", (dtype,), q.shape, device)
     lsep = _plain(lse, "lse", _F32, (d.n, d.h, 2, d.tq), device)
     dlp = _plain(dlam, "dlam", _F32, (d.h,), device)
-    grads = [torch.empty(t.shape, device=device, dtype=dtype) if g is None else g
-             for g, t in ((dq, q), (dk, k), (dv, v))]
-    (_, qs, qp), (_, ks, kp), (_, vs, vp) = (_view(g, name, 4, dtype, t.shape, device)
-                                             for g, t, name in zip(grads, (q, k, v), ("dq", "dk", "dv")))
+    (dq, qs, qp), (dk, ks, kp), (dv, vs, vp) = (
+        _fresh(t.shape, dtype, device) if g is None else (g, *_view(g, name, 4, dtype, t.shape, device)[1:])
+        for g, t, name in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")))
     gd = DiffAttn(d.dtype, d.causal, d.n, d.h, d.hkv, d.dh, d.tq, d.tk, d.scale, 0, qs[0], qs[1], qs[2], ks[0], ks[1],
                   ks[2], vs[0], vs[1], vs[2], gs[0], gs[1], gs[2])
     call("rnn_diffattn_bwd_dev", _ctx_of(q, ctx), d, gd, *ptrs, o2p, lsep, gp, qp, kp, vp, dlp)
-    return tuple(grads)
+    return dq, dk, dv
 
 
 # ---------------------------------------------------------------- norm.rs / linear.rs
