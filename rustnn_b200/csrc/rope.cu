@@ -12,7 +12,8 @@
 // so no table is read.  The product pos * inv_freq is exact in f64 and is
 // reduced to a fraction of a turn there before sincospif, so the error does
 // not grow with the position; the rotation itself is f32, rounded once to the
-// tensor's type.
+// tensor's type.  Measured: 32768 x 32 x 64 bf16, 45 us, 5.9 TB/s of a copy's
+// 6.55; 30011 x 12 x 48 f32 interleaved, 26 us, 5.4 TB/s.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -301,6 +301,30 @@ def test_masked_keys_over_many_tiles(ops, tq, tk, h, hkv, dh, causal):
         assert float(x[4].double().norm()) < 1e-5 * float(y[4].double().norm()) * float(q[4].double().norm())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tq,tk,h,hkv,dh", [(1, 3000, 4, 1, 64), (2, 700, 2, 2, 32), (3, 1111, 8, 2, 40), (1, 90, 2, 1, 16),
+                                            (1, 500, 2, 1, 5)])
+def test_few_rows_over_a_masked_cache(ops, tq, tk, h, hkv, dh, dtype):
+    """New tokens against a cache of which keys are masked (left-padded prompts, dropped entries) and hold anything."""
+    n = 5
+    q, k, v, lam, dout = make(n, tq, tk, h, hkv, dh, dtype, 3)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    kmask = torch.rand(n, tk, device="cuda", generator=g) < 0.7
+    kmask[1] = torch.arange(tk, device="cuda") >= tk // 2 + 3  # left padding
+    kmask[2] = False
+    kmask[2, [0, tk // 2]] = True
+    kmask[3] = False
+    klen = torch.tensor([tk, tk - 1, tk, tk, tk // 2 + 1], dtype=torch.int32, device="cuda")
+    hidden = (torch.arange(tk, device="cuda")[None] >= klen[:, None]) | ~kmask
+    k.masked_fill_(hidden[:, :, None, None], math.nan)
+    v.masked_fill_(hidden[:, :, None, None], math.inf)
+    want = reference(q, k, v, lam, dout, dh ** -0.5, "end", klen, kmask)[0]
+    o = ops.diffattn_forward(q, k, v, lam, causal="end", klen=klen, kmask=kmask)
+    assert bool((o[3] == 0).all())
+    for b in (0, 1, 2, 4):
+        assert rel(o[b], want[b]) < TOL[dtype], (b, rel(o[b], want[b]))
+
+
 def test_nearly_equal_maps_over_a_long_cache(ops):
     """What is left of the difference keeps the type's precision when the keys are split too."""
     q, k, v, _, dout = make(1, 130, 3000, 2, 2, 32, BF16, 9)
