@@ -1228,6 +1228,7 @@ bool aligned(std::initializer_list<const void*> ps, size_t bytes) {
 int join_parts(rnn_ctx* ctx, const Args& a) { return join_launch<__nv_bfloat16, 128>(ctx, a); }
 int join_rows_bf16(rnn_ctx* ctx, const Args& a) { return join_rows_launch<__nv_bfloat16, 128>(ctx, a); }
 int join_rows_f32(rnn_ctx* ctx, const Args& a) { return join_rows_launch<float, 64>(ctx, a); }
+int join_rows_f32_wide(rnn_ctx* ctx, const Args& a) { return join_rows_launch<float, 128>(ctx, a); }
 
 }  // namespace diff
 }  // namespace rnn

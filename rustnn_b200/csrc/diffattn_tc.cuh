@@ -275,6 +275,7 @@ int f32_tc_bwd(rnn_ctx* ctx, const Args& a);
 // Joins parts of many rows: 128 columns in bf16, 64 in f32.
 int join_rows_bf16(rnn_ctx* ctx, const Args& a);
 int join_rows_f32(rnn_ctx* ctx, const Args& a);
+int join_rows_f32_wide(rnn_ctx* ctx, const Args& a);  // 128
 
 }  // namespace diff
 }  // namespace rnn

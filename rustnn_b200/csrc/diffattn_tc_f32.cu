@@ -56,6 +56,10 @@ struct Shared {
   int least[BWD_STAGES][2];                     // least limit of 32 of them
 };
 constexpr size_t FWD_SMEM = 1024 + ROW_TILE + FWD_STAGES * 2 * COL_TILE + sizeof(Shared);
+constexpr size_t FWD_WIDE_SMEM = 1024 + 2 * ROW_TILE + 3 * COL_TILE + sizeof(Shared);
+constexpr size_t GRAD_SMEM = 1024 + 3 * ROW_TILE + 3 * COL_TILE + sizeof(Shared);
+constexpr size_t DV_SMEM = 1024 + 2 * ROW_TILE + 4 * COL_TILE + sizeof(Shared);
+static_assert(GRAD_SMEM <= 232448, "fits an SM");
 constexpr size_t BWD_SMEM = 1024 + 2 * ROW_TILE + BWD_STAGES * 2 * COL_TILE + sizeof(Shared);
 
 struct Params {
@@ -187,6 +191,77 @@ __device__ __forceinline__ bool load_step(uint8_t* dst, const Args& a, int t, Fi
         load8<false, false>(x, second(r), i & 7, a.dh);
       }
       store8<COLS>(dst + (i < ITEMS ? 0 : COL_TILE), x, r, i & 7);
+    }
+  }
+  return true;
+}
+
+// Halves of more than 32 columns take tiles of their own, 64 columns each:
+// chunk c of a tile's row at p, `in` of whose columns exist.
+template <bool VEC>
+__device__ __forceinline__ void load8_wide(float (&x)[8], const float* p, int c, int in) {
+  in = p == nullptr ? 0 : in - c * 8;
+  p += c * 8;
+  if (VEC) {
+    float4 u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v = u;
+    if (in >= 4) u = __ldg(reinterpret_cast<const float4*>(p));
+    if (in >= 8) v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+    x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = k < in ? __ldg(p + k) : 0.0f;
+  }
+}
+// One tile of the block's own rows; row(u) is where the thread's row u starts.
+template <class Row>
+__device__ __forceinline__ void own_wide(uint8_t* dst, const Args& a, int t, int in, float scale, Row row) {
+  auto put = [&](float (&v)[8], int u) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] *= scale;
+    store8<ROWS>(dst, v, own_row(t, u), t & 7);
+  };
+  if (a.vec) {
+    float v[OWN][8];
+#pragma unroll
+    for (int u = 0; u < OWN; u++) load8_wide<true>(v[u], row(u), t & 7, in);
+#pragma unroll
+    for (int u = 0; u < OWN; u++) put(v[u], u);
+  } else {
+#pragma unroll 1
+    for (int u = 0; u < OWN; u++) {
+      float v[8];
+      load8_wide<false>(v, row(u), t & 7, in);
+      put(v, u);
+    }
+  }
+}
+// TILES tiles of a step, as load_step: src(i, r) is where row r of tile i
+// starts, in(i) how many of its columns exist.
+template <int TILES, class Src, class In, class Ready>
+__device__ __forceinline__ bool step_wide(uint8_t* dst, const Args& a, int t, Src src, In in, Ready ready) {
+  constexpr int ITEMS = COLS * 8, N = (TILES * ITEMS + LOADERS - 1) / LOADERS;
+  if (a.vec) {
+    float x[N][8];
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      const int i = t + u * LOADERS, tile = i / ITEMS, r = (i & (ITEMS - 1)) >> 3;
+      if (i < TILES * ITEMS) load8_wide<true>(x[u], src(tile, r), i & 7, in(tile));
+    }
+    if (!ready()) return false;
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+      const int i = t + u * LOADERS, tile = i / ITEMS, r = (i & (ITEMS - 1)) >> 3;
+      if (i < TILES * ITEMS) store8<COLS>(dst + tile * COL_TILE, x[u], r, i & 7);
+    }
+  } else {
+    if (!ready()) return false;
+#pragma unroll 1
+    for (int i = t; i < TILES * ITEMS; i += LOADERS) {
+      const int tile = i / ITEMS, r = (i & (ITEMS - 1)) >> 3;
+      float x[8];
+      load8_wide<false>(x, src(tile, r), i & 7, in(tile));
+      store8<COLS>(dst + tile * COL_TILE, x, r, i & 7);
     }
   }
   return true;
@@ -340,8 +415,9 @@ __device__ __forceinline__ void signal(uint64_t* bar) {
 }
 
 // Loads tiles of keys [kbeg, kend) for the kernels that own query rows.
+template <bool WIDE>
 __device__ __forceinline__ void load_keys(Block& blk, uint8_t* stages, int nstage, const Args& a, int b, int kvh,
-                                          int kbeg, int kend, int nt, int t0) {
+                                          int kbeg, int kend, int nt, int t0, int col0) {
   const float* kp = static_cast<const float*>(a.k) + b * a.kb + kvh * a.kh;
   const float* vp = static_cast<const float*>(a.v) + b * a.vb + kvh * a.vh;
   const uint8_t* mask = a.kmask ? a.kmask + b * a.kmb : nullptr;
@@ -349,22 +425,41 @@ __device__ __forceinline__ void load_keys(Block& blk, uint8_t* stages, int nstag
     const int st = t % nstage, j0 = kbeg + t * COLS;
     auto on = [&](int r) { return j0 + r < kend && (!mask || mask[j0 + r]); };
     const uint32_t bits = __ballot_sync(0xffffffffu, t0 < COLS && on(t0));
-    if (!load_step(stages + st * (2 * COL_TILE), a, t0, [&](int r) { return on(r) ? kp + (j0 + r) * a.kr : nullptr; },
-                   [&](int r) { return on(r) ? vp + (j0 + r) * a.vr : nullptr; },
-                   [&] { return t < nstage || blk.done(&blk.sh.empty[st], (t / nstage - 1) & 1); }))
-      break;
+    auto ready = [&] { return t < nstage || blk.done(&blk.sh.empty[st], (t / nstage - 1) & 1); };
+    bool ok;
+    if constexpr (WIDE) {  // both halves of k, 64 columns of v
+      ok = step_wide<3>(stages + st * (3 * COL_TILE), a, t0,
+                        [&](int i, int r) -> const float* {
+                          if (!on(r)) return nullptr;
+                          return i < 2 ? kp + (j0 + r) * a.kr + i * a.dh : vp + (j0 + r) * a.vr + col0;
+                        },
+                        [&](int i) { return i < 2 ? a.dh : 2 * a.dh - col0; }, ready);
+    } else {
+      ok = load_step(stages + st * (2 * COL_TILE), a, t0, [&](int r) { return on(r) ? kp + (j0 + r) * a.kr : nullptr; },
+                     [&](int r) { return on(r) ? vp + (j0 + r) * a.vr : nullptr; }, ready);
+    }
+    if (!ok) break;
     if (t0 < COLS && (t0 & 31) == 0) blk.sh.seen[st][t0 >> 5] = bits;
     fence_async_smem();
     signal(&blk.sh.full[st]);
   }
 }
 
+// WIDE: halves of 33 to 64 columns.  q and k take two tiles each, and a block
+// computes 64 of the value columns (blockIdx.z), the scores of both twice: there
+// is no room for more, in shared memory or in registers.
+template <bool WIDE>
 __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw[];
   const Args& a = p.a;
   uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-  uint8_t* stages = base + ROW_TILE;
-  Shared& sh = *reinterpret_cast<Shared*>(stages + FWD_STAGES * 2 * COL_TILE);
+  constexpr int STG = WIDE ? 1 : FWD_STAGES;
+  constexpr uint32_t STAGE = (WIDE ? 3 : 2) * COL_TILE, V_AT = WIDE ? 2 * COL_TILE : COL_TILE;
+  constexpr uint32_t Q_HALF = WIDE ? ROW_TILE : 64, K_HALF = WIDE ? COL_TILE : 64;  // bytes from one half to the other
+  constexpr int PART_W = WIDE ? 128 : 64;
+  uint8_t* stages = base + (WIDE ? 2 : 1) * ROW_TILE;
+  Shared& sh = *reinterpret_cast<Shared*>(stages + STG * STAGE);
+  const int col0 = WIDE ? blockIdx.z * 64 : 0;  // first value column
   Block blk{sh, p.dev_error};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rows = a.grp * a.tq, nbh = a.n * a.hkv, ntile = (rows + ROWS - 1) / ROWS;
@@ -386,7 +481,17 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
     if (nt > 0) {
       const float* q = static_cast<const float*>(a.q) + b * a.qb + static_cast<long long>(kvh) * a.grp * a.qh;
       auto at_q = [&](int u) { return packed(q, a, row0 + own_row(tid, u), rows, a.qr, a.qh); };
-      load_own<false>(base, a, tid, a.slog2, at_q, at_q);  // in units that make scores exponents of 2
+      // in units that make scores exponents of 2
+      if (WIDE) {
+#pragma unroll 1
+        for (int m = 0; m < 2; m++)
+          own_wide(base + m * ROW_TILE, a, tid, a.dh, a.slog2, [&](int u) {
+            const float* x = at_q(u);
+            return x ? x + m * a.dh : x;
+          });
+      } else {
+        load_own<false>(base, a, tid, a.slog2, at_q, at_q);
+      }
       fence_async_smem();
       signal(&sh.rows_full);
     }
@@ -403,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
     bool ok = true;
     for (int t = 0; t < nt; t++) {
       // the tile's visible keys come from the loading warps, its scores from the MMAs
-      if (!(ok = blk.done(&sh.full[t % FWD_STAGES], (t / FWD_STAGES) & 1) && blk.done(&sh.s_full, t & 1))) break;
+      if (!(ok = blk.done(&sh.full[t % STG], (t / STG) & 1) && blk.done(&sh.s_full, t & 1))) break;
       tc_fence_after();
       float s1[32], s2[32];
       tmem_ld(at + part * 32, s1);
@@ -411,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
       tmem_landed(s1);
       tmem_landed(s2);
       const int j0 = kbeg + t * COLS + part * 32;
-      const uint32_t seen = sh.seen[t % FWD_STAGES][part];
+      const uint32_t seen = sh.seen[t % STG][part];
       tc_fence_before();
       signal(&sh.s_free);
       const bool edge = j0 + 32 > full || seen != 0xffffffffu;
@@ -457,10 +562,10 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
       float* patch = reinterpret_cast<float*>(base) + warp * 1024;  // q is no longer read
       if (a.nsplit > 1) {
         const long long to = (static_cast<long long>(blockIdx.y) * nbh + bh) * rows + r;
-        float* q = r < rows ? a.part + to * 128 + part * 32 : nullptr;
+        float* q = r < rows ? a.part + to * (2 * PART_W) + col0 + part * 32 : nullptr;
         store_rows(patch, x, 32, true, q);
-        store_rows(patch, y, 32, true, q ? q + 64 : nullptr);
-        if (part == 0 && r < rows) *reinterpret_cast<float4*>(a.stat + to * 4) = make_float4(m1, L1, m2, L2);
+        store_rows(patch, y, 32, true, q ? q + PART_W : nullptr);
+        if (part == 0 && col0 == 0 && r < rows) *reinterpret_cast<float4*>(a.stat + to * 4) = make_float4(m1, L1, m2, L2);
       } else {
         const bool any = L1 > 0.0f && L2 > 0.0f;
         const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f;
@@ -470,15 +575,15 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
           y[c] = any ? y[c] * i2 : 0.0f;
           x[c] = any ? x[c] * i1 - lam * y[c] : 0.0f;
         }
-        const int in = 2 * a.dh - part * 32;
+        const int in = 2 * a.dh - col0 - part * 32;
         store_rows(patch, x, in, p.st16,
-                   r < rows ? static_cast<float*>(a.o) + b * a.ob + head * a.oh + i * a.orow + part * 32 : nullptr);
+                   r < rows ? static_cast<float*>(a.o) + b * a.ob + head * a.oh + i * a.orow + col0 + part * 32 : nullptr);
         if (a.o2)
           store_rows(patch, y, in, p.st16_2,
                      r < rows ? static_cast<float*>(a.o2) +
-                                    ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + part * 32
+                                    ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + col0 + part * 32
                               : nullptr);
-        if (a.lse && part == 0 && r < rows) {
+        if (a.lse && part == 0 && col0 == 0 && r < rows) {
           float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
           s[0] = any ? m1 + log2f(L1) : CUDART_INF_F;
           s[a.tq] = any ? m2 + log2f(L2) : CUDART_INF_F;
@@ -489,42 +594,49 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < WARP_MMA) {
       const int t0 = tid - MATH_WARPS * 32;
-      if (nt > 0) load_keys(blk, stages, FWD_STAGES, a, b, kvh, kbeg, kend, nt, t0);
+      if (nt > 0) load_keys<WIDE>(blk, stages, STG, a, b, kvh, kbeg, kend, nt, t0, col0);
     } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
       const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_o = idesc_bf16(ROWS, 64, true);
       const uint64_t dq = desc_k(smem_u32(base)), dk = desc_k(smem_u32(stages));
-      const uint64_t dv = desc_mn(smem_u32(stages) + COL_TILE, 0);
+      const uint64_t dv = desc_mn(smem_u32(stages) + V_AT, 0);
       const int ksteps = (a.dh + 15) / 16;
       bool ok = blk.done(&sh.rows_full, 0);
-      for (int t = 0; ok && t <= nt; t++) {
-        if (t < nt) {
-          const int st = t % FWD_STAGES;
-          if (!(ok = blk.done(&sh.full[st], (t / FWD_STAGES) & 1) && (t == 0 || blk.done(&sh.s_free, (t - 1) & 1)))) break;
-          tc_fence_after();
-          const uint64_t k = dk + st * (2 * COL_TILE / 16);
+      auto scores = [&](int t) {
+        const int st = t % STG;
+        if (!blk.done(&sh.full[st], (t / STG) & 1) || (t > 0 && !blk.done(&sh.s_free, (t - 1) & 1))) return false;
+        tc_fence_after();
+        const uint64_t k = dk + st * (STAGE / 16);
 #pragma unroll
-          for (int m = 0; m < 2; m++)
-            products<2>(ksteps, [&](int pa, int pb, int ks, bool acc) {
-              mma_ss(tmem + m * 64, dq + (pa * ROW_PLANE + m * 64 + ks * 32) / 16,
-                     k + (pb * COL_PLANE + m * 64 + ks * 32) / 16, id_s, acc, lead);
-            });
-          commit(&sh.s_full, lead);
-        }
-        if (t > 0) {
-          const int st = (t - 1) % FWD_STAGES;
-          if (!(ok = blk.done(&sh.p_full, (t - 1) & 1))) break;
-          tc_fence_after();
-          const uint64_t v = dv + st * (2 * COL_TILE / 16);
+        for (int m = 0; m < 2; m++)
+          products<WIDE ? 4 : 2>(ksteps, [&](int pa, int pb, int ks, bool acc) {
+            mma_ss(tmem + m * 64, dq + (pa * ROW_PLANE + m * Q_HALF + ks * 32) / 16,
+                   k + (pb * COL_PLANE + m * K_HALF + ks * 32) / 16, id_s, acc, lead);
+          });
+        commit(&sh.s_full, lead);
+        return true;
+      };
+      auto values = [&](int t) {
+        const int st = t % STG;
+        if (!blk.done(&sh.p_full, t & 1)) return false;
+        tc_fence_after();
+        const uint64_t v = dv + st * (STAGE / 16);
 #pragma unroll
-          for (int m = 0; m < 2; m++)
-            products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
-              mma_ts(tmem + FWD_O + m * 64, tmem + FWD_P + m * MAP + plane_at(pa, ks),
-                     v + (pb * COL_PLANE + ks * 2048) / 16, id_o, acc, lead);
-            });
-          commit(&sh.empty[st], lead);
-          commit(&sh.o_full, lead);
-        }
+        for (int m = 0; m < 2; m++)
+          products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+            mma_ts(tmem + FWD_O + m * 64, tmem + FWD_P + m * MAP + plane_at(pa, ks),
+                   v + (pb * COL_PLANE + ks * 2048) / 16, id_o, acc, lead);
+          });
+        commit(&sh.empty[st], lead);
+        commit(&sh.o_full, lead);
+        return true;
+      };
+      ok = ok && scores(0);
+      for (int t = 0; ok && t < nt; t++) {
+        // the next scores run under this tile's exponentials, if a stage holds their tile
+        if (STG > 1 && t + 1 < nt && !(ok = scores(t + 1))) break;
+        if (!(ok = values(t))) break;
+        if (STG == 1 && t + 1 < nt) ok = scores(t + 1);
       }
       if (!ok) {  // no MMA may write tensor memory after it is released
         commit(&sh.drain, lead);
@@ -723,7 +835,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_q_kernel(const __grid_cons
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < WARP_MMA) {
-      if (nt > 0) load_keys(blk, stages, BWD_STAGES, a, b, kvh, 0, kend, nt, tid - MATH_WARPS * 32);
+      if (nt > 0) load_keys<false>(blk, stages, BWD_STAGES, a, b, kvh, 0, kend, nt, tid - MATH_WARPS * 32, 0);
     } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
       const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_o = idesc_bf16(ROWS, 32, true);
@@ -1008,6 +1120,482 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
   if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
 }
 
+// Halves of more than 32 columns: the rows of a block with all they meet do not
+// fit an SM, so each block takes one map (blockIdx.y): dq_m of 128 packed query
+// rows, or dk_m of 128 keys,
+//   S_m = X x^T,  dP = Y y^T,  dS_m = P_m (dP - D_m),  dX = dS_m x,
+// with X, x = q_m, k_m and Y, y = do, v for queries and the other way round for
+// keys.  dP is formed twice that way, and dv has a kernel of its own; one stage
+// of tiles fits beside the rows.  Measured: @GRAD@
+constexpr uint32_t G_DP = 64, G_P = 128, G_O = G_P + MAP;
+
+template <bool KEYS>
+__global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  const Args& a = p.a;
+  uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* stage = base + 3 * ROW_TILE;
+  Shared& sh = *reinterpret_cast<Shared*>(stage + 3 * COL_TILE);
+  Block blk{sh, p.dev_error};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m = blockIdx.y;
+  const int rows = KEYS ? a.tk : a.grp * a.tq, nbh = a.n * a.hkv, ntile = (rows + ROWS - 1) / ROWS;
+  const bool work = static_cast<int>(blockIdx.x) < ntile * nbh;  // else a block for dlam only
+  // what takes longest first: late queries, early keys
+  const int order = work ? static_cast<int>(blockIdx.x) / nbh : 0, tile = KEYS ? order : ntile - 1 - order;
+  const int bh = static_cast<int>(blockIdx.x) % nbh, b = bh / a.hkv, kvh = bh - b * a.hkv;
+  const int row0 = tile * ROWS, len = key_len(a, b);
+  const uint8_t* mask = a.kmask ? a.kmask + b * a.kmb : nullptr;
+  const long long h0 = static_cast<long long>(kvh) * a.grp;
+  const float* qp = static_cast<const float*>(a.q) + b * a.qb + h0 * a.qh;
+  const float* gp = static_cast<const float*>(a.dout) + b * a.gb + h0 * a.gh;
+  const float* kp = static_cast<const float*>(a.k) + b * a.kb + kvh * a.kh;
+  const float* vp = static_cast<const float*>(a.v) + b * a.vb + kvh * a.vh;
+  int kend = 0, qbeg = 0, per = 0, nt;
+  if (KEYS) {
+    // queries before `qbeg` see none of these keys
+    if (!work || row0 >= len) {
+      qbeg = a.tq;
+    } else if (a.causal == RNN_CAUSAL_START) {
+      qbeg = min(a.tq, row0);
+    } else if (a.causal == RNN_CAUSAL_END) {
+      qbeg = min(a.tq, max(0, row0 - (len - a.tq)));
+    }
+    per = (a.tq - qbeg + COLS - 1) / COLS;
+    nt = per * a.grp;
+  } else {
+    const int last = min(rows, row0 + ROWS) - 1;
+    const int imax = last / a.tq != row0 / a.tq ? a.tq - 1 : last % a.tq;
+    kend = row_limit(a, imax, len);
+    nt = (kend + COLS - 1) / COLS;
+  }
+  setup(sh, warp);
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < MATH_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    // the place of packed query row r in a tensor of the queries
+    auto query = [&](const float* x, long long sr, long long sh_, int r) { return packed(x, a, r, rows, sr, sh_); };
+    auto key_row = [&](const float* x, long long sr, int j) {
+      return j < len && (!mask || mask[j]) ? x + j * sr : static_cast<const float*>(nullptr);
+    };
+    if (nt > 0) {
+#pragma unroll 1
+      for (int i = 0; i < 3; i++) {
+        const int col = i == 0 ? m * a.dh : (i - 1) * 64, in = i == 0 ? a.dh : 2 * a.dh - col;
+        own_wide(base + i * ROW_TILE, a, tid, in, i == 0 ? a.slog2 : 1.0f, [&](int u) {
+          const int r = row0 + own_row(tid, u);
+          const float* x = KEYS ? (i == 0 ? key_row(kp, a.kr, r) : key_row(vp, a.vr, r))
+                                : (i == 0 ? query(qp, a.qr, a.qh, r) : query(gp, a.gr, a.gh, r));
+          return x ? x + col : x;
+        });
+      }
+      fence_async_smem();
+      signal(&sh.rows_full);
+      // D_m, from do . o and do . o2; rows that see one tile of keys sum P dP
+      if (!KEYS && nt > 1) {
+        const float* o = static_cast<const float*>(a.fo) + b * a.ob + h0 * a.oh;
+        const float* o2 = static_cast<const float*>(a.fo2) + (static_cast<long long>(b) * a.tq * a.h + h0) * (2 * a.dh);
+        auto sums = [&](int u, auto vec) {
+          constexpr bool VEC = decltype(vec)::value;
+          const int r = row0 + own_row(tid, u), c = tid & 7, e = min(r, rows - 1) / a.tq;
+          const float lam = m ? 1.0f : __ldg(a.lam + h0 + e);
+          const float *pg = query(gp, a.gr, a.gh, r), *po = query(o, a.orow, a.oh, r);
+          const float* py = query(o2, static_cast<long long>(a.h) * 2 * a.dh, 2 * a.dh, r);
+          float d = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const int in = 2 * a.dh - i * 64;
+            float x[8], y[8], z[8];
+            load8_wide<VEC>(x, pg ? pg + i * 64 : pg, c, in);
+            load8_wide<VEC>(y, m || !po ? nullptr : po + i * 64, c, in);
+            load8_wide<VEC>(z, py ? py + i * 64 : py, c, in);
+#pragma unroll
+            for (int k = 0; k < 8; k++) d += x[k] * (y[k] + lam * z[k]);
+          }
+#pragma unroll
+          for (int k = 1; k < 8; k <<= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
+          if (c == 0) sh.d[r - row0].x = d;
+        };
+        if (p.ld16) {
+#pragma unroll 2
+          for (int u = 0; u < OWN; u++) sums(u, std::true_type());
+        } else {
+#pragma unroll 1
+          for (int u = 0; u < OWN; u++) sums(u, std::false_type());
+        }
+        signal(&sh.d_full);
+      }
+    }
+    const int part = warp >> 2, w = warp & 3, row = w * 32 + lane, r = row0 + row;
+    const uint32_t at = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    // query rows
+    const int e = KEYS ? 0 : min(r, rows - 1) / a.tq, i = r - e * a.tq, head = static_cast<int>(h0) + e;
+    const int lim = !KEYS && r < rows ? min(kend, row_limit(a, i, len)) : 0;
+    const int full = __reduce_min_sync(0xffffffffu, lim);
+    float ls = CUDART_INF_F, d = 0.0f, dl = 0.0f, pl = 0.0f;
+    if (!KEYS && r < rows) ls = a.flse[((static_cast<long long>(b) * a.h + head) * 2 + m) * a.tq + i];
+    // keys: what a query has to see for this key to count
+    const int need = KEYS && r < len && (!mask || mask[r]) ? r : 0x7fffffff;
+    const int most = __reduce_max_sync(0xffffffffu, need);
+    int turn = 0;
+    bool ok = true;
+    if (!KEYS && nt > 1) {
+      ok = blk.done(&sh.d_full, 0);
+      if (ok && r < rows) d = sh.d[row].x;
+    }
+    float acc[32];
+#pragma unroll
+    for (int c = 0; c < 32; c++) acc[c] = 0.0f;
+    for (int t = 0; ok && t < nt; t++) {
+      if (!(ok = blk.done(&sh.full[0], t & 1) && blk.done(&sh.s_full, t & 1))) break;
+      tc_fence_after();
+      float s[32], dp[32];
+      tmem_ld(at + part * 32, s);
+      tmem_landed(s);
+      const float* stat = &sh.stat[0][0][part * 32];
+      if (KEYS) {
+        if (most >= sh.least[0][part]) {
+#pragma unroll
+          for (int c = 0; c < 32; c++)
+            if (need >= __float_as_int(stat[4 * COLS + c])) s[c] = -CUDART_INF_F;
+        }
+        const float f = m ? -__ldg(a.lam + h0 + t / per) : 1.0f;
+        const f32x2 ff = pair(f, f);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          float u, v;
+          unpair(add2(pair(s[c], s[c + 1]), *reinterpret_cast<const f32x2*>(stat + c)), u, v);
+          unpair(mul2(pair(ex2(u), ex2(v)), ff), s[c], s[c + 1]);
+        }
+      } else {
+        const int j0 = t * COLS + part * 32;
+        const uint32_t seen = sh.seen[0][part];
+        if (j0 + 32 > full || seen != 0xffffffffu) {
+#pragma unroll
+          for (int c = 0; c < 32; c++)
+            if (j0 + c >= lim || !(seen >> c & 1)) s[c] = -CUDART_INF_F;
+        }
+        pl += exp_sum(s, ls);
+      }
+      if (!(ok = blk.done(&sh.dp_full, t & 1))) break;
+      tc_fence_after();
+      tmem_ld(at + G_DP + part * 32, dp);
+      tmem_landed(dp);
+      if (KEYS) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 2)
+          unpair(mul2(pair(s[c], s[c + 1]),
+                      add2(pair(dp[c], dp[c + 1]), *reinterpret_cast<const f32x2*>(stat + 2 * COLS + c))),
+                 s[c], s[c + 1]);
+      } else {
+        const float now = dot_row(s, dp);
+        dl += now;
+        if (nt == 1) {
+          float2 other;
+          if (!(ok = blk.exchange(turn, w, part, row, make_float2(now, 0.0f), other))) break;
+          d = now + other.x;
+        }
+        times_rest(s, dp, d);
+      }
+      if (t > 0) {
+        if (!(ok = blk.done(&sh.o_full, (t - 1) & 1))) break;
+        tc_fence_after();
+        add_tmem(at + G_O + part * 32, acc, 1.0f);
+      }
+      store_planes(at + G_P + part * PART, s);
+      tmem_wait_st();
+      tc_fence_before();
+      signal(&sh.p_full);
+    }
+    if (ok && nt > 0 && (ok = blk.done(&sh.o_full, (nt - 1) & 1))) {
+      tc_fence_after();
+      add_tmem(at + G_O + part * 32, acc, 1.0f);
+    }
+    float* patch = reinterpret_cast<float*>(base) + warp * 1024;  // the rows are no longer read
+    const int in = a.dh - part * 32;
+    if (KEYS) {
+#pragma unroll
+      for (int c = 0; c < 32; c++) acc[c] *= a.scale;
+      if (ok && work)
+        store_rows(patch, acc, in, p.st16,
+                   r < rows ? static_cast<float*>(a.dk) + b * a.dkb + kvh * a.dkh + r * a.dkr + m * a.dh + part * 32
+                            : nullptr);
+    } else {
+      float2 other;
+      if (ok && blk.exchange(turn, w, part, row, make_float2(dl, pl), other)) {
+        if (part == 0 && r < rows) {
+          // over the map's own sum: what the log-sum's rounding does to a whole row cancels
+          const float whole = pl + other.y;
+          a.dsum[((static_cast<long long>(b) * a.h + head) * 2 + m) * a.tq + i] = d;
+          if (m)
+            a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
+                whole > 0.0f ? (dl + other.x) / whole : 0.0f;
+        }
+        const float f = m ? -a.scale * __ldg(a.lam + head) : a.scale;
+#pragma unroll
+        for (int c = 0; c < 32; c++) acc[c] *= f;
+        store_rows(patch, acc, in, p.st16,
+                   r < rows ? static_cast<float*>(a.dq) + b * a.dqb + head * a.dqh + i * a.dqr + m * a.dh + part * 32
+                            : nullptr);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < WARP_MMA) {
+      const int t0 = tid - MATH_WARPS * 32;
+      for (int t = 0; t < nt; t++) {
+        auto ready = [&] { return t == 0 || blk.done(&sh.empty[0], (t - 1) & 1); };
+        auto in = [&](int i) { return i == 0 ? a.dh : 2 * a.dh - (i - 1) * 64; };
+        if (KEYS) {
+          const int e = t / per, i0 = qbeg + (t - e * per) * COLS, i = i0 + t0;
+          const bool on = t0 < COLS && i < a.tq;
+          const long long from = ((static_cast<long long>(b) * a.h + h0 + e) * 2 + m) * a.tq + i;
+          const float l = on ? a.flse[from] : CUDART_INF_F, d = on ? a.dsum[from] : 0.0f;
+          const int lim = on ? row_limit(a, i, len) : 0;
+          if (!step_wide<3>(stage, a, t0,
+                            [&](int k, int r) -> const float* {
+                              if (i0 + r >= a.tq) return nullptr;
+                              return k == 0 ? qp + e * a.qh + (i0 + r) * a.qr + m * a.dh
+                                            : gp + e * a.gh + (i0 + r) * a.gr + (k - 1) * 64;
+                            },
+                            in, ready))
+            break;
+          if (t0 < COLS) {
+            sh.stat[0][0][t0] = -l;
+            sh.stat[0][2][t0] = -d;
+            sh.stat[0][4][t0] = __int_as_float(lim);
+            const int least = __reduce_min_sync(0xffffffffu, lim);
+            if ((t0 & 31) == 0) sh.least[0][t0 >> 5] = least;
+          }
+        } else {
+          const int j0 = t * COLS;
+          auto on = [&](int r) { return j0 + r < kend && (!mask || mask[j0 + r]); };
+          const uint32_t bits = __ballot_sync(0xffffffffu, t0 < COLS && on(t0));
+          if (!step_wide<3>(stage, a, t0,
+                            [&](int k, int r) -> const float* {
+                              if (!on(r)) return nullptr;
+                              return k == 0 ? kp + (j0 + r) * a.kr + m * a.dh : vp + (j0 + r) * a.vr + (k - 1) * 64;
+                            },
+                            in, ready))
+            break;
+          if (t0 < COLS && (t0 & 31) == 0) sh.seen[0][t0 >> 5] = bits;
+        }
+        fence_async_smem();
+        signal(&sh.full[0]);
+      }
+      // dlam: block `head` sums that head's rows in a fixed order
+      if (KEYS && m == 0 && warp == MATH_WARPS && static_cast<int>(blockIdx.x) < a.h && a.tq > 0) {
+        const long long cnt = static_cast<long long>(a.n) * a.tq;
+        const float* x = a.dlrow + blockIdx.x * cnt;
+        double sum = 0.0;
+#pragma unroll 8
+        for (long long i = lane; i < cnt; i += 32) sum += x[i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) a.dlam[blockIdx.x] -= static_cast<float>(sum);
+      }
+    } else if (nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_o = idesc_bf16(ROWS, 64, true);
+      const uint64_t dx = desc_k(smem_u32(base)), dy = desc_k(smem_u32(base) + ROW_TILE);
+      const uint64_t cx = desc_k(smem_u32(stage)), cy = desc_k(smem_u32(stage) + COL_TILE);
+      const uint64_t cn = desc_mn(smem_u32(stage), 0);
+      const int ksteps = (a.dh + 15) / 16, vsteps = (2 * a.dh + 15) / 16;
+      bool ok = blk.done(&sh.rows_full, 0);
+      for (int t = 0; ok && t < nt; t++) {
+        if (!(ok = blk.done(&sh.full[0], t & 1))) break;
+        tc_fence_after();
+        products<4>(ksteps, [&](int pa, int pb, int ks, bool acc) {
+          mma_ss(tmem, dx + (pa * ROW_PLANE + ks * 32) / 16, cx + (pb * COL_PLANE + ks * 32) / 16, id_s, acc, lead);
+        });
+        commit(&sh.s_full, lead);
+        products<8>(vsteps, [&](int pa, int pb, int ks, bool acc) {
+          mma_ss(tmem + G_DP, dy + ((ks >> 2) * ROW_TILE + pa * ROW_PLANE + (ks & 3) * 32) / 16,
+                 cy + ((ks >> 2) * COL_TILE + pb * COL_PLANE + (ks & 3) * 32) / 16, id_s, acc, lead);
+        });
+        commit(&sh.dp_full, lead);
+        if (!(ok = blk.done(&sh.p_full, t & 1))) break;
+        tc_fence_after();
+        products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+          mma_ts(tmem + G_O, tmem + G_P + plane_at(pa, ks), cn + (pb * COL_PLANE + ks * 2048) / 16, id_o, acc, lead);
+        });
+        commit(&sh.empty[0], lead);
+        commit(&sh.o_full, lead);
+      }
+      if (!ok) {
+        commit(&sh.drain, lead);
+        settle(&sh.drain, 0);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+}
+
+// dv of 128 keys for halves of more than 32 columns: (P_1 - lam P_2)^T do.
+__global__ void __launch_bounds__(THREADS, 1) f32_dv_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t raw[];
+  const Args& a = p.a;
+  uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* stage = base + 2 * ROW_TILE;
+  Shared& sh = *reinterpret_cast<Shared*>(stage + 4 * COL_TILE);
+  Block blk{sh, p.dev_error};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nbh = a.n * a.hkv, key0 = static_cast<int>(blockIdx.x) / nbh * ROWS;
+  const int bh = static_cast<int>(blockIdx.x) % nbh, b = bh / a.hkv, kvh = bh - b * a.hkv;
+  const int len = key_len(a, b);
+  const uint8_t* mask = a.kmask ? a.kmask + b * a.kmb : nullptr;
+  int qbeg = 0;
+  if (key0 >= len) {
+    qbeg = a.tq;
+  } else if (a.causal == RNN_CAUSAL_START) {
+    qbeg = min(a.tq, key0);
+  } else if (a.causal == RNN_CAUSAL_END) {
+    qbeg = min(a.tq, max(0, key0 - (len - a.tq)));
+  }
+  const int per = (a.tq - qbeg + COLS - 1) / COLS, nt = per * a.grp;
+  setup(sh, warp);
+  const uint32_t tmem = sh.tmem;
+
+  if (warp < MATH_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if (nt > 0) {
+      const float* kp = static_cast<const float*>(a.k) + b * a.kb + kvh * a.kh;
+#pragma unroll 1
+      for (int m = 0; m < 2; m++)
+        own_wide(base + m * ROW_TILE, a, tid, a.dh, a.slog2, [&](int u) {
+          const int j = key0 + own_row(tid, u);
+          return j < len && (!mask || mask[j]) ? kp + j * a.kr + m * a.dh : static_cast<const float*>(nullptr);
+        });
+      fence_async_smem();
+      signal(&sh.rows_full);
+    }
+    const int part = warp >> 2, w = warp & 3, row = w * 32 + lane, key = key0 + row;
+    const uint32_t at = tmem + (static_cast<uint32_t>(w * 32) << 16);
+    const int need = key < len && (!mask || mask[key]) ? key : 0x7fffffff;
+    const int most = __reduce_max_sync(0xffffffffu, need);
+    float v0[32], v1[32];
+#pragma unroll
+    for (int c = 0; c < 32; c++) v0[c] = v1[c] = 0.0f;
+    bool ok = true;
+    for (int t = 0; t < nt; t++) {
+      if (!(ok = blk.done(&sh.full[0], t & 1) && blk.done(&sh.s_full, t & 1))) break;
+      tc_fence_after();
+      float s1[32], s2[32];
+      tmem_ld(at + part * 32, s1);
+      tmem_ld(at + 64 + part * 32, s2);
+      tmem_landed(s1);
+      tmem_landed(s2);
+      const float* stat = &sh.stat[0][0][part * 32];
+      if (most >= sh.least[0][part]) {
+#pragma unroll
+        for (int c = 0; c < 32; c++)
+          if (need >= __float_as_int(stat[4 * COLS + c])) s1[c] = s2[c] = -CUDART_INF_F;
+      }
+      const float lam = __ldg(a.lam + kvh * a.grp + t / per);
+      const f32x2 ll = pair(-lam, -lam);
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        float x, y, u, v;
+        unpair(add2(pair(s1[c], s1[c + 1]), *reinterpret_cast<const f32x2*>(stat + c)), x, y);
+        unpair(add2(pair(s2[c], s2[c + 1]), *reinterpret_cast<const f32x2*>(stat + COLS + c)), u, v);
+        unpair(fma2(pair(ex2(u), ex2(v)), ll, pair(ex2(x), ex2(y))), s1[c], s1[c + 1]);
+      }
+      if (t > 0) {
+        if (!(ok = blk.done(&sh.o_full, (t - 1) & 1))) break;
+        tc_fence_after();
+        add_tmem(at + G_O + part * 32, v0, 1.0f);
+        add_tmem(at + G_O + 64 + part * 32, v1, 1.0f);
+      }
+      store_planes(at + G_P + part * PART, s1);
+      tmem_wait_st();
+      tc_fence_before();
+      signal(&sh.p_full);
+    }
+    if (ok && nt > 0 && (ok = blk.done(&sh.o_full, (nt - 1) & 1))) {
+      tc_fence_after();
+      add_tmem(at + G_O + part * 32, v0, 1.0f);
+      add_tmem(at + G_O + 64 + part * 32, v1, 1.0f);
+    }
+    if (ok) {
+      float* patch = reinterpret_cast<float*>(base) + warp * 1024;
+      float* to = key < a.tk ? static_cast<float*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr + part * 32 : nullptr;
+      store_rows(patch, v0, 2 * a.dh - part * 32, p.st16, to);
+      store_rows(patch, v1, 2 * a.dh - 64 - part * 32, p.st16, to ? to + 64 : nullptr);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < WARP_MMA) {
+      const int t0 = tid - MATH_WARPS * 32;
+      const float* qp = static_cast<const float*>(a.q) + b * a.qb + static_cast<long long>(kvh) * a.grp * a.qh;
+      const float* gp = static_cast<const float*>(a.dout) + b * a.gb + static_cast<long long>(kvh) * a.grp * a.gh;
+      for (int t = 0; t < nt; t++) {
+        const int e = t / per, i0 = qbeg + (t - e * per) * COLS, i = i0 + t0;
+        const bool on = t0 < COLS && i < a.tq;
+        const long long from = (static_cast<long long>(b) * a.h + kvh * a.grp + e) * 2 * a.tq + i;
+        const float l1 = on ? a.flse[from] : CUDART_INF_F, l2 = on ? a.flse[from + a.tq] : CUDART_INF_F;
+        const int lim = on ? row_limit(a, i, len) : 0;
+        if (!step_wide<2>(stage, a, t0,
+                          [&](int k, int r) { return i0 + r < a.tq ? qp + e * a.qh + (i0 + r) * a.qr + k * a.dh : nullptr; },
+                          [&](int) { return a.dh; }, [&] { return t == 0 || blk.done(&sh.empty[0], (t - 1) & 1); }))
+          break;
+        step_wide<2>(stage + 2 * COL_TILE, a, t0,
+                     [&](int k, int r) { return i0 + r < a.tq ? gp + e * a.gh + (i0 + r) * a.gr + k * 64 : nullptr; },
+                     [&](int k) { return 2 * a.dh - k * 64; }, [] { return true; });
+        if (t0 < COLS) {
+          sh.stat[0][0][t0] = -l1;
+          sh.stat[0][1][t0] = -l2;
+          sh.stat[0][4][t0] = __int_as_float(lim);
+          const int least = __reduce_min_sync(0xffffffffu, lim);
+          if ((t0 & 31) == 0) sh.least[0][t0 >> 5] = least;
+        }
+        fence_async_smem();
+        signal(&sh.full[0]);
+      }
+    } else if (nt > 0) {
+      const uint32_t lead = elect_one() ? 1u : 0u;
+      const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_o = idesc_bf16(ROWS, 64, true);
+      const uint64_t dk = desc_k(smem_u32(base)), cq = desc_k(smem_u32(stage));
+      const uint64_t cg = desc_mn(smem_u32(stage) + 2 * COL_TILE, 0);
+      const int ksteps = (a.dh + 15) / 16;
+      bool ok = blk.done(&sh.rows_full, 0);
+      for (int t = 0; ok && t < nt; t++) {
+        if (!(ok = blk.done(&sh.full[0], t & 1))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+          products<4>(ksteps, [&](int pa, int pb, int ks, bool acc) {
+            mma_ss(tmem + m * 64, dk + (m * ROW_TILE + pa * ROW_PLANE + ks * 32) / 16,
+                   cq + (m * COL_TILE + pb * COL_PLANE + ks * 32) / 16, id_s, acc, lead);
+          });
+        commit(&sh.s_full, lead);
+        if (!(ok = blk.done(&sh.p_full, t & 1))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+          products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
+            mma_ts(tmem + G_O + c * 64, tmem + G_P + plane_at(pa, ks),
+                   cg + (c * COL_TILE + pb * COL_PLANE + ks * 2048) / 16, id_o, acc, lead);
+          });
+        commit(&sh.empty[0], lead);
+        commit(&sh.o_full, lead);
+      }
+      if (!ok) {
+        commit(&sh.drain, lead);
+        settle(&sh.drain, 0);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == WARP_MMA) tmem_dealloc(tmem, 512);
+}
+
 }  // namespace
 
 // A block starts and ends in about 9 us beside 2 us a tile, more than the
@@ -1019,7 +1607,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
 // two stages of tiles beside the block's rows.
 bool f32_tc_ok(const Args& a) {
   const long long rows = static_cast<long long>(a.grp) * a.tq;
-  return a.dh <= 32 && rows >= 64 && rows * a.tk >= 64 * 128;
+  return rows >= 64 && rows * a.tk >= 64 * 128;
 }
 
 int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
@@ -1032,21 +1620,26 @@ int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
   const long long rows = static_cast<long long>(a.grp) * a.tq, nbh = static_cast<long long>(a.n) * a.hkv;
   const long long blocks = (rows + ROWS - 1) / ROWS * nbh;
   RNN_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  const bool wide = a.dh > 32;
   const int tiles = (a.tk + COLS - 1) / COLS;
-  const long long parts = std::max(1ll, std::min<long long>(ctx->num_sms / blocks, tiles / 4));
+  const long long parts = std::max(1ll, std::min<long long>(ctx->num_sms / (wide ? 2 * blocks : blocks), tiles / 4));
   p.a.split_keys = static_cast<int>((tiles + parts - 1) / parts) * COLS;
   p.a.nsplit = (a.tk + p.a.split_keys - 1) / p.a.split_keys;
   if (p.a.nsplit > 1) {
     const size_t all = static_cast<size_t>(p.a.nsplit) * nbh * rows;
-    RNN_TRY(ensure_ws(ctx, all * (128 + 4) * sizeof(float)));
+    const size_t width = wide ? 256 : 128;
+    RNN_TRY(ensure_ws(ctx, all * (width + 4) * sizeof(float)));
     p.a.part = static_cast<float*>(ctx->ws);
-    p.a.stat = p.a.part + all * 128;
+    p.a.stat = p.a.part + all * width;
   }
-  static std::atomic<unsigned long long> optin{0};
-  RNN_TRY(tc::ensure_smem_optin(f32_fwd_kernel, optin, ctx->device, static_cast<int>(FWD_SMEM)));
-  f32_fwd_kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit), THREADS, FWD_SMEM, ctx->stream>>>(p);
+  static std::atomic<unsigned long long> optin[2];
+  const auto kernel = wide ? f32_fwd_kernel<true> : f32_fwd_kernel<false>;
+  const size_t smem = wide ? FWD_WIDE_SMEM : FWD_SMEM;
+  RNN_TRY(tc::ensure_smem_optin(kernel, optin[wide], ctx->device, static_cast<int>(smem)));
+  kernel<<<dim3(static_cast<unsigned>(blocks), p.a.nsplit, wide ? 2 : 1), THREADS, smem, ctx->stream>>>(p);
   RNN_CHECK_LAUNCH();
-  return p.a.nsplit > 1 ? join_rows_f32(ctx, p.a) : RNN_OK;
+  if (p.a.nsplit == 1) return RNN_OK;
+  return wide ? join_rows_f32_wide(ctx, p.a) : join_rows_f32(ctx, p.a);
 }
 
 int f32_tc_bwd(rnn_ctx* ctx, const Args& a) {
@@ -1066,6 +1659,19 @@ int f32_tc_bwd(rnn_ctx* ctx, const Args& a) {
   const long long qblocks = (rows + ROWS - 1) / ROWS * nbh;
   const long long kblocks = std::max<long long>((a.tk + ROWS - 1ll) / ROWS * nbh, a.h);
   RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  if (a.dh > 32) {
+    static std::atomic<unsigned long long> optin_r{0}, optin_c{0}, optin_v{0};
+    RNN_TRY(tc::ensure_smem_optin(f32_grad_kernel<false>, optin_r, ctx->device, static_cast<int>(GRAD_SMEM)));
+    RNN_TRY(tc::ensure_smem_optin(f32_grad_kernel<true>, optin_c, ctx->device, static_cast<int>(GRAD_SMEM)));
+    RNN_TRY(tc::ensure_smem_optin(f32_dv_kernel, optin_v, ctx->device, static_cast<int>(DV_SMEM)));
+    f32_grad_kernel<false><<<dim3(static_cast<unsigned>(qblocks), 2), THREADS, GRAD_SMEM, ctx->stream>>>(p);
+    RNN_CHECK_LAUNCH();
+    f32_grad_kernel<true><<<dim3(static_cast<unsigned>(kblocks), 2), THREADS, GRAD_SMEM, ctx->stream>>>(p);
+    RNN_CHECK_LAUNCH();
+    f32_dv_kernel<<<static_cast<unsigned>((a.tk + ROWS - 1ll) / ROWS * nbh), THREADS, DV_SMEM, ctx->stream>>>(p);
+    RNN_CHECK_LAUNCH();
+    return RNN_OK;
+  }
   static std::atomic<unsigned long long> optin_q{0}, optin_k{0};
   RNN_TRY(tc::ensure_smem_optin(f32_bwd_q_kernel, optin_q, ctx->device, static_cast<int>(BWD_SMEM)));
   RNN_TRY(tc::ensure_smem_optin(f32_bwd_kv_kernel, optin_k, ctx->device, static_cast<int>(BWD_SMEM)));
