@@ -57,7 +57,7 @@ struct Shared {
 };
 constexpr size_t FWD_SMEM = 1024 + ROW_TILE + FWD_STAGES * 2 * COL_TILE + sizeof(Shared);
 constexpr size_t FWD_WIDE_SMEM = 1024 + 2 * ROW_TILE + 3 * COL_TILE + sizeof(Shared);
-constexpr size_t GRAD_SMEM = 1024 + 3 * ROW_TILE + 3 * COL_TILE + sizeof(Shared);
+constexpr size_t GRAD_SMEM = 1024 + ROW_TILE + BWD_STAGES * 3 * COL_TILE + sizeof(Shared);
 constexpr size_t DV_SMEM = 1024 + 2 * ROW_TILE + 4 * COL_TILE + sizeof(Shared);
 static_assert(GRAD_SMEM <= 232448, "fits an SM");
 constexpr size_t BWD_SMEM = 1024 + 2 * ROW_TILE + BWD_STAGES * 2 * COL_TILE + sizeof(Shared);
@@ -1125,17 +1125,18 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
 // rows, or dk_m of 128 keys,
 //   S_m = X x^T,  dP = Y y^T,  dS_m = P_m (dP - D_m),  dX = dS_m x,
 // with X, x = q_m, k_m and Y, y = do, v for queries and the other way round for
-// keys.  dP is formed twice that way, and dv has a kernel of its own; one stage
-// of tiles fits beside the rows.  Measured: @GRAD@
-constexpr uint32_t G_DP = 64, G_P = 128, G_O = G_P + MAP;
+// keys.  dP is formed twice that way, and dv has a kernel of its own.  Y, the
+// larger of the rows, stays in tensor memory (columns 288 to 480).  Measured: @GRAD@
+constexpr uint32_t G_DP = 64, G_P = 128, G_O = G_P + MAP, G_Y = G_O + 64, Y_PLANE = 64;
 
 template <bool KEYS>
 __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t raw[];
   const Args& a = p.a;
   uint8_t* base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-  uint8_t* stage = base + 3 * ROW_TILE;
-  Shared& sh = *reinterpret_cast<Shared*>(stage + 3 * COL_TILE);
+  constexpr uint32_t STAGE = 3 * COL_TILE;
+  uint8_t* stage = base + ROW_TILE;
+  Shared& sh = *reinterpret_cast<Shared*>(stage + BWD_STAGES * STAGE);
   Block blk{sh, p.dev_error};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m = blockIdx.y;
   const int rows = KEYS ? a.tk : a.grp * a.tq, nbh = a.n * a.hkv, ntile = (rows + ROWS - 1) / ROWS;
@@ -1179,16 +1180,37 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
       return j < len && (!mask || mask[j]) ? x + j * sr : static_cast<const float*>(nullptr);
     };
     if (nt > 0) {
+      own_wide(base, a, tid, a.dh, a.slog2, [&](int u) {
+        const int r = row0 + own_row(tid, u);
+        const float* x = KEYS ? key_row(kp, a.kr, r) : query(qp, a.qr, a.qh, r);
+        return x ? x + m * a.dh : x;
+      });
+      // a thread's 64 columns of its row of Y
+      const int c0 = (warp >> 2) * 64, r = row0 + (warp & 3) * 32 + lane, in = 2 * a.dh - c0;
+      const float* y = KEYS ? key_row(vp, a.vr, r) : query(gp, a.gr, a.gh, r);
+      const uint32_t to = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + G_Y + (warp >> 2) * 32;
 #pragma unroll 1
-      for (int i = 0; i < 3; i++) {
-        const int col = i == 0 ? m * a.dh : (i - 1) * 64, in = i == 0 ? a.dh : 2 * a.dh - col;
-        own_wide(base + i * ROW_TILE, a, tid, in, i == 0 ? a.slog2 : 1.0f, [&](int u) {
-          const int r = row0 + own_row(tid, u);
-          const float* x = KEYS ? (i == 0 ? key_row(kp, a.kr, r) : key_row(vp, a.vr, r))
-                                : (i == 0 ? query(qp, a.qr, a.qh, r) : query(gp, a.gr, a.gh, r));
-          return x ? x + col : x;
-        });
+      for (int g = 0; g < 4; g++) {
+        float x[16];
+        if (a.vec) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (y && g * 16 + c < in) v = __ldg(reinterpret_cast<const float4*>(y + c0 + g * 16 + c));
+            x[c] = v.x, x[c + 1] = v.y, x[c + 2] = v.z, x[c + 3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; c++) x[c] = y && g * 16 + c < in ? __ldg(y + c0 + g * 16 + c) : 0.0f;
+        }
+        uint32_t z[3][8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) split3(x[2 * k], x[2 * k + 1], z[0][k], z[1][k], z[2][k]);
+#pragma unroll
+        for (int q = 0; q < 3; q++) tmem_st(to + q * Y_PLANE + g * 8, z[q]);
       }
+      tmem_wait_st();
+      tc_fence_before();
       fence_async_smem();
       signal(&sh.rows_full);
       // D_m, from do . o and do . o2; rows that see one tile of keys sum P dP
@@ -1247,14 +1269,17 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
 #pragma unroll
     for (int c = 0; c < 32; c++) acc[c] = 0.0f;
     for (int t = 0; ok && t < nt; t++) {
-      if (!(ok = blk.done(&sh.full[0], t & 1) && blk.done(&sh.s_full, t & 1))) break;
+      const int st = t % BWD_STAGES;
+      if (!(ok = blk.done(&sh.full[st], (t / BWD_STAGES) & 1) && blk.done(&sh.s_full, t & 1))) break;
       tc_fence_after();
       float s[32], dp[32];
       tmem_ld(at + part * 32, s);
       tmem_landed(s);
-      const float* stat = &sh.stat[0][0][part * 32];
+      tc_fence_before();
+      signal(&sh.s_free);
+      const float* stat = &sh.stat[st][0][part * 32];
       if (KEYS) {
-        if (most >= sh.least[0][part]) {
+        if (most >= sh.least[st][part]) {
 #pragma unroll
           for (int c = 0; c < 32; c++)
             if (need >= __float_as_int(stat[4 * COLS + c])) s[c] = -CUDART_INF_F;
@@ -1269,7 +1294,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
         }
       } else {
         const int j0 = t * COLS + part * 32;
-        const uint32_t seen = sh.seen[0][part];
+        const uint32_t seen = sh.seen[st][part];
         if (j0 + 32 > full || seen != 0xffffffffu) {
 #pragma unroll
           for (int c = 0; c < 32; c++)
@@ -1344,7 +1369,8 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
     if (warp < WARP_MMA) {
       const int t0 = tid - MATH_WARPS * 32;
       for (int t = 0; t < nt; t++) {
-        auto ready = [&] { return t == 0 || blk.done(&sh.empty[0], (t - 1) & 1); };
+        const int st = t % BWD_STAGES;
+        auto ready = [&] { return t < BWD_STAGES || blk.done(&sh.empty[st], (t / BWD_STAGES - 1) & 1); };
         auto in = [&](int i) { return i == 0 ? a.dh : 2 * a.dh - (i - 1) * 64; };
         if (KEYS) {
           const int e = t / per, i0 = qbeg + (t - e * per) * COLS, i = i0 + t0;
@@ -1352,7 +1378,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
           const long long from = ((static_cast<long long>(b) * a.h + h0 + e) * 2 + m) * a.tq + i;
           const float l = on ? a.flse[from] : CUDART_INF_F, d = on ? a.dsum[from] : 0.0f;
           const int lim = on ? row_limit(a, i, len) : 0;
-          if (!step_wide<3>(stage, a, t0,
+          if (!step_wide<3>(stage + st * STAGE, a, t0,
                             [&](int k, int r) -> const float* {
                               if (i0 + r >= a.tq) return nullptr;
                               return k == 0 ? qp + e * a.qh + (i0 + r) * a.qr + m * a.dh
@@ -1361,27 +1387,27 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
                             in, ready))
             break;
           if (t0 < COLS) {
-            sh.stat[0][0][t0] = -l;
-            sh.stat[0][2][t0] = -d;
-            sh.stat[0][4][t0] = __int_as_float(lim);
+            sh.stat[st][0][t0] = -l;
+            sh.stat[st][2][t0] = -d;
+            sh.stat[st][4][t0] = __int_as_float(lim);
             const int least = __reduce_min_sync(0xffffffffu, lim);
-            if ((t0 & 31) == 0) sh.least[0][t0 >> 5] = least;
+            if ((t0 & 31) == 0) sh.least[st][t0 >> 5] = least;
           }
         } else {
           const int j0 = t * COLS;
           auto on = [&](int r) { return j0 + r < kend && (!mask || mask[j0 + r]); };
           const uint32_t bits = __ballot_sync(0xffffffffu, t0 < COLS && on(t0));
-          if (!step_wide<3>(stage, a, t0,
+          if (!step_wide<3>(stage + st * STAGE, a, t0,
                             [&](int k, int r) -> const float* {
                               if (!on(r)) return nullptr;
                               return k == 0 ? kp + (j0 + r) * a.kr + m * a.dh : vp + (j0 + r) * a.vr + (k - 1) * 64;
                             },
                             in, ready))
             break;
-          if (t0 < COLS && (t0 & 31) == 0) sh.seen[0][t0 >> 5] = bits;
+          if (t0 < COLS && (t0 & 31) == 0) sh.seen[st][t0 >> 5] = bits;
         }
         fence_async_smem();
-        signal(&sh.full[0]);
+        signal(&sh.full[st]);
       }
       // dlam: block `head` sums that head's rows in a fixed order
       if (KEYS && m == 0 && warp == MATH_WARPS && static_cast<int>(blockIdx.x) < a.h && a.tq > 0) {
@@ -1397,29 +1423,39 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
     } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
       const uint32_t id_s = idesc_bf16(ROWS, COLS, false), id_o = idesc_bf16(ROWS, 64, true);
-      const uint64_t dx = desc_k(smem_u32(base)), dy = desc_k(smem_u32(base) + ROW_TILE);
+      const uint64_t dx = desc_k(smem_u32(base));
       const uint64_t cx = desc_k(smem_u32(stage)), cy = desc_k(smem_u32(stage) + COL_TILE);
       const uint64_t cn = desc_mn(smem_u32(stage), 0);
       const int ksteps = (a.dh + 15) / 16, vsteps = (2 * a.dh + 15) / 16;
       bool ok = blk.done(&sh.rows_full, 0);
-      for (int t = 0; ok && t < nt; t++) {
-        if (!(ok = blk.done(&sh.full[0], t & 1))) break;
+      auto scores = [&](int t) {
+        const int st = t % BWD_STAGES;
+        if (!blk.done(&sh.full[st], (t / BWD_STAGES) & 1) || (t > 0 && !blk.done(&sh.s_free, (t - 1) & 1))) return false;
         tc_fence_after();
         products<4>(ksteps, [&](int pa, int pb, int ks, bool acc) {
-          mma_ss(tmem, dx + (pa * ROW_PLANE + ks * 32) / 16, cx + (pb * COL_PLANE + ks * 32) / 16, id_s, acc, lead);
+          mma_ss(tmem, dx + (pa * ROW_PLANE + ks * 32) / 16, cx + st * (STAGE / 16) + (pb * COL_PLANE + ks * 32) / 16, id_s,
+                 acc, lead);
         });
         commit(&sh.s_full, lead);
+        return true;
+      };
+      ok = ok && scores(0);
+      for (int t = 0; ok && t < nt; t++) {
+        const int st = t % BWD_STAGES;
+        const uint32_t off = st * (STAGE / 16);
         products<8>(vsteps, [&](int pa, int pb, int ks, bool acc) {
-          mma_ss(tmem + G_DP, dy + ((ks >> 2) * ROW_TILE + pa * ROW_PLANE + (ks & 3) * 32) / 16,
-                 cy + ((ks >> 2) * COL_TILE + pb * COL_PLANE + (ks & 3) * 32) / 16, id_s, acc, lead);
+          mma_ts(tmem + G_DP, tmem + G_Y + pa * Y_PLANE + ks * 8,
+                 cy + off + ((ks >> 2) * COL_TILE + pb * COL_PLANE + (ks & 3) * 32) / 16, id_s, acc, lead);
         });
         commit(&sh.dp_full, lead);
+        if (t + 1 < nt && !(ok = scores(t + 1))) break;  // under this step's arithmetic
         if (!(ok = blk.done(&sh.p_full, t & 1))) break;
         tc_fence_after();
         products<COLS / 16>(COLS / 16, [&](int pa, int pb, int ks, bool acc) {
-          mma_ts(tmem + G_O, tmem + G_P + plane_at(pa, ks), cn + (pb * COL_PLANE + ks * 2048) / 16, id_o, acc, lead);
+          mma_ts(tmem + G_O, tmem + G_P + plane_at(pa, ks), cn + off + (pb * COL_PLANE + ks * 2048) / 16, id_o, acc,
+                 lead);
         });
-        commit(&sh.empty[0], lead);
+        commit(&sh.empty[st], lead);
         commit(&sh.o_full, lead);
       }
       if (!ok) {
