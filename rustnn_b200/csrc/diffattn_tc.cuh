@@ -268,8 +268,8 @@ int tc_bwd_parts(rnn_ctx* ctx, const Args& a);  // parts (256 floats a key each)
 bool dec_ok(const Args& a);
 int dec_fwd(rnn_ctx* ctx, const Args& a);
 int join_parts(rnn_ctx* ctx, const Args& a);
-// The tensor-core kernels in f32 (halves of up to 32 columns).
-bool f32_tc_ok(const Args& a);
+// The tensor-core kernels in f32.
+bool f32_tc_ok(const Args& a, bool backward);
 int f32_tc_fwd(rnn_ctx* ctx, const Args& a);
 int f32_tc_bwd(rnn_ctx* ctx, const Args& a);
 // Joins parts of many rows: 128 columns in bf16, 64 in f32.

@@ -1,5 +1,5 @@
-// Differential attention in f32 on tcgen05: halves of up to 32 columns, every
-// stride and mask, forward and backward.
+// Differential attention in f32 on tcgen05: every stride and mask, forward and
+// backward.
 //
 // An f32 operand is split into three bf16 planes, x = h + m + l with h, m, l the
 // rounded value, the rounded rest and its rest (24 bits), and a product is six
@@ -10,7 +10,8 @@
 //
 // Operands go through registers to be split, so they are read with plain loads
 // (any stride, masked keys as zeros) and written as 128-byte-swizzled tiles:
-// rows of 64 columns, the two halves of q and k side by side.  A block owns 128
+// rows of 64 columns, the two halves of q and k side by side, or (more than 32
+// columns) in tiles of their own.  A block owns 128
 // packed rows (queries of a key head's group, or keys) and has 8 arithmetic
 // warps, two threads a row with 32 columns each, 7 loading warps and one that
 // issues MMAs.  Measured: 32 x 256 x 256, 4 heads of 32: 34 us forward and 91
@@ -1126,7 +1127,9 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
 //   S_m = X x^T,  dP = Y y^T,  dS_m = P_m (dP - D_m),  dX = dS_m x,
 // with X, x = q_m, k_m and Y, y = do, v for queries and the other way round for
 // keys.  dP is formed twice that way, and dv has a kernel of its own.  Y, the
-// larger of the rows, stays in tensor memory (columns 288 to 480).  Measured: @GRAD@
+// larger of the rows, stays in tensor memory (columns 288 to 480).  Measured: 4 x 1024
+// x 1024, 4 heads of 64: 190 us forward and 357 backward, 300 and 1076 on the
+// kernels of mma.sync.
 constexpr uint32_t G_DP = 64, G_P = 128, G_O = G_P + MAP, G_Y = G_O + 64, Y_PLANE = 64;
 
 template <bool KEYS>
@@ -1639,11 +1642,14 @@ __global__ void __launch_bounds__(THREADS, 1) f32_dv_kernel(const __grid_constan
 // x 64, 4 heads of 32: 28 and 70 us against 38 and 83 here).  Here are faster: 64
 // x 128 x 128: 25 and 62 against 47 and 116; 32 x 256 x 256: 34 and 91 against 82
 // and 206; 64 x 64 x 256: 35 and 91 against 43 and 103; 1 x 64 x 5000: 25 and 283
-// against 26 and 524.  Halves of more than 32 columns would not leave room for
-// two stages of tiles beside the block's rows.
-bool f32_tc_ok(const Args& a) {
+// against 26 and 524.  Halves of more than 32 columns the same (4 x 64 x 64: no
+// difference; 64 x 100 x 100 of 48: 66 and 168 against 80 and 315), but forward,
+// where the scores are formed twice, only if rows fill a block or keys are many
+// (128 x 64 x 128, 4 heads of 64: 120 against 88, backward 276 against 353).
+bool f32_tc_ok(const Args& a, bool backward) {
   const long long rows = static_cast<long long>(a.grp) * a.tq;
-  return rows >= 64 && rows * a.tk >= 64 * 128;
+  if (rows < 64 || rows * a.tk < 64 * 128) return false;
+  return backward || a.dh <= 32 || rows >= 96 || a.tk >= 256;
 }
 
 int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
