@@ -1,4 +1,4 @@
-// Differential attention forward on tcgen05: bf16, halves of 16 .. 64 columns
+// Differential attention forward on tcgen05: bf16, halves of 8 .. 64 columns
 // (multiples of 8).
 //
 // A block owns 128 queries of one head.  Its 8 softmax warps are two teams, one
@@ -575,17 +575,22 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
 
 }  // namespace
 
-// A block costs about 5 us beside its tiles and holds one head's rows, while the
-// kernels of mma.sync pack the rows of all heads that share keys and run several
-// blocks an SM.  So they keep what is short on both sides (256 x 32 x 32, 4 heads
-// of 32: 20 us against 41 here; 128 x 64 x 64: 19 against 22) and rows too few to
-// fill a tile (64 x 3 x 1024, 32 heads on 4: 96 against 346; 64 x 9 x 512, 8 on
+// A block costs about 5 us beside its tiles, whose time does not go by dh, and
+// holds one head's rows, while the kernels of mma.sync pack the rows of all heads
+// that share keys and run several blocks an SM.  So they keep what is short on
+// both sides (256 x 32 x 32, 4 heads of 32: 20 us against 41 here), what is little
+// work (128 x 64 x 64 of 8: 12 and, backward, 27 against 24 and 54; 32 x 1000 x 4
+// of 16: 50 against 79; but 64 x 100 x 100 of 8: 19 and 45 against 16 and 35) and
+// rows too few to fill a tile (64 x 3 x 1024, 32 heads on 4: 96 against 346; 64 x 9 x 512, 8 on
 // 2: 50 against 62).  The rest is faster here: 64 x 24 x 256, 8 of 32: 39 against
 // 51; 128 x 33 x 1000, 8 of 64: 181 against 508; 32 x 1000 x 16: 102 against 131
 // (the others timed with a mask of keys that hides none).
+bool big_enough(const Args& a) {
+  return std::max(a.tq, a.tk) >= 64 && static_cast<long long>(a.tq) * a.tk * a.dh >= 65536;
+}
 bool tc_fwd_ok(const Args& a) {
-  if (a.dh % 8 || a.dh < 16 || a.dh > 64 || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
-  if (a.tq < 16 || std::max(a.tq, a.tk) < 64) return false;
+  if (a.dh % 8 || a.dh > 64 || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
+  if (a.tq < 16 || !big_enough(a)) return false;
   if (reinterpret_cast<uintptr_t>(a.o2) % 16) return false;
   return map_ok(a.q, a.n, a.tq, a.h, a.dh, a.qb, a.qr, a.qh) && map_ok(a.k, a.n, a.tk, a.hkv, a.dh, a.kb, a.kr, a.kh) &&
          map_ok(a.v, a.n, a.tk, a.hkv, 2 * a.dh, a.vb, a.vr, a.vh);

@@ -258,6 +258,7 @@ bool map_ok(const void* base, int n, int t, int heads, int cols, long long sb, l
 
 // Whether the tensor-core kernels take a call, and the calls themselves (the
 // backward's workspace pointers are set).
+bool big_enough(const Args& a);  // for a block's start and end to be worth it
 bool tc_fwd_ok(const Args& a);
 int tc_fwd(rnn_ctx* ctx, const Args& a);
 bool tc_bwd_ok(const Args& a);

@@ -1,4 +1,4 @@
-// Differential attention backward on tcgen05: bf16, halves of 16 .. 64 columns
+// Differential attention backward on tcgen05: bf16, halves of 8 .. 64 columns
 // (multiples of 8).  Two kernels, as in diffattn.cu: one owns 128 queries of a
 // head (dq, D_1, D_2, the row sums of P_2 dP), one owns 128 keys of a key head
 // (dk, dv).  Both form scores and dP = do v^T anew, 64 columns at a time, and
@@ -866,14 +866,14 @@ bool mult8(std::initializer_list<long long> s) {
 
 }  // namespace
 
-// What is short on both sides stays with the kernels of mma.sync, whose blocks
-// start and end faster (256 x 48 x 48, 4 heads of 32: 69 us against 86 here; 128 x
+// What is short on both sides or little work stays with the kernels of mma.sync,
+// whose blocks start and end faster (256 x 48 x 48, 4 heads of 32: 69 us against 86 here; 128 x
 // 64 x 64: 49 against 50).  The rest is faster here, few rows over many keys too
 // (4 x 4 x 4096, 32 heads on 4: 132 us against 468; 64 x 24 x 256, 8 heads of 32:
 // 84 against 88; 32 x 1000 x 16, 8 of 64: 163 against 281).
 bool tc_bwd_ok(const Args& a) {
-  if (a.dh % 8 || a.dh < 16 || a.dh > 64 || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
-  if (std::max(a.tq, a.tk) < 64) return false;
+  if (a.dh % 8 || a.dh > 64 || !(a.slog2 > 0.0f) || a.slog2 > 1e30f) return false;
+  if (!big_enough(a)) return false;
   if (reinterpret_cast<uintptr_t>(a.fo) % 16 || reinterpret_cast<uintptr_t>(a.fo2) % 16) return false;
   if (!mult8({a.ob, a.orow, a.oh})) return false;
   return map_ok(a.q, a.n, a.tq, a.h, a.dh, a.qb, a.qr, a.qh) && map_ok(a.k, a.n, a.tk, a.hkv, a.dh, a.kb, a.kr, a.kh) &&

@@ -325,6 +325,22 @@ def test_few_rows_over_a_masked_cache(ops, tq, tk, h, hkv, dh, dtype):
         assert rel(o[b], want[b]) < TOL[dtype], (b, rel(o[b], want[b]))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [None, "start", "end"])
+@pytest.mark.parametrize("n,tq,tk,h,hkv", [(2, 200, 200, 2, 2), (3, 70, 500, 4, 2), (1, 513, 65, 2, 1), (4, 130, 3000, 2, 2)])
+def test_narrowest_heads(ops, n, tq, tk, h, hkv, causal, dtype):
+    """Halves of eight columns over tiles, with lengths and masked keys that hold anything."""
+    q, k, v, lam, dout = make(n, tq, tk, h, hkv, 8, dtype, 41)
+    check_all(ops, q, k, v, lam, dout, causal=causal)
+    klen = torch.tensor([tk - 3, 1, tk // 2, 0][:n], dtype=torch.int32, device="cuda")
+    kmask = torch.rand(n, tk, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)) < 0.7
+    for m in (None, kmask):
+        hidden = torch.arange(tk, device="cuda")[None] >= klen[:, None]
+        hidden = hidden if m is None else hidden | ~m
+        k2, v2 = k.masked_fill(hidden[:, :, None, None], math.nan), v.masked_fill(hidden[:, :, None, None], math.inf)
+        check_all(ops, q, k2, v2, lam, dout, causal=causal, klen=klen, kmask=m)
+
+
 def test_nearly_equal_maps_over_a_long_cache(ops):
     """What is left of the difference keeps the type's precision when the keys are split too."""
     q, k, v, _, dout = make(1, 130, 3000, 2, 2, 32, BF16, 9)
