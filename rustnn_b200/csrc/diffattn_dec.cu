@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(DEC_THREADS) dec_kernel(const __grid_constant_
     }
     const int full = __reduce_min_sync(0xffffffffu, low);
     const float c2 = a.slog2;
-    int st = 0, ph = 0, slices = 0;
+    int st = 0, ph = 0;
     // whether a masked call's key `lane` of the warp's 16 counts, a tile ahead
     const uint8_t* mask = MASK ? a.kmask + b * a.kmb : nullptr;
     auto counts = [&](int j) { return lane < 16 && j + lane < len && mask[j + lane] != 0; };
@@ -206,11 +206,18 @@ __global__ void __launch_bounds__(DEC_THREADS) dec_kernel(const __grid_constant_
             far |= !(x1[nb][e] <= FAR_SUM) || !(x2[nb][e] <= FAR_SUM) ||
                    (n1 == -CUDART_INF_F && u != -CUDART_INF_F);
           }
-        // references and ratios: changed where a score is far above, the ratio
-        // also after 1, 4, 16, ... slices
-        slices++;
-        const bool check = (slices & (slices - 1)) == 0 && (__ffs(slices) & 1);
-        if (__builtin_expect(__any_sync(0xffffffffu, far) || check, 0)) {
+        // references and ratios: changed where a score is far above a reference,
+        // or the ratio half off lam l_1 / l_2 (what it is off by is what the
+        // rounding of P_2 is multiplied with)
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float q1 = lam[nb][e] * keys_sum(l1[nb][e] + x1[nb][e] + x1[nb][e + 2]);
+            const float q2 = r[nb][e] * keys_sum(l2[nb][e] + x2[nb][e] + x2[nb][e + 2]);
+            far |= fabsf(q1 - q2) > 0.5f * fabsf(q1);
+          }
+        if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) {
 #pragma unroll
           for (int nb = 0; nb < NB; nb++)
 #pragma unroll

@@ -18,7 +18,7 @@
 // A row's references (maxima m_1, m_2 and the ratio r) sit in shared memory and
 // change rarely: a map's maximum when a tile exceeds it by 2^20 (sums and
 // products are f32 and bf16, whose range allows that, so that most tiles need
-// no maximum at all: their sums tell), the ratio when it is a quarter off
+// no maximum at all: their sums tell), the ratio when it is half off
 // lam l_1 / l_2.  They pass from tile to tile with a token per pair of warps
 // that own the same rows; who changes one waits for the products so far and
 // rescales A and B.  With P_1 and P_2 in units of 2^m:
@@ -190,10 +190,6 @@ __device__ __forceinline__ void store_maps(uint32_t dst, const float (&s1)[2][32
     tmem_st(dst + 32 + h * 16, e);
   }
 }
-// Whether tile j compares the ratio with the sums so far (always the second
-// team's, after the first tile).
-__device__ __forceinline__ bool check_at(int j) { return j == 0 || (j >= 3 && (j & (j + 1)) == 0); }
-
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <bool MASK>
@@ -298,16 +294,21 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
       // the sums and maps of this tile move to what the references become.
       bool change = true;
       float4 ref = make_float4(-CUDART_INF_F, -CUDART_INF_F, lam, 0.0f);
+      float4 other = make_float4(-CUDART_INF_F, 0.0f, -CUDART_INF_F, 0.0f);  // the other team's sums
       if (j > 0) {
         if (!warp_wait(&sh.tok[w], (j - 1) & 1, abort_flag, dev_error)) break;
         ref = sh.ref[row];
-        change = check_at(j) || ref.x != u1 || ref.y != u2 || ref.x != m1 || ref.y != m2;
+        other = sh.sum[team ^ 1][row];
+        // The ratio has to stay near lam l_1 / l_2: what it is off by is what the
+        // rounding of P_2 is multiplied with.
+        const float q1 = lam * (l1 + sum1 + other.y), q2 = ref.z * (l2 + sum2 + other.w);
+        change = ref.x != u1 || ref.y != u2 || ref.x != m1 || ref.y != m2 || fabsf(q1 - q2) > 0.5f * fabsf(q1);
       }
       r = ref.z;
       if (__builtin_expect(!__any_sync(0xffffffffu, change), 1)) {
         l1 += sum1;
         l2 += sum2;
-        if (check_at(j + 1)) sh.sum[team][row] = make_float4(m1, l1, m2, l2);
+        sh.sum[team][row] = make_float4(m1, l1, m2, l2);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.tok[w]);
       } else {
@@ -320,22 +321,17 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
         event |= raise(m2, u2, al2, f2);
         l1 = l1 * al1 + sum1 * f1;
         l2 = l2 * al2 + sum2 * f2;
-        if (check_at(j)) {
-          // the sums so far: own ones, and the other team's as it gave them with
-          // its last token (which tiles they cover does not depend on timing)
-          float q1 = l1, q2 = l2;
-          if (j > 0) {
-            const float4 z = sh.sum[team ^ 1][row];
-            if (z.y > 0.0f) q1 += z.y * ex2(z.x - m1);
-            if (z.w > 0.0f) q2 += z.w * ex2(z.z - m2);
-          }
-          const float want = lam * __fdividef(q1, q2);
-          if (q1 > 0.0f && q2 > 0.0f && (j == 0 || fabsf(want - r) > 0.25f * fabsf(want))) {
-            rn = want;
-            event = true;
-          }
+        // the sums so far: own ones, and the other team's as it gave them with its
+        // last token (which tiles they cover does not depend on timing)
+        float q1 = l1, q2 = l2;
+        if (other.y > 0.0f) q1 += other.y * ex2(other.x - m1);
+        if (other.w > 0.0f) q2 += other.w * ex2(other.z - m2);
+        const float want = lam * __fdividef(q1, q2);
+        if (q1 > 0.0f && q2 > 0.0f && (j == 0 || fabsf(want - r) > 0.25f * fabsf(want))) {
+          rn = want;
+          event = true;
         }
-        if (check_at(j + 1)) sh.sum[team][row] = make_float4(m1, l1, m2, l2);
+        sh.sum[team][row] = make_float4(m1, l1, m2, l2);
         sh.ref[row] = make_float4(m1, m2, rn, 0.0f);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.tok[w]);

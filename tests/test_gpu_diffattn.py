@@ -341,6 +341,22 @@ def test_narrowest_heads(ops, n, tq, tk, h, hkv, causal, dtype):
         check_all(ops, q, k2, v2, lam, dout, causal=causal, klen=klen, kmask=m)
 
 
+@pytest.mark.parametrize("tq,tk,h,hkv,dh", [(409, 409, 3, 3, 56), (100, 210, 4, 2, 32), (1, 223, 8, 2, 64), (2, 3000, 4, 1, 64),
+                                            (273, 273, 2, 2, 64), (130, 3000, 2, 2, 48), (300, 300, 2, 1, 5)])
+@pytest.mark.parametrize("scale", [0.3, -0.2, 0.6])
+def test_sharp_maps(ops, tq, tk, h, hkv, dh, scale):
+    """A few keys hold most of a row, and the maps' sums grow apart from tile to tile: the bf16 output keeps its
+    precision, masked or not."""
+    q, k, v, lam, dout = make(3, tq, tk, h, hkv, dh, BF16, 12)
+    kmask = torch.rand(3, tk, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)) < 0.3
+    kmask[2] &= torch.arange(tk, device="cuda") > tk // 2
+    for m in (None, kmask):
+        want = reference(q, k, v, lam, dout, scale, None, None, m)
+        o, o2, _ = ops.diffattn_forward(q, k, v, lam, scale=scale, kmask=m, save=True)
+        for b in range(3):
+            assert rel(o[b], want[0][b]) < TOL[BF16] and rel(o2[b], want[1][b]) < TOL[BF16]
+
+
 def test_nearly_equal_maps_over_a_long_cache(ops):
     """What is left of the difference keeps the type's precision when the keys are split too."""
     q, k, v, _, dout = make(1, 130, 3000, 2, 2, 32, BF16, 9)
