@@ -343,9 +343,12 @@ typedef struct rnn_diffattn {
 } rnn_diffattn;
 /* s_m = scale q_m k_m^T and P_m = softmax(s_m) over the visible keys, m = 1, 2;
  * o = (P_1 - lambda[head] P_2) v.  lambda [h] f32.  A query that sees no key
- * gets 0.  For the backward pass, o2 (dtype, contiguous [n, tq, h, 2*dh]; P_2 v)
+ * gets 0, and a map whose visible scores are all -inf is 0.  NaN in a query or
+ * a key that it sees, or a score of +inf, makes the query's outputs NaN; so may
+ * any score beyond f32's range where operands are f32 (they are multiplied in
+ * parts).  For the backward pass, o2 (dtype, contiguous [n, tq, h, 2*dh]; P_2 v)
  * and lse (f32, [n, h, 2, tq]: log2 of each map's sum of exponentials, +inf
- * for a query that sees no key) are written when non-NULL, both or neither.
+ * for a map of 0) are written when non-NULL, both or neither.
  * No score matrix is stored.  dh in 1 .. 64. */
 int rnn_diffattn_fwd_dev(rnn_ctx *ctx, const rnn_diffattn *d, const void *q,
                          const void *k, const void *v, const float *lambda,

@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
       }
       return;
     }
-    const float i1 = L1 > 0.0f ? 1.0f / L1 : 0.0f, i2 = L2 > 0.0f ? 1.0f / L2 : 0.0f;
-    const float lm = __ldg(a.lam + head);
+    const float i1 = inverse(L1), i2 = inverse(L2);
+    const float lm = L2 == 0.0f ? 0.0f : __ldg(a.lam + head);
     T* o = static_cast<T*>(a.o) + b * a.ob + head * a.oh + i * a.orow;
     T* o2 = a.o2 ? static_cast<T*>(a.o2) + ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) : nullptr;
     for (int c = c0; c < 2 * a.dh; c += 8) {
@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
     }
     if (a.lse && c0 == 0) {
       float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-      s[0] = L1 > 0.0f ? M1 + log2f(L1) : CUDART_INF_F;
-      s[a.tq] = L2 > 0.0f ? M2 + log2f(L2) : CUDART_INF_F;
+      s[0] = log_sum(M1, L1);
+      s[a.tq] = log_sum(M2, L2);
     }
   } else {
 #pragma unroll
@@ -358,20 +358,23 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
           *reinterpret_cast<float4*>(a.stat + row * 4) = make_float4(m1[h], l1[h], m2[h], l2[h]);
         continue;
       }
-      const float i1 = l1[h] > 0.0f ? 1.0f / l1[h] : 0.0f, i2 = l2[h] > 0.0f ? 1.0f / l2[h] : 0.0f;
+      const float i2 = inverse(l2[h]);
+      // where the first map is 0 A holds nothing, and o = -lam P_2 v
+      const float i1 = inverse(l1[h]), f2 = l1[h] == 0.0f && l2[h] != 0.0f ? -lam[h] * i2 : 0.0f;
       T* o = static_cast<T*>(a.o) + b * a.ob + head * a.oh + i * a.orow;
       T* o2 =
           a.o2 ? static_cast<T*>(a.o2) + ((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) : nullptr;
 #pragma unroll
       for (int nb = 0; nb < NB; nb++) {
         const int c = nb * 8 + 2 * (lane & 3);
-        store2(o + c, A[nb][2 * h] * i1, A[nb][2 * h + 1] * i1, c < 2 * a.dh, c + 1 < 2 * a.dh, a.pair);
+        const float x = A[nb][2 * h] * i1 + f2 * B[nb][2 * h], y = A[nb][2 * h + 1] * i1 + f2 * B[nb][2 * h + 1];
+        store2(o + c, x, y, c < 2 * a.dh, c + 1 < 2 * a.dh, a.pair);
         if (o2) store2(o2 + c, B[nb][2 * h] * i2, B[nb][2 * h + 1] * i2, c < 2 * a.dh, c + 1 < 2 * a.dh, true);
       }
       if (a.lse && (lane & 3) == 0) {
         float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-        s[0] = l1[h] > 0.0f ? m1[h] + log2f(l1[h]) : CUDART_INF_F;
-        s[a.tq] = l2[h] > 0.0f ? m2[h] + log2f(l2[h]) : CUDART_INF_F;
+        s[0] = log_sum(m1[h], l1[h]);
+        s[a.tq] = log_sum(m2[h], l2[h]);
       }
     }
   }
@@ -441,17 +444,17 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(Args a) {
   }
   const int e = p / a.tq, i = p - e * a.tq;
   const int head = kvh * a.grp + e;
-  const float i1 = L1 > 0.0f ? 1.0f / L1 : 0.0f, i2 = L2 > 0.0f ? 1.0f / L2 : 0.0f;
+  const float i1 = inverse(L1), i2 = inverse(L2), lm = L2 == 0.0f ? 0.0f : __ldg(a.lam + head);
   if (col < 2 * a.dh) {
-    static_cast<T*>(a.o)[b * a.ob + head * a.oh + i * a.orow + col] = from_f<T>(x * i1 - __ldg(a.lam + head) * (y * i2));
+    static_cast<T*>(a.o)[b * a.ob + head * a.oh + i * a.orow + col] = from_f<T>(x * i1 - lm * (y * i2));
     if (a.o2)
       static_cast<T*>(a.o2)[((static_cast<long long>(b) * a.tq + i) * a.h + head) * (2 * a.dh) + col] =
           from_f<T>(y * i2);
   }
   if (a.lse && tid == 0) {
     float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-    s[0] = L1 > 0.0f ? M1 + log2f(L1) : CUDART_INF_F;
-    s[a.tq] = L2 > 0.0f ? M2 + log2f(L2) : CUDART_INF_F;
+    s[0] = log_sum(M1, L1);
+    s[a.tq] = log_sum(M2, L2);
   }
 }
 
@@ -501,8 +504,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_rows_kernel(const __grid
   const int rows = a.grp * a.tq;
   const int bh = static_cast<int>(idx / rows), r = static_cast<int>(idx - static_cast<long long>(bh) * rows);
   const int b = bh / a.hkv, e = r / a.tq, i = r - e * a.tq, head = (bh - b * a.hkv) * a.grp + e;
-  const bool any = L1 > 0.0f && L2 > 0.0f;
-  const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f, f = any ? __ldg(a.lam + head) * i2 : 0.0f;
+  const float i1 = inverse(L1), i2 = inverse(L2), f = L2 == 0.0f ? 0.0f : __ldg(a.lam + head) * i2;
   if (mine) {
     T* o = static_cast<T*>(a.o) + b * a.ob + head * a.oh + i * a.orow + lane * 4;
     const int in = 2 * a.dh - lane * 4;  // at least 2
@@ -516,8 +518,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_rows_kernel(const __grid
   }
   if (a.lse && lane < 2) {
     float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-    if (lane == 0) s[0] = any ? M1 + log2f(L1) : CUDART_INF_F;
-    else s[a.tq] = any ? M2 + log2f(L2) : CUDART_INF_F;
+    if (lane == 0) s[0] = log_sum(M1, L1);
+    else s[a.tq] = log_sum(M2, L2);
   }
 }
 
@@ -823,7 +825,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
   for (int h = 0; h < 2; h++) {
     // over the map's own sum: what the log-sum's rounding does to a whole row cancels
     const float whole = quad_sum(pl[h]), part = quad_sum(dl[h]);
-    const float sum = whole > 0.0f ? part / whole : 0.0f;
+    const float sum = whole == 0.0f ? 0.0f : part / whole;
     const int p = row0 + warp * 16 + (lane >> 2) + 8 * h;
     if (p >= rows) continue;
     const int e = p / a.tq, i = p - e * a.tq;

@@ -49,6 +49,13 @@ struct Args {
 __device__ __forceinline__ int key_len(const Args& a, int b) {
   return a.klen ? min(max(__ldg(a.klen + b), 0), a.tk) : a.tk;
 }
+// A map's normaliser and log-sum from its reference m and sum l.  A sum is 0 only
+// where no key counts (none is visible, or every score is -inf): that map is 0,
+// its log-sum +inf.  A sum that is not a number, from NaN or infinite scores,
+// makes the row NaN, as the formula has it.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.0f ? CUDART_INF_F : m + log2f(l); }
+
 // Number of leading keys that query i of a sequence of `len` keys may see.
 __device__ __forceinline__ int row_limit(const Args& a, int i, int len) {
   if (a.causal == RNN_CAUSAL_START) return min(len, i + 1);

@@ -353,8 +353,8 @@ __global__ void __launch_bounds__(DEC_THREADS) dec_kernel(const __grid_constant_
     }
     const long long at = (static_cast<long long>(blockIdx.y) * nbh + bh) * rows + row;
     const int head = kvh * a.grp + row / a.tq, i = row % a.tq;
-    const float i1 = L1 > 0.0f ? 1.0f / L1 : 0.0f, i2 = L2 > 0.0f ? 1.0f / L2 : 0.0f;
-    const float lm = __ldg(a.lam + head);
+    const float i1 = inverse(L1), i2 = inverse(L2);
+    const float lm = L2 == 0.0f ? 0.0f : __ldg(a.lam + head);
     for (int c = lane; c < 2 * a.dh; c += 32) {
       float x = 0.0f, y = 0.0f;
 #pragma unroll
@@ -378,8 +378,8 @@ __global__ void __launch_bounds__(DEC_THREADS) dec_kernel(const __grid_constant_
         *reinterpret_cast<float4*>(a.stat + at * 4) = make_float4(M1, L1, M2, L2);
       } else if (a.lse) {
         float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-        s[0] = L1 > 0.0f ? M1 + log2f(L1) : CUDART_INF_F;
-        s[a.tq] = L2 > 0.0f ? M2 + log2f(L2) : CUDART_INF_F;
+        s[0] = log_sum(M1, L1);
+        s[a.tq] = log_sum(M2, L2);
       }
     }
   }

@@ -382,9 +382,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
     sh.sum[team][row] = make_float4(0.0f, l1, 0.0f, l2);
     soft_sync();
     const float L1 = sh.sum[0][row].y + sh.sum[1][row].y, L2 = sh.sum[0][row].w + sh.sum[1][row].w;
-    const bool any = L1 > 0.0f && L2 > 0.0f;
-    const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f;
-    const float rest = any ? last.z - lam * L1 * i2 : 0.0f;
+    // o = (A + (r - lam l_1 / l_2) B) / l_1; where the first map is 0, -lam B / l_2
+    const bool one = L1 != 0.0f, two = L2 != 0.0f;
+    const float i1 = one ? 1.0f / L1 : 1.0f, i2 = inverse(L2);
+    const float rest = one ? last.z - lam * L1 * i2 : two ? -lam * i2 : 0.0f;
     bool ok = true;
     if (nt > 0) {
       ok = warp_wait(&sh.o_full, 0, abort_flag, dev_error);
@@ -426,10 +427,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
       uint32_t po[8], p2[8];
 #pragma unroll
       for (int k = 0; k < 8; k++) {
-        const float x0 = any ? (x[2 * k] + rest * y[2 * k]) * i1 : 0.0f;
-        const float x1 = any ? (x[2 * k + 1] + rest * y[2 * k + 1]) * i1 : 0.0f;
+        // a map without a key has no part in the products but what 0 * inf or 0 * NaN left
+        const float y0 = two ? y[2 * k] : 0.0f, y1 = two ? y[2 * k + 1] : 0.0f;
+        const float x0 = ((one ? x[2 * k] : 0.0f) + rest * y0) * i1;
+        const float x1 = ((one ? x[2 * k + 1] : 0.0f) + rest * y1) * i1;
         po[k] = pack2(x0, x1);
-        p2[k] = pack2(any ? y[2 * k] * i2 : 0.0f, any ? y[2 * k + 1] * i2 : 0.0f);
+        p2[k] = pack2(y0 * i2, y1 * i2);
       }
       if (i < a.tq) {
         if (p.o16) {
@@ -452,8 +455,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1) tc_fwd_kernel(const __grid_con
     }
     if (whole && a.lse && team == 0 && i < a.tq) {
       float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-      s[0] = any ? last.x + log2f(L1) : CUDART_INF_F;
-      s[a.tq] = any ? last.y + log2f(L2) : CUDART_INF_F;
+      s[0] = log_sum(last.x, L1);
+      s[a.tq] = log_sum(last.y, L2);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");

@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       const float part = (sh.part[0][row].x + sh.part[1][row].x) + (sh.part[2][row].x + sh.part[3][row].x);
       const float whole = (sh.part[0][row].y + sh.part[1][row].y) + (sh.part[2][row].y + sh.part[3][row].y);
       a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
-          whole > 0.0f ? part / whole : 0.0f;
+          whole == 0.0f ? 0.0f : part / whole;
     }
 
     bool ok = true;

@@ -568,13 +568,13 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
         store_rows(patch, y, 32, true, q ? q + PART_W : nullptr);
         if (part == 0 && col0 == 0 && r < rows) *reinterpret_cast<float4*>(a.stat + to * 4) = make_float4(m1, L1, m2, L2);
       } else {
-        const bool any = L1 > 0.0f && L2 > 0.0f;
-        const float i1 = any ? 1.0f / L1 : 0.0f, i2 = any ? 1.0f / L2 : 0.0f;
-        const float lam = any ? __ldg(a.lam + head) : 0.0f;
+        // a map without a key has no part in the products but what 0 * inf or 0 * NaN left
+        const bool one = L1 != 0.0f, two = L2 != 0.0f;
+        const float i1 = inverse(L1), i2 = inverse(L2), lam = two ? __ldg(a.lam + head) : 0.0f;
 #pragma unroll
         for (int c = 0; c < 32; c++) {
-          y[c] = any ? y[c] * i2 : 0.0f;
-          x[c] = any ? x[c] * i1 - lam * y[c] : 0.0f;
+          y[c] = two ? y[c] * i2 : 0.0f;
+          x[c] = (one ? x[c] * i1 : 0.0f) - lam * y[c];
         }
         const int in = 2 * a.dh - col0 - part * 32;
         store_rows(patch, x, in, p.st16,
@@ -586,8 +586,8 @@ __global__ void __launch_bounds__(THREADS, 1) f32_fwd_kernel(const __grid_consta
                               : nullptr);
         if (a.lse && part == 0 && col0 == 0 && r < rows) {
           float* s = a.lse + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
-          s[0] = any ? m1 + log2f(L1) : CUDART_INF_F;
-          s[a.tq] = any ? m2 + log2f(L2) : CUDART_INF_F;
+          s[0] = log_sum(m1, L1);
+          s[a.tq] = log_sum(m2, L2);
         }
       }
     }
@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_q_kernel(const __grid_cons
         s[0] = d1;
         s[a.tq] = d2;
         a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
-            whole > 0.0f ? (dl + other.x) / whole : 0.0f;
+            whole == 0.0f ? 0.0f : (dl + other.x) / whole;
       }
       const float f = part ? -a.scale * __ldg(a.lam + head) : a.scale;
 #pragma unroll
@@ -1357,7 +1357,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
           a.dsum[((static_cast<long long>(b) * a.h + head) * 2 + m) * a.tq + i] = d;
           if (m)
             a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
-                whole > 0.0f ? (dl + other.x) / whole : 0.0f;
+                whole == 0.0f ? 0.0f : (dl + other.x) / whole;
         }
         const float f = m ? -a.scale * __ldg(a.lam + head) : a.scale;
 #pragma unroll

@@ -397,7 +397,8 @@ def diffattn_forward(q, k, v, lam, scale=None, causal=None, klen=None, kmask=Non
     defaults to 1/sqrt(dh).  Key j is visible to query i when j < klen[b]
     (int32 [n]), kmask[b, j] (bool [n, tk]) and, for causal "start", j <= i, or
     for "end", j <= i + klen[b] - tq (new tokens against a cache).  A query that
-    sees no key gets 0; hidden keys and values may hold anything.
+    sees no key gets 0; hidden keys and values may hold anything.  NaN in a query
+    or in a key that it sees, or a score of +inf, makes the query's output NaN.
 
     Returns o [n, tq, h, 2*dh], or with save (o, o2, lse) for the backward."""
     d, out, ptrs = _diffattn(q, k, v, lam, out, scale, causal, klen, kmask)
