@@ -324,7 +324,8 @@ int rnn_rope_dev(rnn_ctx *ctx, int dtype, const void *x, long long xrow,
  *   causal RNN_CAUSAL_START: j <= i          (query i sits at key i),
  *   causal RNN_CAUSAL_END:   j <= i + klen[b] - tq  (the last query sits at
  *                            the last key: new tokens against a cache).
- * Keys and values that klen or kmask hides may hold anything. */
+ * Keys and values that klen or kmask hides, and with RNN_CAUSAL_START those
+ * from tq on, may hold anything. */
 #define RNN_CAUSAL_NONE 0
 #define RNN_CAUSAL_START 1
 #define RNN_CAUSAL_END 2

@@ -46,8 +46,12 @@ struct Args {
   float* kpart;  // [part][n * hkv][tk][256]: dv, dk_1, dk_2 of a part, 64 columns each piece
 };
 
+// Leading keys of sequence b that some query may see.  With RNN_CAUSAL_START the
+// last query sits at key tq - 1, and what lies beyond is like what lies beyond
+// klen: never read into a product, where 0 times it might be NaN.
 __device__ __forceinline__ int key_len(const Args& a, int b) {
-  return a.klen ? min(max(__ldg(a.klen + b), 0), a.tk) : a.tk;
+  const int most = a.causal == RNN_CAUSAL_START ? min(a.tk, a.tq) : a.tk;
+  return a.klen ? min(max(__ldg(a.klen + b), 0), most) : most;
 }
 // A map's normaliser and log-sum from its reference m and sum l.  A sum is 0 only
 // where no key counts (none is visible, or every score is -inf): that map is 0,
