@@ -357,6 +357,7 @@ int rnn_diffattn_fwd_dev(rnn_ctx *ctx, const rnn_diffattn *d, const void *q,
 /* Gradients from dout and the forward's o, o2 and lse: dq, dk, dv are written,
  * dlambda [h] (f32) accumulates.  The q, k, v and o strides of g are those of
  * dq, dk, dv and dout (nothing else of g is read); g NULL: those of d.
+ * Keys that are hidden from every query, as above, get 0 whatever the rest holds.
  * Deterministic. */
 int rnn_diffattn_bwd_dev(rnn_ctx *ctx, const rnn_diffattn *d,
                          const rnn_diffattn *g, const void *q, const void *k,

@@ -1051,6 +1051,10 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
 #pragma unroll
   for (int h = 0; h < 2; h++) {
     if (key[h] >= a.tk) continue;
+    if (!seen[h]) {  // 0, whatever a query's NaN made of 0 times it
+#pragma unroll
+      for (int nb = 0; nb < NB; nb++) dk[nb][2 * h] = dk[nb][2 * h + 1] = dv[nb][2 * h] = dv[nb][2 * h + 1] = 0.0f;
+    }
     T* ok = static_cast<T*>(a.dk) + b * a.dkb + kvh * a.dkh + key[h] * a.dkr;
     T* ov = static_cast<T*>(a.dv) + b * a.dvb + kvh * a.dvh + key[h] * a.dvr;
 #pragma unroll

@@ -1005,10 +1005,13 @@ __global__ void __launch_bounds__(THREADS, 1) f32_bwd_kv_kernel(const __grid_con
     }
     if (ok && work) {
       float* patch = reinterpret_cast<float*>(base) + warp * 1024;
+      const bool hidden = need == 0x7fffffff;  // 0, whatever a query's NaN made of 0 times it
+#pragma unroll
+      for (int c = 0; c < 32; c++) dv[c] = hidden ? 0.0f : dv[c];
       store_rows(patch, dv, 2 * a.dh - part * 32, p.st16,
                  key < a.tk ? static_cast<float*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr + part * 32 : nullptr);
 #pragma unroll
-      for (int c = 0; c < 32; c++) dk[c] *= a.scale;
+      for (int c = 0; c < 32; c++) dk[c] = hidden ? 0.0f : dk[c] * a.scale;
       store_rows(patch, dk, a.dh, p.st16,
                  key < a.tk ? static_cast<float*>(a.dk) + b * a.dkb + kvh * a.dkh + key * a.dkr + part * a.dh : nullptr);
     }
@@ -1343,7 +1346,7 @@ __global__ void __launch_bounds__(THREADS, 1) f32_grad_kernel(const __grid_const
     const int in = a.dh - part * 32;
     if (KEYS) {
 #pragma unroll
-      for (int c = 0; c < 32; c++) acc[c] *= a.scale;
+      for (int c = 0; c < 32; c++) acc[c] = need == 0x7fffffff ? 0.0f : acc[c] * a.scale;  // a hidden key's is 0
       if (ok && work)
         store_rows(patch, acc, in, p.st16,
                    r < rows ? static_cast<float*>(a.dk) + b * a.dkb + kvh * a.dkh + r * a.dkr + m * a.dh + part * 32
@@ -1562,6 +1565,11 @@ __global__ void __launch_bounds__(THREADS, 1) f32_dv_kernel(const __grid_constan
     if (ok) {
       float* patch = reinterpret_cast<float*>(base) + warp * 1024;
       float* to = key < a.tk ? static_cast<float*>(a.dv) + b * a.dvb + kvh * a.dvh + key * a.dvr + part * 32 : nullptr;
+#pragma unroll
+      for (int c = 0; c < 32; c++) {  // a hidden key's is 0, whatever a query's NaN made of 0 times it
+        v0[c] = need == 0x7fffffff ? 0.0f : v0[c];
+        v1[c] = need == 0x7fffffff ? 0.0f : v1[c];
+      }
       store_rows(patch, v0, 2 * a.dh - part * 32, p.st16, to);
       store_rows(patch, v1, 2 * a.dh - 64 - part * 32, p.st16, to ? to + 64 : nullptr);
     }
