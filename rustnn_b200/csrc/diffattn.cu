@@ -15,7 +15,7 @@
 //   dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,
 //   dv = (P_1 - lam P_2)^T do,  dlam = -sum_rows D_2.
 // Two kernels recompute the maps from the saved log-sums: one owns query rows
-// (dq, D, the f32 row sums of P_2 dP for dlam), one owns keys (dk, dv).  No
+// (dq, and D, of which dlam is the sum), one owns keys (dk, dv).  No
 // atomics: results do not depend on scheduling.
 //
 // Bound by the latency of dependent instructions (8 to 12 warps fit an SM, two
@@ -545,8 +545,7 @@ struct BwdQ {
   static constexpr size_t SMEM = TILES + ROWS * 2 * sizeof(float) + 2 * BN;
 };
 
-// dq of 64 packed rows, D_1 and D_2 of each (for the key kernel), and the row
-// sums of P_2 dP.
+// dq of 64 packed rows, and D_1 and D_2 of each for the key kernel.
 template <class T, int DH>
 __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
   using F = BwdQ<T, DH>;
@@ -615,24 +614,12 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
   cp_commit();
   if (ntk > 0) load_kv(0);
 
-  // D_1 = do . (o + lam o2) and D_2 = do . o2 of the warp's 16 rows.  What the
-  // rounding of o and o2 leaves in D reaches dq in proportion to |o| / |v|, so
-  // it matters where few keys are averaged: rows that see one register step of
-  // keys sum P dP there (dS of a lone key comes out as 0), and in bf16 rows of
-  // up to 128 keys sum it in a pass of its own.
+  // D_1 = do . (o + lam o2) and D_2 = do . o2 of the warp's 16 rows.  Rows that see
+  // one register step of keys sum P dP there instead (dS of a lone key comes out as
+  // 0), and in bf16 rows of up to 128 keys, of which few share each row, sum it in a
+  // pass of its own; the others follow too_far().
   const bool one_step = kend <= SUB;
-  bool own_pass = !one_step && sizeof(T) == 2 && kend <= 128;
-  if (sizeof(T) == 2 && mask && kend > 128) {  // few of many keys
-    __shared__ int count;
-    if (tid == 0) count = 0;
-    __syncthreads();
-    int c = 0;
-    for (int j = tid; j < kend; j += THREADS) c += mask[j] != 0;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0 && c) atomicAdd(&count, c);
-    __syncthreads();
-    own_pass = count <= 128;
-  }
+  const bool own_pass = !one_step && sizeof(T) == 2 && kend <= 128;
   if (!one_step && !own_pass) {
     if (ntk > 0) {
       cp_wait<1>();
@@ -680,7 +667,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
   }
 
   int lim[2];
-  float ls1[2], ls2[2], d1[2], d2[2], dl[2] = {0.0f, 0.0f}, pl[2] = {0.0f, 0.0f};
+  float ls1[2], ls2[2], d1[2], d2[2];
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const int r = warp * 16 + (lane >> 2) + 8 * i, p = row0 + r;
@@ -707,125 +694,149 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < 4; j++) dq[i][j] = 0.0f;
 
-  for (int it = own_pass ? -ntk : 0; it < ntk; it++) {
-    const bool sums = it < 0;  // the pass for D alone
-    const int t = sums ? it + ntk : it;
-    if (it == 0 && own_pass) {
+  float b1[2], b2[2], sq1[2], sq2[2];  // sums of dS and of its squares
+  for (int pass = own_pass ? -1 : 0;; pass++) {
+    const bool sums = pass < 0;  // the pass for D alone
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 2; i++) b1[i] = b2[i] = sq1[i] = sq2[i] = 0.0f;
+    for (int t = 0; t < ntk; t++) {
+      if (t + 1 < ntk) {
+        load_kv(t + 1);
+        cp_wait<1>();
+      } else {
+        cp_wait<0>();
+      }
+      __syncthreads();
+      const T* k = sk + (t & 1) * F::KV_ELEMS;
+      const T* v = sv + (t & 1) * F::KV_ELEMS;
+      const uint8_t* ok = sok + (t & 1) * BN;
+      for (int s0 = 0; s0 < BN; s0 += SUB) {
+        const int j0 = t * BN + s0;
+        if (j0 >= kend) break;
+        float s1[NS][4], s2[NS][4], dp[NS][4];
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) s1[i][j] = s2[i][j] = dp[i][j] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < DH / KS; ks++) {
+          const typename FR::A q1 = FR::ldA(sq, PITCH, warp * 16, ks * KS, lane);
+          const typename FR::A q2 = FR::ldA(sq, PITCH, warp * 16, DH + ks * KS, lane);
+#pragma unroll
+          for (int nb = 0; nb < NS; nb += NSIDE) {
+            typename FR::B f[NSIDE], g[NSIDE];
+            FR::ldB_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
+            FR::ldB_nk(g, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
+            FR::mma(s1 + nb, q1, f, s2 + nb, q2, g);
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < W / KS; ks++) {
+          const typename FR::A g = FR::ldA(sdo, PITCH, warp * 16, ks * KS, lane);
+#pragma unroll
+          for (int nb = 0; nb < NS; nb += NSIDE) {
+            typename FR::B f[NSIDE];
+            FR::ldB_nk(f, v, PITCH, s0 + nb * 8, ks * KS, lane);
+            FR::mma(dp + nb, g, f);
+          }
+        }
+        const bool edge = mask != nullptr || j0 + SUB > full;
+#pragma unroll
+        for (int nb = 0; nb < NS; nb++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float x = ex2(s1[nb][e] * a.slog2 - ls1[e >> 1]), y = ex2(s2[nb][e] * a.slog2 - ls2[e >> 1]);
+            if (edge) {
+              const int c = nb * 8 + 2 * (lane & 3) + (e & 1);
+              if (j0 + c >= lim[e >> 1] || (mask && !ok[s0 + c])) x = y = 0.0f;
+            }
+            s1[nb][e] = x;
+            s2[nb][e] = y;
+            if (sums) {
+              d1[e >> 1] += x * dp[nb][e];
+              d2[e >> 1] += y * dp[nb][e];
+            }
+          }
+        if (sums) continue;
+        if (one_step) {
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            float x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (int nb = 0; nb < NS; nb++) {
+              x += s1[nb][2 * i] * dp[nb][2 * i] + s1[nb][2 * i + 1] * dp[nb][2 * i + 1];
+              y += s2[nb][2 * i] * dp[nb][2 * i] + s2[nb][2 * i + 1] * dp[nb][2 * i + 1];
+            }
+            d1[i] = quad_sum(x);
+            d2[i] = quad_sum(y);
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NS; nb++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int i = e >> 1;
+            const float x = s1[nb][e] * (dp[nb][e] - d1[i]), y = s2[nb][e] * (dp[nb][e] - d2[i]);
+            s1[nb][e] = x;
+            s2[nb][e] = y;
+            b1[i] += x;
+            b2[i] += y;
+            if (sizeof(T) == 2) {
+              sq1[i] += x * x;
+              sq2[i] += y * y;
+            }
+          }
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          typename FR::A ds[SUB / KS];
+#pragma unroll
+          for (int ks = 0; ks < SUB / KS; ks++) ds[ks] = m ? FR::from_acc(s2, ks) : FR::from_acc(s1, ks);
+#pragma unroll
+          for (int nb = m * NB / 2; nb < (m + 1) * NB / 2; nb += G::HALF_SIDE) {
+            float x[G::HALF_SIDE][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < SUB / KS; ks++) {
+              typename FR::B f[G::HALF_SIDE];
+              FR::ldB_kn(f, k, PITCH, s0 + ks * KS, nb * 8, lane);
+              FR::mma(x, ds[ks], f);
+            }
+#pragma unroll
+            for (int i = 0; i < G::HALF_SIDE; i++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) dq[nb + i][e] += x[i][e];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      if (sums) {
         d1[i] = quad_sum(d1[i]);
         d2[i] = quad_sum(d2[i]);
+        continue;
       }
-      load_kv(0);
+      b1[i] = quad_sum(b1[i]);
+      b2[i] = quad_sum(b2[i]);
+      sq1[i] = quad_sum(sq1[i]);  // all lanes take part, so not within the condition
+      sq2[i] = quad_sum(sq2[i]);
+      far |= too_far(b1[i], sq1[i]) || too_far(b2[i], sq2[i]);
+      // a map that has no key has no D either
+      d1[i] = ls1[i] == CUDART_INF_F ? 0.0f : d1[i] + b1[i];
+      d2[i] = ls2[i] == CUDART_INF_F ? 0.0f : d2[i] + b2[i];
     }
-    if (t + 1 < ntk) {
-      load_kv(t + 1);
-      cp_wait<1>();
-    } else {
-      cp_wait<0>();
-    }
-    __syncthreads();
-    const T* k = sk + (t & 1) * F::KV_ELEMS;
-    const T* v = sv + (t & 1) * F::KV_ELEMS;
-    const uint8_t* ok = sok + (t & 1) * BN;
-    for (int s0 = 0; s0 < BN; s0 += SUB) {
-      const int j0 = t * BN + s0;
-      if (j0 >= kend) break;
-      float s1[NS][4], s2[NS][4], dp[NS][4];
+    if (!sums && (sizeof(T) == 4 || one_step || own_pass || pass > 0 || !__syncthreads_or(far))) break;
 #pragma unroll
-      for (int i = 0; i < NS; i++)
+    for (int i = 0; i < NB; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) s1[i][j] = s2[i][j] = dp[i][j] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < DH / KS; ks++) {
-        const typename FR::A q1 = FR::ldA(sq, PITCH, warp * 16, ks * KS, lane);
-        const typename FR::A q2 = FR::ldA(sq, PITCH, warp * 16, DH + ks * KS, lane);
-#pragma unroll
-        for (int nb = 0; nb < NS; nb += NSIDE) {
-          typename FR::B f[NSIDE], g[NSIDE];
-          FR::ldB_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::ldB_nk(g, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma(s1 + nb, q1, f, s2 + nb, q2, g);
-        }
-      }
-#pragma unroll
-      for (int ks = 0; ks < W / KS; ks++) {
-        const typename FR::A g = FR::ldA(sdo, PITCH, warp * 16, ks * KS, lane);
-#pragma unroll
-        for (int nb = 0; nb < NS; nb += NSIDE) {
-          typename FR::B f[NSIDE];
-          FR::ldB_nk(f, v, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma(dp + nb, g, f);
-        }
-      }
-      const bool edge = mask != nullptr || j0 + SUB > full;
-#pragma unroll
-      for (int nb = 0; nb < NS; nb++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float x = ex2(s1[nb][e] * a.slog2 - ls1[e >> 1]), y = ex2(s2[nb][e] * a.slog2 - ls2[e >> 1]);
-          if (edge) {
-            const int c = nb * 8 + 2 * (lane & 3) + (e & 1);
-            if (j0 + c >= lim[e >> 1] || (mask && !ok[s0 + c])) x = y = 0.0f;
-          }
-          s1[nb][e] = x;
-          s2[nb][e] = y;
-          if (sums) {
-            d1[e >> 1] += x * dp[nb][e];
-            d2[e >> 1] += y * dp[nb][e];
-          } else {
-            dl[e >> 1] += y * dp[nb][e];
-            pl[e >> 1] += y;
-          }
-        }
-      if (sums) continue;
-      if (one_step) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          float x = 0.0f;
-#pragma unroll
-          for (int nb = 0; nb < NS; nb++) x += s1[nb][2 * i] * dp[nb][2 * i] + s1[nb][2 * i + 1] * dp[nb][2 * i + 1];
-          d1[i] = quad_sum(x);
-          d2[i] = quad_sum(dl[i]);
-        }
-      }
-#pragma unroll
-      for (int nb = 0; nb < NS; nb++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          s1[nb][e] *= dp[nb][e] - d1[e >> 1];
-          s2[nb][e] *= dp[nb][e] - d2[e >> 1];
-        }
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        typename FR::A ds[SUB / KS];
-#pragma unroll
-        for (int ks = 0; ks < SUB / KS; ks++) ds[ks] = m ? FR::from_acc(s2, ks) : FR::from_acc(s1, ks);
-#pragma unroll
-        for (int nb = m * NB / 2; nb < (m + 1) * NB / 2; nb += G::HALF_SIDE) {
-          float x[G::HALF_SIDE][4] = {};
-#pragma unroll
-          for (int ks = 0; ks < SUB / KS; ks++) {
-            typename FR::B f[G::HALF_SIDE];
-            FR::ldB_kn(f, k, PITCH, s0 + ks * KS, nb * 8, lane);
-            FR::mma(x, ds[ks], f);
-          }
-#pragma unroll
-          for (int i = 0; i < G::HALF_SIDE; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) dq[nb + i][e] += x[i][e];
-        }
-      }
-    }
-    __syncthreads();
+      for (int j = 0; j < 4; j++) dq[i][j] = 0.0f;
+    if (ntk > 0) load_kv(0);
   }
   cp_wait<0>();
 
 #pragma unroll
   for (int h = 0; h < 2; h++) {
-    // over the map's own sum: what the log-sum's rounding does to a whole row cancels
-    const float whole = quad_sum(pl[h]), part = quad_sum(dl[h]);
-    const float sum = whole == 0.0f ? 0.0f : part / whole;
     const int p = row0 + warp * 16 + (lane >> 2) + 8 * h;
     if (p >= rows) continue;
     const int e = p / a.tq, i = p - e * a.tq;
@@ -834,7 +845,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
       float* s = a.dsum + (static_cast<long long>(b) * a.h + head) * 2 * a.tq + i;
       s[0] = d1[h];
       s[a.tq] = d2[h];
-      a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] = sum;
+      a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] = d2[h];
     }
     const float f1 = a.scale, f2 = -a.scale * __ldg(a.lam + head);
     T* o = static_cast<T*>(a.dq) + b * a.dqb + head * a.dqh + i * a.dqr;

@@ -1,6 +1,6 @@
 // Differential attention backward on tcgen05: bf16, halves of 8 .. 64 columns
 // (multiples of 8).  Two kernels, as in diffattn.cu: one owns 128 queries of a
-// head (dq, D_1, D_2, the row sums of P_2 dP), one owns 128 keys of a key head
+// head (dq, D_1, D_2), one owns 128 keys of a key head
 // (dk, dv).  Both form scores and dP = do v^T anew, 64 columns at a time, and
 // both are bound by the exponentials and the tensor cores about alike.
 //
@@ -10,8 +10,8 @@
 // log-sums and D).  Two warps issue MMAs, 17 the products with dS and dP, 18 the
 // scores: an issuing warp stalls while the tensor cores are busy, and one warp
 // alone left them idle at each of its waits.  Measured: 1 x 8192 x 8192, 8 heads
-// of 64: 1116 us for both, 0.62 PF/s of the formula's products (1850 clocks a
-// tile in the queries' kernel, 2220 in the keys').  Warp 19 clears what is masked or
+// of 64: 1176 us for both, 0.59 PF/s of the formula's products (about 2000 clocks
+// a tile in the queries' kernel, 2220 in the keys').  Warp 19 clears what is masked or
 // lies beyond a sequence's length (queries' kernel) or sums dlam (keys' kernel).
 #include <algorithm>
 #include <cmath>
@@ -63,12 +63,12 @@ constexpr int Q_STAGES = 4;
 constexpr uint32_t Q_STAGE = 4 * SMALL;  // k halves, v parts
 struct QShared {
   uint64_t q_full, kv_full[Q_STAGES], kv_empty[Q_STAGES], landed[Q_STAGES], s_full[2], s_free[2], d_full[2], p_full[2];
-  uint64_t o_full, drain[2];
+  uint64_t o_full[2], decided, drain[2];
   uint32_t tmem;
   int abort_flag;
+  int again;             // whether the tiles are gone over once more
   uint2 seen[Q_STAGES];  // masked calls: which keys of a tile count
-  int count;             // and how many of all
-  float2 part[4][ROWS];
+  float4 part[4][ROWS];
 };
 constexpr size_t Q_SMEM = 1024 + 4 * BIG + Q_STAGES * Q_STAGE + sizeof(QShared);
 
@@ -94,10 +94,12 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
   // tiles from clear0 on have hidden keys and values to be cleared, as in the forward pass
   const uint8_t* mask = MASK ? a.kmask + b * a.kmb : nullptr;
   const int clear0 = MASK ? 0 : nt > 0 && nt * COLS > len && len < a.tk ? nt - 1 : nt;
-  auto clears = [&](int t) { return t >= clear0 && clear0 > 0 ? 0u : static_cast<uint32_t>(t / Q_STAGES) & 1u; };
-  // Where a mask leaves few keys of many, their D comes from a pass of its own
-  // over the tiles: step t is tile t - lead_in, or t while t < lead_in.
-  int lead_in = 0;
+  // Step t is tile t, or t - nt the second time over the tiles.  Phase of a step's arrival for the clearing
+  // warp: the stage's uses so far, which without a mask are the last tile's alone.
+  auto clears = [&](int t) {
+    return MASK ? static_cast<uint32_t>(t / Q_STAGES) & 1u : t >= nt && nt % Q_STAGES == 0 ? 1u : 0u;
+  };
+  auto cleared = [&](int t) { return (t < nt ? t : t - nt) >= clear0; };
   const int wide = 2 * a.dh > 64 ? 2 : 1, ksteps = (a.dh + 15) / 16, dsteps = a.dh / 8;
 
   if (tid == 0) {
@@ -113,11 +115,12 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       mbar_init(&sh.d_full[i], 1);
       mbar_init(&sh.p_full[i], 8);
     }
-    mbar_init(&sh.o_full, 1);
+    mbar_init(&sh.o_full[0], 1);
+    mbar_init(&sh.o_full[1], 1);
+    mbar_init(&sh.decided, SOFT);
     mbar_init(&sh.drain[0], 1);
     mbar_init(&sh.drain[1], 1);
-    sh.abort_flag = 0;
-    if (MASK) sh.count = 0;
+    sh.abort_flag = sh.again = 0;
     fence_barrier_init();
   }
   if (warp == WARP_MMA) {
@@ -128,15 +131,12 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  if (MASK && nt > 2) {
-    int c = 0;
-    for (int j = tid; j < kend; j += THREADS) c += mask[j] != 0;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0 && c) atomicAdd(&sh.count, c);
-    __syncthreads();
-    if (sh.count <= 128) lead_in = nt;
-  }
-  const int steps = nt + lead_in;
+  // Whether to go over the tiles `pass` times and once more (a row of at most two tiles has its D from P dP).
+  auto goes_on = [&](int pass) {
+    if (pass == 0) return nt > 0;
+    return pass == 1 && nt > 2 && wait(&sh.decided, 0, abort_flag, dev_error) &&
+           *static_cast<volatile int*>(&sh.again) != 0;
+  };
 
   // registers: 640 threads x 96 at launch = 512 x 104 + 128 x 64
   if (warp < SOFT) {
@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
     // which of this thread's 32 keys of step t count
     auto counts = [&](int t) { return !MASK ? 0xffffffffu : half ? sh.seen[t % Q_STAGES].y : sh.seen[t % Q_STAGES].x; };
 
-    // D_1 and D_2: from o and o2, or, where a row sees at most two tiles, from
-    // P dP itself (see diffattn.cu on what their rounding does to short rows).
+    // D_1 and D_2: from o and o2 (too_far() on what their rounding does), or, where a
+    // row sees at most two tiles, from P dP itself.
     float d1 = 0.0f, d2 = 0.0f;
-    if (nt > 2 && lead_in == 0) {
+    if (nt > 2) {
       if (in) {
         const int c0 = k4 * (a.dh / 2);
         const __nv_bfloat16* po = static_cast<const __nv_bfloat16*>(a.fo) + b * a.ob + head * a.oh + i * a.orow + c0;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
           }
         }
       }
-    } else if (lead_in == 0 && team < nt) {
+    } else if (team < nt) {
       warp_wait(&sh.kv_full[team], 0, abort_flag, dev_error);
       warp_wait(&sh.s_full[team], 0, abort_flag, dev_error);
       warp_wait(&sh.d_full[team], 0, abort_flag, dev_error);
@@ -224,115 +224,111 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
         }
       }
     }
-    f32x2 e1, e2;  // -D_1, -D_2
-    // sums the row's four shares of D
-    auto settle_d = [&] {
-      sh.part[k4][row] = make_float2(d1, d2);
+    // a row's sum of its four threads' shares
+    auto row_sum = [&](float4 mine) {
+      sh.part[k4][row] = mine;
       soft_sync();
-      d1 = d2 = 0.0f;
+      float4 s = sh.part[0][row];
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        d1 += sh.part[k][row].x;
-        d2 += sh.part[k][row].y;
-      }
-      if (in && k4 == 0) {
-        a.dsum[stat] = d1;
-        a.dsum[stat + a.tq] = d2;
+      for (int k = 1; k < 4; k++) {
+        const float4 x = sh.part[k][row];
+        s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
       }
       soft_sync();
-      e1 = pair(-d1, -d1);
-      e2 = pair(-d2, -d2);
+      return s;
     };
-    if (lead_in == 0) settle_d();
-    f32x2 dl = 0ull, pl = 0ull;
-    bool settled = lead_in == 0;
-    for (int t = team; t < steps; t += 2) {
-      const uint32_t par = (t >> 1) & 1;
-      const int j = t < lead_in ? t : t - lead_in;
-      if (MASK && !settled && t >= lead_in) {
-        settle_d();
-        settled = true;
-      }
-      bool edge = j * COLS + 32 > full;
-      uint32_t seen = 0xffffffffu;
-      if (MASK) {  // from the clearing warp
-        if (!warp_wait(&sh.kv_full[t % Q_STAGES], (t / Q_STAGES) & 1, abort_flag, dev_error)) break;
-        seen = counts(t);
-        edge |= seen != 0xffffffffu;
-      }
-      float x[2][16], y[2][16];
-      if (!warp_wait(&sh.s_full[team], par, abort_flag, dev_error)) break;
-      tc_fence_after();
+    const float4 d = row_sum(make_float4(d1, d2, 0.0f, 0.0f));
+    f32x2 e1 = pair(-d.x, -d.x), e2 = pair(-d.y, -d.y);  // -D_1, -D_2
+    int pass = 0;
+    for (;; pass++) {
+      // sums of dS and of its squares
+      f32x2 b1 = 0ull, b2 = 0ull, sq1 = 0ull, sq2 = 0ull;
+      for (int t = pass * nt + ((team + pass * nt) & 1); t < (pass + 1) * nt; t += 2) {
+        const uint32_t par = (t >> 1) & 1;
+        const int j = t - pass * nt;
+        bool edge = j * COLS + 32 > full;
+        uint32_t seen = 0xffffffffu;
+        if (MASK) {  // from the clearing warp
+          if (!warp_wait(&sh.kv_full[t % Q_STAGES], (t / Q_STAGES) & 1, abort_flag, dev_error)) break;
+          seen = counts(t);
+          edge |= seen != 0xffffffffu;
+        }
+        float x[2][16], y[2][16];
+        if (!warp_wait(&sh.s_full[team], par, abort_flag, dev_error)) break;
+        tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 2; c++) maps(ts + c * 16, x[c], y[c], lim - j * COLS - c * 16, edge, seen >> (c * 16));
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.s_free[team]);
-      if (!warp_wait(&sh.d_full[team], par, abort_flag, dev_error)) break;
-      tc_fence_after();
-      if (MASK && t < lead_in) {
+        for (int c = 0; c < 2; c++) maps(ts + c * 16, x[c], y[c], lim - j * COLS - c * 16, edge, seen >> (c * 16));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.s_free[team]);
+        if (!warp_wait(&sh.d_full[team], par, abort_flag, dev_error)) break;
+        tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          float dp[16];
-          tmem_ld(ts + 128 + c * 16, dp);
-          tmem_landed(dp);
+          uint32_t u[8], v[8];
 #pragma unroll
-          for (int e = 0; e < 16; e++) {
-            d1 += x[c][e] * dp[e];
-            d2 += y[c][e] * dp[e];
+          for (int h = 0; h < 2; h++) {
+            float dp[8];
+            tmem_ld(ts + 128 + c * 16 + h * 8, dp);
+            tmem_landed(dp);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int k = h * 4 + e;
+              const f32x2 g = pair(dp[2 * e], dp[2 * e + 1]);
+              const f32x2 s1 = mul2(pair(x[c][2 * k], x[c][2 * k + 1]), add2(g, e1));
+              const f32x2 s2 = mul2(pair(y[c][2 * k], y[c][2 * k + 1]), add2(g, e2));
+              unpair(s1, x[c][2 * k], x[c][2 * k + 1]);
+              u[k] = pack2(x[c][2 * k], x[c][2 * k + 1]);
+              unpair(s2, y[c][2 * k], y[c][2 * k + 1]);
+              v[k] = pack2(y[c][2 * k], y[c][2 * k + 1]);
+            }
           }
+          tmem_st(ts + 128 + c * 16, u);
+          tmem_st(ts + 128 + c * 16 + 8, v);
         }
+        tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_full[team]);
-        continue;
-      }
+        // under the products with this tile's dS, which others wait for
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        uint32_t u[8], v[8];
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float dp[8];
-          tmem_ld(ts + 128 + c * 16 + h * 8, dp);
-          tmem_landed(dp);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int k = h * 4 + e;
-            const f32x2 g = pair(dp[2 * e], dp[2 * e + 1]), y2 = pair(y[c][2 * k], y[c][2 * k + 1]);
-            dl = fma2(y2, g, dl);
-            pl = add2(pl, y2);
-            float r0, r1;
-            unpair(mul2(pair(x[c][2 * k], x[c][2 * k + 1]), add2(g, e1)), r0, r1);
-            u[k] = pack2(r0, r1);
-            unpair(mul2(y2, add2(g, e2)), r0, r1);
-            v[k] = pack2(r0, r1);
+          for (int k = 0; k < 16; k += 2) {
+            const f32x2 s1 = pair(x[c][k], x[c][k + 1]), s2 = pair(y[c][k], y[c][k + 1]);
+            b1 = add2(b1, s1);
+            b2 = add2(b2, s2);
+            sq1 = fma2(s1, s1, sq1);
+            sq2 = fma2(s2, s2, sq2);
           }
-        }
-        tmem_st(ts + 128 + c * 16, u);
-        tmem_st(ts + 128 + c * 16 + 8, v);
       }
-      tmem_wait_st();
-      tc_fence_before();
+      if (pass > 0) break;
+      auto both = [](f32x2 z) {
+        float l, r;
+        unpair(z, l, r);
+        return l + r;
+      };
+      const float4 off = row_sum(make_float4(both(b1), both(b2), both(sq1), both(sq2)));
+      // a map that has no key has no D either
+      const float D1 = ls1 == CUDART_INF_F ? 0.0f : d.x + off.x, D2 = ls2 == CUDART_INF_F ? 0.0f : d.y + off.y;
+      if (in && k4 == 0) {
+        a.dsum[stat] = D1;
+        a.dsum[stat + a.tq] = D2;
+        a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] = D2;
+      }
+      if (nt <= 2) break;
+      e1 = pair(-D1, -D1);
+      e2 = pair(-D2, -D2);
+      const bool far = in && (too_far(off.x, off.z) || too_far(off.y, off.w));
+      if (__any_sync(0xffffffffu, far) && lane == 0) *static_cast<volatile int*>(&sh.again) = 1;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[team]);
-    }
-    if (MASK && !settled) settle_d();  // every soft warp does, an aborting one too
-    float l0, l1, p0, p1;
-    unpair(dl, l0, l1);
-    unpair(pl, p0, p1);
-    sh.part[k4][row] = make_float2(l0 + l1, p0 + p1);
-    soft_sync();
-    if (in && k4 == 0) {
-      // over the map's own sum: what the log-sum's rounding does to a whole row cancels
-      const float part = (sh.part[0][row].x + sh.part[1][row].x) + (sh.part[2][row].x + sh.part[3][row].x);
-      const float whole = (sh.part[0][row].y + sh.part[1][row].y) + (sh.part[2][row].y + sh.part[3][row].y);
-      a.dlrow[static_cast<long long>(head) * a.n * a.tq + static_cast<long long>(b) * a.tq + i] =
-          whole == 0.0f ? 0.0f : part / whole;
+      if (lane == 0) mbar_arrive(&sh.decided);
+      if (!__all_sync(0xffffffffu, goes_on(1))) break;
     }
 
     bool ok = true;
     if (nt > 0) {
-      ok = warp_wait(&sh.o_full, 0, abort_flag, dev_error);
+      ok = warp_wait(&sh.o_full[pass], 0, abort_flag, dev_error);
       tc_fence_after();
     }
     __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.dq) + b * a.dqb + head * a.dqh + i * a.dqr;
@@ -356,12 +352,12 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
         for (int h = 0; h < 2; h++) tma_5d(sq + h * BIG, &p.q, 0, h, head, i0, b, &sh.q_full);
         for (int c = 0; c < wide; c++) tma_5d(sg + c * BIG, &p.g, c * 64, 0, head, i0, b, &sh.q_full);
         int t = 0;
-        for (; t < steps; t++) {
-          const int st = t % Q_STAGES, j = t < lead_in ? t : t - lead_in;
+        for (; t < nt || (t < 2 * nt && goes_on(1)); t++) {
+          const int st = t % Q_STAGES, j = t < nt ? t : t - nt;
           if (t >= Q_STAGES && !wait(&sh.kv_empty[st], (t / Q_STAGES - 1) & 1, abort_flag, dev_error)) break;
           const uint32_t dst = skv + st * Q_STAGE;
           // a tile to be cleared lands for the clearing warp, which passes it on
-          uint64_t* bar = t >= clear0 ? &sh.landed[st] : &sh.kv_full[st];
+          uint64_t* bar = cleared(t) ? &sh.landed[st] : &sh.kv_full[st];
           mbar_arrive_expect_tx(bar, (2 + wide) * SMALL);
           for (int h = 0; h < 2; h++) tma_5d(dst + h * SMALL, &p.k, 0, h, kvh, j * COLS, b, bar);
           for (int c = 0; c < wide; c++) tma_5d(dst + (2 + c) * SMALL, &p.v, c * 64, 0, kvh, j * COLS, b, bar);
@@ -369,22 +365,25 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
         // what was asked for lands before the block may end, aborting or not
         settle(&sh.q_full, 0);
         for (int i = max(0, t - Q_STAGES); i < t; i++)
-          settle(i >= clear0 ? &sh.landed[i % Q_STAGES] : &sh.kv_full[i % Q_STAGES], clears(i));
+          if (cleared(i)) settle(&sh.landed[i % Q_STAGES], clears(i));
+          else settle(&sh.kv_full[i % Q_STAGES], (i / Q_STAGES) & 1);
       }
       __syncwarp();
     } else if (warp == WARP_AUX) {
       Seen keys;
-      if (clear0 < nt) keys.load(mask, clear0 * COLS, len);
-      for (int t = clear0; t < steps; t++) {
-        const int st = t % Q_STAGES, next = t + 1 < lead_in ? t + 1 : t + 1 - lead_in;
-        const uint2 seen = keys.bits();
-        if (t + 1 < steps) keys.load(mask, next * COLS, len);
-        if (!warp_wait(&sh.landed[st], clears(t), abort_flag, dev_error)) break;
-        clear_hidden(base + 4 * BIG + st * Q_STAGE, seen, 2 + wide);
-        if (lane == 0) sh.seen[st] = seen;
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.kv_full[st]);
+      for (int pass = 0; clear0 < nt && __all_sync(0xffffffffu, goes_on(pass)); pass++) {
+        keys.load(mask, clear0 * COLS, len);
+        for (int j = clear0; j < nt; j++) {
+          const int t = pass * nt + j, st = t % Q_STAGES;
+          const uint2 seen = keys.bits();
+          if (j + 1 < nt) keys.load(mask, (j + 1) * COLS, len);
+          if (!warp_wait(&sh.landed[st], clears(t), abort_flag, dev_error)) break;
+          clear_hidden(base + 4 * BIG + st * Q_STAGE, seen, 2 + wide);
+          if (lane == 0) sh.seen[st] = seen;
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.kv_full[st]);
+        }
       }
     } else if (nt > 0) {
       const uint32_t lead = elect_one() ? 1u : 0u;
@@ -395,8 +394,8 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
       int st = 0;
       if (warp == WARP_SCORE) {
         const uint64_t dq = desc_k(sq), dkv = desc_k(skv);
-        for (int j = 0; ok && j < steps; j++) {
-          // the team has the scores of tile j - 2 in registers
+        for (int j = 0; ok && (j < nt || (j < 2 * nt && __all_sync(0xffffffffu, goes_on(1)))); j++) {
+          // the team has the scores of step j - 2 in registers
           if (!(ok = landed(j, st) && (j < 2 || done(&sh.s_free[j & 1], ((j >> 1) - 1) & 1)))) break;
           tc_fence_after();
           const uint64_t kv = dkv + st * (Q_STAGE / 16);
@@ -425,31 +424,33 @@ __global__ void __launch_bounds__(THREADS, 1) tc_bwd_q_kernel(const __grid_const
                      kv + ((2 + (ks >> 2)) * SMALL + (ks & 3) * 32) / 16, id_s, ks > 0, lead);
           commit(&sh.d_full[j & 1], lead);
         };
-        for (int j = 0; ok && j < min(steps, 2); j++)
-          if ((ok = landed(j, j))) {
+        for (int pass = 0; ok && __all_sync(0xffffffffu, goes_on(pass)); pass++) {
+          const int first = pass * nt, last = first + nt;
+          for (int j = first; ok && j < min(first + 2, last); j++)
+            if ((ok = landed(j, j % Q_STAGES))) {
+              tc_fence_after();
+              slopes(j, j % Q_STAGES);
+            }
+          st = first % Q_STAGES;
+          int st2 = (first + 2) % Q_STAGES;
+          for (int j = first; ok && j < last; j++) {
+            if (!(ok = (j + 2 >= last || landed(j + 2, st2)) && done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
             tc_fence_after();
-            slopes(j, j);
-          }
-        int st2 = 2;
-        for (int j = 0; ok && j < steps; j++) {
-          if (!(ok = (j + 2 >= steps || landed(j + 2, st2)) && done(&sh.p_full[j & 1], (j >> 1) & 1))) break;
-          tc_fence_after();
-          const uint64_t k = dmn + st * (Q_STAGE / 16);
-          const uint32_t s = tmem + 256 + (j & 1) * 192;
-          if (!MASK || j >= lead_in) {
+            const uint64_t k = dmn + st * (Q_STAGE / 16);
+            const uint32_t s = tmem + 256 + (j & 1) * 192;
 #pragma unroll
             for (int m = 0; m < 2; m++)
 #pragma unroll
               for (int ks = 0; ks < 4; ks++)
-                mma_ts(tmem + m * 64, s + ks * 16 + m * 8, k + (m * SMALL + ks * 2048) / 16, id_o, j > lead_in || ks > 0,
+                mma_ts(tmem + m * 64, s + ks * 16 + m * 8, k + (m * SMALL + ks * 2048) / 16, id_o, j > first || ks > 0,
                        lead);
+            // the scores of step j are long done: dS came of them
+            commit(&sh.kv_empty[st], lead);
+            if (j + 1 == last) commit(&sh.o_full[pass], lead);
+            if (j + 2 < last) slopes(j + 2, st2);
+            if (++st == Q_STAGES) st = 0;
+            if (++st2 == Q_STAGES) st2 = 0;
           }
-          // the scores of tile j are long done: dS came of them
-          commit(&sh.kv_empty[st], lead);
-          if (j + 1 == steps) commit(&sh.o_full, lead);
-          if (j + 2 < steps) slopes(j + 2, st2);
-          if (++st == Q_STAGES) st = 0;
-          if (++st2 == Q_STAGES) st2 = 0;
         }
       }
       if (!ok) {  // no MMA may write tensor memory after it is released
