@@ -303,9 +303,10 @@ int rnn_hint_mse_dev(rnn_ctx *ctx, const float *pred, const float *target,
  *   y_i = x_i cos - x_j sin,  y_j = x_i sin + x_j cos,
  * (i, j) = (p, p + total), or (2p, 2p + 1) when interleaved.  Columns from
  * 2*total on are copied.  backward != 0 turns by the negative angle: the
- * gradient of x from that of y.  Angles are exact to f32 at any position;
- * the rotation is f32, rounded once to dtype.  y may be x with the same
- * strides; otherwise they must not share elements. */
+ * gradient of x from that of y.  Angles are exact to f32 at any position and
+ * frequency (below 2^20 radians a step); the rotation is f32, rounded once to
+ * dtype.  y may be x with the same strides; otherwise they must not share
+ * elements. */
 int rnn_rope_dev(rnn_ctx *ctx, int dtype, const void *x, long long xrow,
                  long long xhead, int rows, int heads, int dh,
                  const int32_t *pos, int axes, const int *pairs,
