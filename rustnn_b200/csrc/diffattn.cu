@@ -1087,7 +1087,7 @@ int fwd_launch(rnn_ctx* ctx, Args a) {
   const long long rows = static_cast<long long>(a.grp) * a.tq;
   const long long nbh = static_cast<long long>(a.n) * a.hkv;
   const long long blocks = (rows + F::ROWS - 1) / F::ROWS * nbh;
-  RNN_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  RNN_REQUIRE(blocks < (1ll << 31), "diffattn: too many rows");
   static std::atomic<unsigned long long> optin{0};
   RNN_TRY(tc::ensure_smem_optin(fwd_kernel<T, DH, RW>, optin, ctx->device, static_cast<int>(F::SMEM)));
   // Split the keys when the rows alone do not give every SM a block: in parts of
@@ -1137,7 +1137,7 @@ int bwd_launch(rnn_ctx* ctx, Args a) {
   const long long rows = static_cast<long long>(a.grp) * a.tq, nbh = static_cast<long long>(a.n) * a.hkv;
   const long long qblocks = (rows + FQ::ROWS - 1) / FQ::ROWS * nbh;
   const long long kblocks = std::max<long long>((a.tk + FK::KEYS - 1ll) / FK::KEYS * nbh, a.h);
-  RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31), "diffattn: too many rows");
   static std::atomic<unsigned long long> optin_q{0}, optin_kv{0};
   RNN_TRY(tc::ensure_smem_optin(bwd_q_kernel<T, DH>, optin_q, ctx->device, static_cast<int>(FQ::SMEM)));
   RNN_TRY(tc::ensure_smem_optin(bwd_kv_kernel<T, DH>, optin_kv, ctx->device, static_cast<int>(FK::SMEM)));
@@ -1190,7 +1190,9 @@ int fill(rnn_ctx* ctx, const rnn_diffattn* d, const void* q, const void* k, cons
               "diffattn: bad shape n=%d tq=%d tk=%d h=%d hkv=%d", d->n, d->tq, d->tk, d->h, d->hkv);
   RNN_REQUIRE(d->dh >= 1, "diffattn: dh=%d", d->dh);
   if (d->dh > 64) return set_error(RNN_ERR_UNSUPPORTED, "diffattn: dh=%d, at most 64 columns a half", d->dh);
-  RNN_REQUIRE(d->n * (long long)d->hkv < (1ll << 31) && d->tk < (1 << 30) && d->tq < (1 << 30),
+  // the kernels count a (sequence, key head)'s rows in int, to the end of a block of up to 128
+  RNN_REQUIRE(d->n * (long long)d->hkv < (1ll << 31) && d->tk < (1 << 30) && d->tq < (1 << 30) &&
+                  (long long)(d->h / d->hkv) * d->tq < (1ll << 31) - 128,
               "diffattn: shape too large");
   RNN_REQUIRE(d->q_batch >= 0 && d->q_row >= 0 && d->q_head >= 0 && d->k_batch >= 0 && d->k_row >= 0 &&
                   d->k_head >= 0 && d->v_batch >= 0 && d->v_row >= 0 && d->v_head >= 0 && d->o_batch >= 0 &&

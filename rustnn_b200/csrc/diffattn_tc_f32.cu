@@ -1669,7 +1669,7 @@ int f32_tc_fwd(rnn_ctx* ctx, const Args& a) {
   p.st16_2 = reinterpret_cast<uintptr_t>(a.o2) % 16 == 0 && a.dh % 2 == 0;
   const long long rows = static_cast<long long>(a.grp) * a.tq, nbh = static_cast<long long>(a.n) * a.hkv;
   const long long blocks = (rows + ROWS - 1) / ROWS * nbh;
-  RNN_REQUIRE(blocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  RNN_REQUIRE(blocks < (1ll << 31), "diffattn: too many rows");
   const bool wide = a.dh > 32;
   const int tiles = (a.tk + COLS - 1) / COLS;
   const long long parts = std::max(1ll, std::min<long long>(ctx->num_sms / (wide ? 2 * blocks : blocks), tiles / 4));
@@ -1708,7 +1708,7 @@ int f32_tc_bwd(rnn_ctx* ctx, const Args& a) {
   const long long rows = static_cast<long long>(a.grp) * a.tq, nbh = static_cast<long long>(a.n) * a.hkv;
   const long long qblocks = (rows + ROWS - 1) / ROWS * nbh;
   const long long kblocks = std::max<long long>((a.tk + ROWS - 1ll) / ROWS * nbh, a.h);
-  RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31) && rows < (1ll << 31), "diffattn: too many rows");
+  RNN_REQUIRE(qblocks < (1ll << 31) && kblocks < (1ll << 31), "diffattn: too many rows");
   if (a.dh > 32) {
     static std::atomic<unsigned long long> optin_r{0}, optin_c{0}, optin_v{0};
     RNN_TRY(tc::ensure_smem_optin(f32_grad_kernel<false>, optin_r, ctx->device, static_cast<int>(GRAD_SMEM)));

@@ -1,0 +1,18 @@
+"""Sizes next to what the kernels' 32-bit row counts hold: refused before any launch."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_up_to_the_end_of_int(dtype):
+    """2^30 - 1 queries of two heads on one key head: 2^31 - 2 rows, whose last block would end past 2^31."""
+    from rustnn_b200 import ops
+
+    tq = (1 << 30) - 1
+    q = torch.zeros(1, 1, 1, 2, device="cuda", dtype=dtype).expand(1, tq, 2, 2)
+    k = torch.zeros(1, 1, 1, 2, device="cuda", dtype=dtype)
+    lam = torch.zeros(2, device="cuda")
+    with pytest.raises(ops.RnnError, match="too large"):
+        ops.diffattn_forward(q, k, k, lam)
