@@ -12,9 +12,9 @@
 // so no table is read.  The product pos * inv_freq (31 bits by 24) is kept whole in
 // two f64 numbers and reduced to a fraction of a turn there before sincospif, so
 // the error does not grow with position or frequency; the rotation itself is f32,
-// rounded once to the tensor's type.  Measured: 32768 x 32 x 64 bf16, 46 us, 5.8
-// TB/s of a copy's 6.55 (45 without what the product's rounding leaves); 30011 x 12
-// x 48 f32 interleaved, 26 us, 5.4 TB/s.
+// rounded once to the tensor's type.  Measured with a cold L2: 32768 x 32 x 64 bf16,
+// 49 us, 5.5 TB/s of a copy's 6.55 (48 without what the product's rounding leaves);
+// 30011 x 12 x 48 f32 interleaved, 28 us, 4.9 TB/s.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -160,7 +160,7 @@ int rope_launch(rnn_ctx* ctx, RopeArgs a) {
   rpb = std::min<long long>(rpb, (a.rows + 4ll * ctx->num_sms - 1) / (4ll * ctx->num_sms));
   rpb = std::min<long long>(rpb, std::max(1, ROPE_SMEM_PAIRS / std::max(1, a.total)));
   a.rpb = static_cast<int>(std::max<long long>(1, rpb));
-  const int grid = (a.rows + a.rpb - 1) / a.rpb;
+  const int grid = (a.rows - 1) / a.rpb + 1;
   rope_kernel<T, V, INTER>
       <<<grid, ROPE_THREADS, static_cast<size_t>(a.rpb) * a.total * sizeof(float2), ctx->stream>>>(a);
   RNN_CHECK_LAUNCH();

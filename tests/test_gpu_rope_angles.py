@@ -40,3 +40,20 @@ def test_angles_are_exact(low, high, inter):
     c, s = (y[:, 0, 0::2], y[:, 0, 1::2]) if inter else (y[:, 0, :count], y[:, 0, count:])
     assert float((c.double() - torch.cos(a)).abs().max()) < 2.0 ** -21
     assert float((s.double() - torch.sin(a)).abs().max()) < 2.0 ** -21
+
+
+def test_most_rows():
+    """2^31 - 1 rows of two columns: the launch counts its blocks without passing int."""
+    from rustnn_b200 import ops
+
+    rows = (1 << 31) - 1
+    pos = torch.zeros(rows, 1, device="cuda", dtype=torch.int32)
+    pos[-1] = 1
+    x = torch.ones(rows, 1, 2, device="cuda", dtype=torch.bfloat16)
+    y = ops.rope(x, pos, torch.ones(1, device="cuda"), (1,), out=x)
+    assert y is x and bool((y[:4] == 1).all())
+    want = torch.tensor([math.cos(1) - math.sin(1), math.cos(1) + math.sin(1)], device="cuda").bfloat16()
+    assert torch.equal(y[-1, 0], want)
+    torch.cuda.synchronize()
+    del x, y, pos
+    torch.cuda.empty_cache()
