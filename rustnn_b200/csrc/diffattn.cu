@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
     for (int s0 = kw * (BN / F::KW); s0 < (kw + 1) * (BN / F::KW); s0 += SUB) {
       const int j0 = kbeg + t * BN + s0;
       if (j0 >= kend) break;
-      float s1[NS][4], s2[NS][4];
+      float s1[NS][4], s2[NS][4], m1s[NS][4] = {}, m2s[NS][4] = {};
 #pragma unroll
       for (int i = 0; i < NS; i++)
 #pragma unroll
@@ -172,9 +172,12 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
           typename FR::B f[NSIDE], g[NSIDE];
           FR::ldB_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
           FR::ldB_nk(g, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma(s1 + nb, q1, f, s2 + nb, q2, g);
+          FR::mma(s1 + nb, m1s + nb, q1, f);
+          FR::mma(s2 + nb, m2s + nb, q2, g);
         }
       }
+      FR::join(s1, m1s);
+      FR::join(s2, m2s);
       const bool edge = mask != nullptr || j0 + SUB > full;
       float mx1[2] = {m1[0], m1[1]}, mx2[2] = {m2[0], m2[1]};
 #pragma unroll
@@ -235,13 +238,16 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(Args a) {
       // f32 addition, so long sums are not left to the MMA's own rounding
 #pragma unroll
       for (int nb = 0; nb < NB; nb += G::SIDE) {
-        float x[G::SIDE][4] = {}, y[G::SIDE][4] = {};
+        float x[G::SIDE][4] = {}, y[G::SIDE][4] = {}, xs[G::SIDE][4] = {}, ys[G::SIDE][4] = {};
 #pragma unroll
         for (int ks = 0; ks < SUB / KS; ks++) {
           typename FR::B f[G::SIDE];
           FR::ldB_kn(f, v, PITCH, s0 + ks * KS, nb * 8, lane);
-          FR::mma(x, pa[ks], f, y, pb[ks], f);
+          FR::mma(x, xs, pa[ks], f);
+          FR::mma(y, ys, pb[ks], f);
         }
+        FR::join(x, xs);
+        FR::join(y, ys);
 #pragma unroll
         for (int i = 0; i < G::SIDE; i++)
 #pragma unroll
@@ -713,7 +719,7 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
       for (int s0 = 0; s0 < BN; s0 += SUB) {
         const int j0 = t * BN + s0;
         if (j0 >= kend) break;
-        float s1[NS][4], s2[NS][4], dp[NS][4];
+        float s1[NS][4], s2[NS][4], dp[NS][4], m1[NS][4] = {}, m2[NS][4] = {}, mp[NS][4] = {};
 #pragma unroll
         for (int i = 0; i < NS; i++)
 #pragma unroll
@@ -727,7 +733,8 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
             typename FR::B f[NSIDE], g[NSIDE];
             FR::ldB_nk(f, k, PITCH, s0 + nb * 8, ks * KS, lane);
             FR::ldB_nk(g, k, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-            FR::mma(s1 + nb, q1, f, s2 + nb, q2, g);
+            FR::mma(s1 + nb, m1 + nb, q1, f);
+            FR::mma(s2 + nb, m2 + nb, q2, g);
           }
         }
 #pragma unroll
@@ -737,9 +744,12 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
           for (int nb = 0; nb < NS; nb += NSIDE) {
             typename FR::B f[NSIDE];
             FR::ldB_nk(f, v, PITCH, s0 + nb * 8, ks * KS, lane);
-            FR::mma(dp + nb, g, f);
+            FR::mma(dp + nb, mp + nb, g, f);
           }
         }
+        FR::join(s1, m1);
+        FR::join(s2, m2);
+        FR::join(dp, mp);
         const bool edge = mask != nullptr || j0 + SUB > full;
 #pragma unroll
         for (int nb = 0; nb < NS; nb++)
@@ -793,13 +803,14 @@ __global__ void __launch_bounds__(THREADS) bwd_q_kernel(Args a) {
           for (int ks = 0; ks < SUB / KS; ks++) ds[ks] = m ? FR::from_acc(s2, ks) : FR::from_acc(s1, ks);
 #pragma unroll
           for (int nb = m * NB / 2; nb < (m + 1) * NB / 2; nb += G::HALF_SIDE) {
-            float x[G::HALF_SIDE][4] = {};
+            float x[G::HALF_SIDE][4] = {}, xs[G::HALF_SIDE][4] = {};
 #pragma unroll
             for (int ks = 0; ks < SUB / KS; ks++) {
               typename FR::B f[G::HALF_SIDE];
               FR::ldB_kn(f, k, PITCH, s0 + ks * KS, nb * 8, lane);
-              FR::mma(x, ds[ks], f);
+              FR::mma(x, xs, ds[ks], f);
             }
+            FR::join(x, xs);
 #pragma unroll
             for (int i = 0; i < G::HALF_SIDE; i++)
 #pragma unroll
@@ -988,7 +999,7 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
     const float* st = sst + (t & 1) * 5 * BM;
     const float lam = __ldg(a.lam + kvh * a.grp + t / per);
     for (int s0 = 0; s0 < BM; s0 += SUB) {
-      float s1[NS][4], s2[NS][4], dp[NS][4];
+      float s1[NS][4], s2[NS][4], dp[NS][4], m1[NS][4] = {}, m2[NS][4] = {}, mp[NS][4] = {};
 #pragma unroll
       for (int i = 0; i < NS; i++)
 #pragma unroll
@@ -1002,7 +1013,8 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
           typename FR::B f[NSIDE], h[NSIDE];
           FR::ldB_nk(f, q, PITCH, s0 + nb * 8, ks * KS, lane);
           FR::ldB_nk(h, q, PITCH, s0 + nb * 8, DH + ks * KS, lane);
-          FR::mma(s1 + nb, k1, f, s2 + nb, k2, h);
+          FR::mma(s1 + nb, m1 + nb, k1, f);
+          FR::mma(s2 + nb, m2 + nb, k2, h);
         }
       }
 #pragma unroll
@@ -1012,9 +1024,12 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
         for (int nb = 0; nb < NS; nb += NSIDE) {
           typename FR::B f[NSIDE];
           FR::ldB_nk(f, g, PITCH, s0 + nb * 8, ks * KS, lane);
-          FR::mma(dp + nb, x, f);
+          FR::mma(dp + nb, mp + nb, x, f);
         }
       }
+      FR::join(s1, m1);
+      FR::join(s2, m2);
+      FR::join(dp, mp);
       // after this: s1 = dS_1, s2 = dS_2, dp = P_1 - lam P_2 (transposed)
 #pragma unroll
       for (int nb = 0; nb < NS; nb++)
@@ -1037,13 +1052,14 @@ __global__ void __launch_bounds__(THREADS) bwd_kv_kernel(Args a) {
         const T* src = m == 2 ? g : q;
 #pragma unroll
         for (int nb = (m == 1 ? NB / 2 : 0); nb < (m == 0 ? NB / 2 : NB); nb += G::HALF_SIDE) {
-          float x[G::HALF_SIDE][4] = {};
+          float x[G::HALF_SIDE][4] = {}, xs[G::HALF_SIDE][4] = {};
 #pragma unroll
           for (int ks = 0; ks < SUB / KS; ks++) {
             typename FR::B w[G::HALF_SIDE];
             FR::ldB_kn(w, src, PITCH, s0 + ks * KS, nb * 8, lane);
-            FR::mma(x, f[ks], w);
+            FR::mma(x, xs, f[ks], w);
           }
+          FR::join(x, xs);
 #pragma unroll
           for (int i = 0; i < G::HALF_SIDE; i++)
 #pragma unroll
