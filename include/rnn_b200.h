@@ -351,7 +351,8 @@ typedef struct rnn_diffattn {
  * parts).  For the backward pass, o2 (dtype, contiguous [n, tq, h, 2*dh]; P_2 v)
  * and lse (f32, [n, h, 2, tq]: log2 of each map's sum of exponentials, +inf
  * for a map of 0) are written when non-NULL, both or neither.
- * No score matrix is stored.  dh in 1 .. 64. */
+ * No score matrix is stored.  dh in 1 .. 64.  Outputs share no memory with
+ * inputs, here and below. */
 int rnn_diffattn_fwd_dev(rnn_ctx *ctx, const rnn_diffattn *d, const void *q,
                          const void *k, const void *v, const float *lambda,
                          void *o, void *o2, float *lse);

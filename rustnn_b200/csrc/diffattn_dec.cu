@@ -9,13 +9,16 @@
 //   S_m^T = k_m q_m^T,   A^T += v^T (P_1 - r P_2)^T,   B^T += v^T P_2^T,
 // so that up to 8 rows cost half of what 16-row products would and a lane's
 // accumulators all belong to two rows.  As in the other kernels (diffattn.cu on
-// A, B and r) the references change only where a slice's sums show they must;
-// no step exchanges values between lanes otherwise.
+// A, B and r) the references change only where a slice's sums show they must: each
+// slice adds its 16 keys' sums of both maps over 8 lanes for that comparison, and
+// nothing else passes between lanes.  P_1 - r P_2 and P_2 are rounded to bf16 for
+// the products with v (the tensors' own type): outputs are 2.3e-3 from the formula
+// in the mean square, of which rounding the output is 1.7e-3.
 //
 // Keys are split over blocks, several parts per resident block: sequences of
 // different lengths then balance by themselves.  Parts are joined by a second
-// kernel.  Measured: 8 sequences of up to 32768 keys, 16 heads on 4 of 64: 82 us,
-// 4.9 TB/s of a copy's 6.55, and the join 14 with a cold L2; on the kernels of
+// kernel.  Measured with a cold L2: 8 sequences of up to 32768 keys, 16 heads on 4
+// of 64: 90 us, 4.5 TB/s of a copy's 6.55, and the join 7; on the kernels of
 // mma.sync, which read a tile through all four warps, 274 together.
 #include <algorithm>
 
