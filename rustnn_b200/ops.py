@@ -288,6 +288,8 @@ def _view(t, name, dim, dtype=None, shape=None, device=None):
         raise RnnError(f"{name}: {t.dtype} on {t.device}, expected {dtype} on {device}")
     if strides[-1] != 1 and got[-1] > 1:
         raise RnnError(f"{name}: columns must be contiguous")
+    if max(got) > 0x7FFFFFFF:  # sizes are C ints, which ctypes would cut to their low 32 bits
+        raise RnnError(f"{name}: shape {tuple(got)}, more than 2^31 - 1 along an axis")
     return got, strides, t.data_ptr()
 
 
